@@ -39,7 +39,8 @@ enum llq_status {
   LLQ_ENOSPACE = 5      /* workspace too small */
 };
 
-enum llq_dtype { LLQ_F32 = 0, LLQ_F16 = 1, LLQ_BF16 = 2 };
+/* LLQ_E4M3 (1 sign, 4 exponent, 3 mantissa bits, largest 448): llq_fp8_* only. */
+enum llq_dtype { LLQ_F32 = 0, LLQ_F16 = 1, LLQ_BF16 = 2, LLQ_E4M3 = 3 };
 
 enum llq_scale_search { LLQ_SEARCH_AMAX = 0, LLQ_SEARCH_MSE = 1 };
 
@@ -311,6 +312,77 @@ int llq_fused_moe_packed_noalloc(const void* x, const int8_t* qw1, const float* 
                                  const int8_t* qw2, const float* sw2, const float* topk_w,
                                  const int32_t* topk_ids, int64_t T, int E, int H, int I, int k,
                                  int bits, int group_size, void* out, int impl, void* stream);
+
+/* ------------------------------------------------------------------------ */
+/* The layer for a few tokens.                                                */
+/* ------------------------------------------------------------------------ */
+
+/*
+ * One PACKED layer as llq_moe_few reads it.  gate_w bf16 [E, H], or NULL when
+ * the caller brings the routing; bias float32 [E] or NULL (-inf bars an
+ * expert); the packed buffers and group_size as for llq_fused_moe_packed.
+ */
+typedef struct llq_few_layer {
+  const void* gate_w;
+  const float* bias;
+  const int8_t* qw1;
+  const float* sw1;
+  const int8_t* qw2;
+  const float* sw2;
+  int32_t E, H, I, k, bits, group_size, renormalize;
+} llq_few_layer;
+
+/*
+ * The routed layer of llq_moe_block_packed (gate_w given: topk_w and topk_ids
+ * are written) or of llq_fused_moe_packed (gate_w NULL: they are read) for at
+ * most 32 tokens, in two launches.  W = q * s in fp32 without the bf16
+ * rounding of each weight, router logits and h kept in fp32 accuracy, one
+ * rounding of the result: close to, and more exact than, the calls for many
+ * tokens, which round logits, weights and h to bf16.  logits float32 [T, E]
+ * or NULL.  Ids outside [0, E) contribute nothing (experts of other ranks); an
+ * expert that appears twice in a token counts with the sum of its weights.
+ * T <= 32, E <= 256, k <= 32, H and I in multiples of 32 up to 32768, a group
+ * size in multiples of 128 or one scale per row (others: LLQ_EUNSUPPORTED).
+ * workspace: llq_moe_few_workspace_size bytes, of this call alone until it is
+ * done on the stream.
+ */
+size_t llq_moe_few_workspace_size(int64_t T, int k, int I);
+int llq_moe_few(const llq_few_layer* layer, const void* x, int64_t T, float* logits, float* topk_w,
+                int32_t* topk_ids, void* out, void* workspace, size_t workspace_bytes,
+                void* stream);
+
+/* ------------------------------------------------------------------------ */
+/* 8-bit floating point (e4m3) with a scale per block of 128.                 */
+/* ------------------------------------------------------------------------ */
+
+/*
+ * x [M, K] (row stride ldx elements) to e4m3: block_rows == 1 gives one scale
+ * per 128 values of a row, block_rows == 128 one per 128 x 128 block; the last
+ * block of a row or column may be short.  amax = max(|x| of the block,
+ * 448 * 2^-60); scale [ceil(M / block_rows), ceil(K / 128)] = amax / 448; code =
+ * nearest e4m3 (ties to even) to x * 448 / amax.  A NaN or an infinity makes
+ * its block's products NaN.  codes: row pitch ldc bytes, base and pitch
+ * multiples of 16; bytes past K are not written.
+ */
+int llq_fp8_quantize(const void* x, int x_dtype, int64_t M, int64_t K, int64_t ldx, int block_rows,
+                     uint8_t* codes, int64_t ldc, float* scale, void* stream);
+
+/*
+ * out[m, n] = sum over blocks g of x_scale[m, g] * w_scale[n / 128, g] *
+ * sum_{k in g} x[m, k] * w[n, k]  (+ bias[n]), fp32 sums, one rounding to
+ * out_dtype.  x: e4m3 codes with x_scale [M, G] (x_dtype LLQ_E4M3), or fp32,
+ * fp16 or bf16 values, which are quantized as by llq_fp8_quantize with
+ * block_rows == 1.  w e4m3 [N, K] with w_scale [ceil(N / 128), G] from
+ * block_rows == 128; bias [N] of out_dtype or NULL.  Row strides ldx (elements)
+ * and ldw; e4m3 operands need 16-byte aligned bases and pitches.  K a multiple
+ * of 16.  The products of two scales and their sums must stay finite in fp32.
+ * workspace: llq_fp8_linear_workspace_size bytes (may be 0 and NULL), of this
+ * call alone until it is done on the stream.
+ */
+size_t llq_fp8_linear_workspace_size(int64_t M, int K, int N, int x_dtype);
+int llq_fp8_linear(const void* x, int x_dtype, const float* x_scale, int64_t M, int K, int64_t ldx,
+                   const uint8_t* w, const float* w_scale, int N, int64_t ldw, const void* bias,
+                   void* out, int out_dtype, void* workspace, size_t workspace_bytes, void* stream);
 
 /*
  * Device error word written by bounded waits inside the tcgen05 kernels

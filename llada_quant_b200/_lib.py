@@ -9,19 +9,27 @@ from __future__ import annotations
 
 import ctypes
 import os
-from ctypes import c_double, c_int, c_int64, c_size_t, c_void_p
+from ctypes import byref, c_double, c_int, c_int64, c_size_t, c_void_p  # noqa: F401
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libllada_quant_cuda.so")
 
 LLQ_OK, LLQ_EINVAL, LLQ_EUNSUPPORTED, LLQ_ECUDA, LLQ_ETIMEOUT, LLQ_ENOSPACE = range(6)
-LLQ_F32, LLQ_F16, LLQ_BF16 = 0, 1, 2
+LLQ_F32, LLQ_F16, LLQ_BF16, LLQ_E4M3 = 0, 1, 2, 3
 LLQ_SEARCH_AMAX, LLQ_SEARCH_MSE = 0, 1
 LLQ_GEMM_AUTO, LLQ_GEMM_TCGEN05, LLQ_GEMM_SIMT, LLQ_GEMM_TCGEN05_FAST = 0, 1, 2, 3
 
 P = c_void_p
 I = c_int
 L = c_int64
+
+
+class FewLayer(ctypes.Structure):
+    """``llq_few_layer`` of the header."""
+
+    _fields_ = [(n, c_void_p) for n in ("gate_w", "bias", "qw1", "sw1", "qw2", "sw2")] + [
+        (n, ctypes.c_int32) for n in ("E", "H", "I", "k", "bits", "group_size", "renormalize")]
+
 
 #: every entry point of include/llada_quant.h with its ctypes signature
 SIGNATURES = {
@@ -61,6 +69,11 @@ SIGNATURES = {
     "llq_ep_experts_workspace_size": (c_size_t, [I, I, I, I, I]),
     "llq_ep_experts": (I, [P, P, I, I, I, ctypes.c_uint32, P, P, P, P, I, I, I, I, I, L, P, c_size_t, I, P]),
     "llq_ep_combine_wait": (I, [P, I, I, I, ctypes.c_uint32, P, L, I, I, P, P]),
+    "llq_moe_few_workspace_size": (c_size_t, [L, I, I]),
+    "llq_moe_few": (I, [P, P, L, P, P, P, P, P, c_size_t, P]),
+    "llq_fp8_quantize": (I, [P, I, L, L, L, I, P, L, P, P]),
+    "llq_fp8_linear_workspace_size": (c_size_t, [L, I, I, I]),
+    "llq_fp8_linear": (I, [P, I, P, L, I, L, P, P, I, L, P, P, I, P, c_size_t, P]),
     "llq_device_error": (I, [P]),
     "llq_clear_device_error": (I, []),
 }

@@ -346,6 +346,30 @@ int llq_moe_block_packed(const void* x, const void* gate_w, const float* bias, i
   return experts_after_align(ws, x, qw1, sw1, qw2, sw2, topk_w, T, E, H, I, k, bits, group_size, out, impl, st);
 }
 
+size_t llq_moe_few_workspace_size(int64_t T, int k, int I) { return moe_few_workspace(T, k, I); }
+
+int llq_moe_few(const llq_few_layer* layer, const void* x, int64_t T, float* logits, float* topk_w,
+                int32_t* topk_ids, void* out, void* workspace, size_t workspace_bytes, void* stream) {
+  if (layer == nullptr) return fail(LLQ_EINVAL, "null layer");
+  return moe_few(*layer, x, T, logits, topk_w, topk_ids, out, workspace, workspace_bytes, as_stream(stream));
+}
+
+int llq_fp8_quantize(const void* x, int x_dtype, int64_t M, int64_t K, int64_t ldx, int block_rows, uint8_t* codes,
+                     int64_t ldc, float* scale, void* stream) {
+  return fp8_quantize(x, x_dtype, M, K, ldx, block_rows, codes, ldc, scale, as_stream(stream));
+}
+
+size_t llq_fp8_linear_workspace_size(int64_t M, int K, int N, int x_dtype) {
+  return fp8_linear_workspace(M, K, N, x_dtype);
+}
+
+int llq_fp8_linear(const void* x, int x_dtype, const float* x_scale, int64_t M, int K, int64_t ldx, const uint8_t* w,
+                   const float* w_scale, int N, int64_t ldw, const void* bias, void* out, int out_dtype,
+                   void* workspace, size_t workspace_bytes, void* stream) {
+  return fp8_linear(x, x_dtype, x_scale, M, K, ldx, w, w_scale, N, ldw, bias, out, out_dtype, workspace,
+                    workspace_bytes, as_stream(stream));
+}
+
 int llq_device_error(int32_t* code) {
   if (code == nullptr) return fail(LLQ_EINVAL, "null code pointer");
   cudaError_t e = cudaMemcpyFromSymbol(code, g_device_error, sizeof(int32_t));

@@ -1,0 +1,137 @@
+"""8-bit floating point (e4m3) with one scale per block of 128: quantizer, product, linear module.
+
+Rows carry one fp32 scale per 128 values, weights one per 128 x 128 block, and
+both operands of the product stay in 8 bits: ``out = sum over blocks of
+(row scale * weight scale) * (codes . codes)``, fp32 sums, one rounding.  It
+stands beside :class:`llada_quant_b200.linear.QuantLinear`, whose integer
+weights meet bf16 rows: :class:`Fp8Linear` reads half the bytes of bf16 and,
+with many rows, multiplies at the tensor cores' 8-bit rate.  CUDA only, no
+backward pass.
+"""
+
+from __future__ import annotations
+
+from dataclasses import dataclass
+from typing import Optional, Union
+
+import torch
+import torch.nn as nn
+
+from . import ops
+
+BLOCK = ops.FP8_BLOCK
+
+
+@dataclass(frozen=True)
+class Fp8Tensor:
+    """e4m3 ``codes [M, K]`` and fp32 ``scale [ceil(M / block_rows), ceil(K / 128)]``: value = code * scale."""
+
+    codes: torch.Tensor
+    scale: torch.Tensor
+    block_rows: int
+
+    @property
+    def shape(self) -> torch.Size:
+        return self.codes.shape
+
+    def dequantize(self, dtype: torch.dtype = torch.float32) -> torch.Tensor:
+        M, K = self.codes.shape
+        wide = self.scale.repeat_interleave(self.block_rows, 0)[:M].repeat_interleave(BLOCK, 1)[:, :K]
+        return (self.codes.to(torch.float32) * wide).to(dtype)
+
+    def storage_bytes(self) -> int:
+        return self.codes.numel() + self.scale.numel() * 4
+
+
+def quantize_fp8(x: torch.Tensor, block_rows: int = 1) -> Fp8Tensor:
+    """x ``[M, K]`` (fp32, fp16 or bf16) to e4m3: ``block_rows`` 1 for rows, 128 for weights.
+
+    ``scale = amax / 448`` of the block and ``code`` the e4m3 nearest to ``x * 448 / amax`` (ties to
+    even); amax is taken as at least ``448 * 2**-60``.  A block with a NaN or an infinity dequantizes to NaN.
+    """
+    codes, scale = ops._fp8_quantize_impl(x, block_rows)
+    return Fp8Tensor(codes, scale, block_rows)
+
+
+def fp8_linear(x: Union[torch.Tensor, Fp8Tensor], weight: Fp8Tensor, bias: Optional[torch.Tensor] = None,
+               out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """``x . weight^T + bias``: x ``[M, K]`` values (quantized on the way as by :func:`quantize_fp8`) or an
+    :class:`Fp8Tensor` of rows; weight ``[N, K]`` in 128 x 128 blocks; K a multiple of 16."""
+    if weight.block_rows != BLOCK:
+        raise ValueError("the weight needs one scale per 128 x 128 block")
+    if isinstance(x, Fp8Tensor):
+        if x.block_rows != 1:
+            raise ValueError("the rows need one scale per 128 values of a row")
+        return ops._fp8_linear_impl(x.codes, x.scale, weight.codes, weight.scale, bias, out_dtype)
+    return ops._fp8_linear_impl(x, None, weight.codes, weight.scale, bias, out_dtype)
+
+
+class Fp8Linear(nn.Module):
+    """Linear layer on e4m3 weights: ``qweight`` uint8 ``[out, pitch]`` (the codes' bytes, rows padded to
+    16), ``scale`` fp32 ``[ceil(out / 128), ceil(in / 128)]``, ``bias`` of ``compute_dtype`` or None.
+
+    The buffers are bytes, not float8, so that ``module.half()`` and the like leave them alone.
+    """
+
+    def __init__(self, in_features: int, out_features: int, bias: bool = False,
+                 compute_dtype: torch.dtype = torch.bfloat16) -> None:
+        super().__init__()
+        if in_features < 16 or in_features % 16 != 0 or out_features < 1:
+            raise ValueError(f"Fp8Linear needs in_features in multiples of 16, got {in_features} -> {out_features}")
+        if compute_dtype not in (torch.float32, torch.float16, torch.bfloat16):
+            raise ValueError(f"compute_dtype must be fp32, fp16 or bf16, got {compute_dtype}")
+        self.in_features = in_features
+        self.out_features = out_features
+        self.compute_dtype = compute_dtype
+        self.register_buffer("qweight", torch.zeros(out_features, in_features, dtype=torch.uint8))
+        self.register_buffer("scale", torch.ones(ops.fp8_groups(out_features), ops.fp8_groups(in_features)))
+        self.register_buffer("bias", torch.zeros(out_features, dtype=compute_dtype) if bias else None)
+
+    @classmethod
+    def from_codes(cls, weight: Fp8Tensor, bias: Optional[torch.Tensor] = None,
+                   compute_dtype: torch.dtype = torch.bfloat16) -> "Fp8Linear":
+        """A layer over codes that are there already (no copy where their rows are whole and aligned)."""
+        if weight.block_rows != BLOCK:
+            raise ValueError("the weight needs one scale per 128 x 128 block")
+        N, K = weight.shape
+        m = cls(K, N, bias is not None, compute_dtype)
+        m.qweight = ops.fp8_operand(weight.codes, "the weight").view(torch.uint8).contiguous()
+        if tuple(weight.scale.shape) != tuple(m.scale.shape) or weight.scale.dtype != torch.float32:
+            raise ValueError(f"scales must be float32 {tuple(m.scale.shape)}, got {weight.scale.dtype} {tuple(weight.scale.shape)}")
+        m.scale = weight.scale.contiguous()
+        if bias is not None:
+            if tuple(bias.shape) != (N,):
+                raise ValueError(f"bias must be [{N}], got {tuple(bias.shape)}")
+            m.bias = bias.detach().to(compute_dtype).contiguous()
+        return m
+
+    @classmethod
+    def from_linear(cls, linear: nn.Linear, compute_dtype: torch.dtype = torch.bfloat16) -> "Fp8Linear":
+        """Quantize a linear layer's weight on its GPU."""
+        w = linear.weight.detach()
+        if w.dtype not in (torch.float32, torch.float16, torch.bfloat16):
+            w = w.to(torch.float32)
+        bias = None if linear.bias is None else linear.bias.detach()
+        return cls.from_codes(quantize_fp8(w, BLOCK), bias, compute_dtype)
+
+    @property
+    def weight(self) -> Fp8Tensor:
+        return Fp8Tensor(self.qweight.view(torch.float8_e4m3fn), self.scale, BLOCK)
+
+    def dequantize_weight(self) -> torch.Tensor:
+        return self.weight.dequantize(self.compute_dtype)
+
+    def storage_bytes(self) -> int:
+        tensors = [self.qweight, self.scale] + ([self.bias] if self.bias is not None else [])
+        return sum(t.numel() * t.element_size() for t in tensors)
+
+    def extra_repr(self) -> str:
+        return f"{self.in_features} -> {self.out_features}, e4m3 codes, blocks of {BLOCK}"
+
+    def forward(self, x: Union[torch.Tensor, Fp8Tensor]) -> torch.Tensor:
+        """x ``[..., in]`` (any of fp32, fp16, bf16) or an :class:`Fp8Tensor` ``[M, in]`` -> ``[..., out]``."""
+        if isinstance(x, Fp8Tensor):
+            return fp8_linear(x, self.weight, self.bias, self.compute_dtype)
+        lead = x.shape[:-1]
+        y = fp8_linear(x.reshape(-1, x.shape[-1]), self.weight, self.bias, self.compute_dtype)
+        return y.reshape(*lead, self.out_features)

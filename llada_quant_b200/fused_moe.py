@@ -26,6 +26,9 @@ import torch
 from . import _lib, ops
 from .moe import PackedExperts
 
+#: ``impl`` of the calls below that runs at most 32 tokens in two launches (``few_tokens``); no GEMM choice of the C ABI
+FEW = "few"
+
 IMPL = {"auto": _lib.LLQ_GEMM_AUTO, "tcgen05": _lib.LLQ_GEMM_TCGEN05, "simt": _lib.LLQ_GEMM_SIMT,
         "tcgen05_fast": _lib.LLQ_GEMM_TCGEN05_FAST}
 
@@ -66,6 +69,10 @@ def fused_moe(hidden_states: torch.Tensor, w1, w2, gating_output: Optional[torch
             raise ValueError("pass gating_output or topk_weights with topk_ids")
         topk_weights = routing_weights(gating_output.reshape(-1, gating_output.shape[-1]),
                                        topk_ids, renormalize)
+    if impl == FEW:
+        return ops.moe_few_routed(x, packed.qw1, packed.sw1, packed.qw2, packed.sw2,
+                                  topk_weights.reshape(x.shape[0], -1), topk_ids.reshape(x.shape[0], -1),
+                                  packed.bits).reshape(shape)
     out = ops.fused_moe_packed(x, packed.qw1, packed.sw1, packed.qw2, packed.sw2,
                                topk_weights.reshape(x.shape[0], -1),
                                topk_ids.reshape(x.shape[0], -1), packed.bits, IMPL[impl])
@@ -80,7 +87,16 @@ def moe_layer(x: torch.Tensor, gate_w: torch.Tensor, packed: PackedExperts, top_
     ``routing_stats.RoutingRecorder`` the call's per-expert loads are added to it on
     the device, from the expert offsets the GEMMs used; with a
     ``router_capture.RouterCapture`` the router kernel's own ids and logits are
-    recorded under ``name``."""
+    recorded under ``name``.  ``impl="few"``: the two-launch layer for at most 32 tokens, whose logits
+    are fp32 (``few_tokens`` says how its roundings differ)."""
+    if impl == FEW:
+        out, topk_w, topk_ids, logits = ops._moe_few_impl(x, gate_w, bias, renormalize, packed.qw1, packed.sw1,
+                                                          packed.qw2, packed.sw2, top_k, packed.bits)
+        if capture is not None:
+            capture.record(name, topk_ids, logits)
+        if recorder is not None:
+            recorder.record_offsets(ops._moe_align_impl(topk_ids, packed.num_experts)[0], x.shape[0], top_k)
+        return out
     # eager hot path: one library call (router through combine), no per-call dispatcher cost
     out, topk_w, topk_ids, logits = ops._moe_block_packed_impl(
         x, gate_w, bias, renormalize, packed.qw1, packed.sw1, packed.qw2, packed.sw2, top_k, packed.bits,

@@ -527,6 +527,269 @@ def _moe_block_packed_impl(x: torch.Tensor, gate_w: torch.Tensor, bias: Optional
     return out, tw, ids, logits
 
 
+# ---------------------------------------------------------------------------
+# the layer for a few tokens
+# ---------------------------------------------------------------------------
+
+FEW_TOKENS = 32  # most tokens of one ``moe_few`` call
+
+
+def _no_grad_through(name: str, *ts: Optional[torch.Tensor]) -> None:
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts):
+        raise RuntimeError(f"{name} has no backward pass: call it under torch.no_grad() or on detached tensors")
+
+
+def _aligned(t: torch.Tensor) -> torch.Tensor:
+    """``t`` contiguous and on a 16-byte boundary (a copy where it is not)."""
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def few_layer(qw1: torch.Tensor, sw1: torch.Tensor, qw2: torch.Tensor, sw2: torch.Tensor, k: int, bits: int,
+              gate_w: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
+              renormalize: bool = False) -> _lib.FewLayer:
+    """``llq_few_layer`` of one packed layer.  It holds pointers alone: the caller keeps the tensors."""
+    _need_cuda(qw1, sw1, qw2, sw2, gate_w, bias)
+    if bits not in (4, 8):
+        raise ValueError(f"bits must be 8 or 4, got {bits}")
+    if qw1.dim() != 3 or qw2.dim() != 3 or sw1.dim() != 3 or sw2.dim() != 3:
+        raise ValueError("packed experts are [E, rows, bytes] with scales [E, rows, groups]")
+    E, two_i, H, inter = qw1.shape[0], qw1.shape[1], qw2.shape[1], qw1.shape[1] // 2
+    per = 2 if bits == 4 else 1
+    if (two_i % 2 or tuple(qw2.shape) != (E, H, inter // per) or qw1.shape[2] * per != H
+            or sw1.shape[:2] != qw1.shape[:2] or sw2.shape[:2] != qw2.shape[:2]):
+        raise ValueError(f"w1 {tuple(qw1.shape)} and w2 {tuple(qw2.shape)} are not one layer's INT{bits} experts")
+    if any(t.dtype != torch.int8 or not t.is_contiguous() for t in (qw1, qw2)):
+        raise ValueError("packed codes are contiguous int8 tensors")
+    if any(t.dtype != torch.float32 or not t.is_contiguous() for t in (sw1, sw2)):
+        raise ValueError("the few-token layer reads contiguous float32 scales")
+    group = _group_pair(qw1, sw1, qw2, sw2, bits)
+    for K, sc in ((H, sw1), (inter, sw2)):
+        if sc.shape[2] != (K // group if group > 0 and K % group == 0 else 1):
+            raise ValueError(f"{sc.shape[2]} scales for rows of {K}")
+    if gate_w is not None and (tuple(gate_w.shape) != (E, H) or gate_w.dtype != torch.bfloat16
+                               or not gate_w.is_contiguous()):
+        raise ValueError(f"gate_w must be a contiguous bfloat16 [{E}, {H}] tensor")
+    if bias is not None and (tuple(bias.shape) != (E,) or bias.dtype != torch.float32 or not bias.is_contiguous()):
+        raise ValueError(f"bias must be a contiguous float32 [{E}] tensor")
+    devs = {t.device for t in (qw1, sw1, qw2, sw2, gate_w, bias) if t is not None}
+    if len(devs) > 1:
+        raise ValueError(f"one layer's tensors lie on several devices: {sorted(map(str, devs))}")
+    return _lib.FewLayer(_ptr(gate_w), _ptr(bias), qw1.data_ptr(), sw1.data_ptr(), qw2.data_ptr(), sw2.data_ptr(),
+                         E, H, inter, k, bits, group, int(renormalize))
+
+
+def few_call(layer: _lib.FewLayer, x: torch.Tensor, topk_w: torch.Tensor, topk_ids: torch.Tensor,
+             logits: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """One ``llq_moe_few`` call on checked operands: x bf16 [T, H] (aligned), topk_w f32 and topk_ids i32 [T, k]."""
+    dev = x.device.index
+    if dev != torch.cuda.current_device():
+        with torch.cuda.device(dev):
+            return few_call(layer, x, topk_w, topk_ids, logits)
+    lib = load()
+    T = x.shape[0]
+    out = torch.empty_like(x)
+    # scratch of this call alone: the caching allocator orders its reuse by stream and by graph
+    nbytes = lib.llq_moe_few_workspace_size(T, layer.k, layer.I)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+    check(lib.llq_moe_few(_lib.byref(layer), x.data_ptr(), T, _ptr(logits), topk_w.data_ptr(), topk_ids.data_ptr(),
+                          out.data_ptr(), ws.data_ptr(), nbytes, _stream(x)), "moe_few")
+    return out
+
+
+def few_rows(x: torch.Tensor, H: int, device: torch.device) -> torch.Tensor:
+    """x as the few-token layer reads it, or an error that says why it cannot."""
+    _need_cuda(x)
+    _no_grad_through("the few-token layer", x)
+    if x.dim() != 2 or x.shape[1] != H or x.dtype != torch.bfloat16:
+        raise ValueError(f"x must be bfloat16 [tokens, {H}], got {x.dtype} {tuple(x.shape)}")
+    if x.device != device:
+        raise ValueError(f"x lies on {x.device}, the layer on {device}")
+    return _aligned(x)
+
+
+def few_routing(topk_w: torch.Tensor, topk_ids: torch.Tensor, T: int, k: int, E: int, device: torch.device):
+    """Caller's routing as (f32, i32) [T, k]; ids outside [0, E) stay outside when they are narrowed."""
+    _need_cuda(topk_w, topk_ids)
+    _no_grad_through("the few-token layer", topk_w)
+    if tuple(topk_w.shape) != (T, k) or tuple(topk_ids.shape) != (T, k):
+        raise ValueError(f"routing must be [{T}, {k}], got weights {tuple(topk_w.shape)} and ids {tuple(topk_ids.shape)}")
+    if not topk_w.is_floating_point() or topk_ids.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"routing needs floating weights and int32 or int64 ids, got {topk_w.dtype} and {topk_ids.dtype}")
+    if topk_w.device != device or topk_ids.device != device:
+        raise ValueError(f"the routing lies on {topk_w.device} and {topk_ids.device}, the layer on {device}")
+    ids = topk_ids if topk_ids.dtype == torch.int32 else topk_ids.clamp(-1, E).to(torch.int32)
+    return topk_w.to(torch.float32).contiguous(), ids.contiguous()
+
+
+def _moe_few_impl(x: torch.Tensor, gate_w: torch.Tensor, bias: Optional[torch.Tensor], renormalize: bool,
+                  qw1: torch.Tensor, sw1: torch.Tensor, qw2: torch.Tensor, sw2: torch.Tensor, k: int,
+                  bits: int) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Router + routed experts on PACKED weights for at most 32 tokens, two launches ->
+    (out bf16 [T,H], topk_w f32 [T,k], topk_ids i32 [T,k], logits f32 [T,E])."""
+    layer = few_layer(qw1, sw1, qw2, sw2, k, bits, gate_w.contiguous(),
+                      None if bias is None else bias.contiguous().to(torch.float32), renormalize)
+    x = few_rows(x, layer.H, qw1.device)
+    T = x.shape[0]
+    tw = torch.empty(T, k, dtype=torch.float32, device=x.device)
+    ids = torch.empty(T, k, dtype=torch.int32, device=x.device)
+    logits = torch.empty(T, layer.E, dtype=torch.float32, device=x.device)
+    return few_call(layer, x, tw, ids, logits), tw, ids, logits
+
+
+moe_few = torch.library.custom_op("llada_quant::moe_few", mutates_args=())(_moe_few_impl)
+
+
+@moe_few.register_fake
+def _(x, gate_w, bias, renormalize, qw1, sw1, qw2, sw2, k, bits):
+    T = x.shape[0]
+    return (torch.empty_like(x), x.new_empty(T, k, dtype=torch.float32), x.new_empty(T, k, dtype=torch.int32),
+            x.new_empty(T, gate_w.shape[0], dtype=torch.float32))
+
+
+def _moe_few_routed_impl(x: torch.Tensor, qw1: torch.Tensor, sw1: torch.Tensor, qw2: torch.Tensor,
+                         sw2: torch.Tensor, topk_w: torch.Tensor, topk_ids: torch.Tensor, bits: int) -> torch.Tensor:
+    """The routed experts of at most 32 tokens on PACKED weights, with the caller's routing."""
+    k = topk_ids.shape[-1]
+    layer = few_layer(qw1, sw1, qw2, sw2, k, bits)
+    x = few_rows(x, layer.H, qw1.device)
+    tw, ids = few_routing(topk_w, topk_ids, x.shape[0], k, layer.E, qw1.device)
+    return few_call(layer, x, tw, ids)
+
+
+moe_few_routed = torch.library.custom_op("llada_quant::moe_few_routed", mutates_args=())(_moe_few_routed_impl)
+
+
+@moe_few_routed.register_fake
+def _(x, qw1, sw1, qw2, sw2, topk_w, topk_ids, bits):
+    return torch.empty_like(x)
+
+
+# ---------------------------------------------------------------------------
+# 8-bit floating point with a scale per block of 128
+# ---------------------------------------------------------------------------
+
+FP8_BLOCK = 128
+
+
+def fp8_groups(n: int) -> int:
+    return -(-n // FP8_BLOCK)
+
+
+def fp8_pitch(K: int) -> int:
+    """Bytes between the rows of e4m3 codes that the quantizer lays out: K up to a multiple of 16."""
+    return -(-K // 16) * 16
+
+
+def _fp8_quantize_impl(x: torch.Tensor, block_rows: int) -> Tuple[torch.Tensor, torch.Tensor]:
+    """e4m3 codes [M, K] (pitch ``fp8_pitch(K)``) and fp32 scales of x [M, K]."""
+    _need_cuda(x)
+    _no_grad_through("the e4m3 quantizer", x)
+    if x.dim() != 2 or x.shape[1] == 0 or x.dtype not in _DT:
+        raise ValueError(f"the e4m3 quantizer takes fp32, fp16 or bf16 [rows, K >= 1], got {x.dtype} {tuple(x.shape)}")
+    if block_rows not in (1, FP8_BLOCK):
+        raise ValueError(f"block_rows must be 1 or {FP8_BLOCK}, got {block_rows}")
+    M, K = x.shape
+    if x.stride(1) != 1 or (M > 1 and x.stride(0) < K):
+        x = x.contiguous()
+    dev = x.device.index
+    if dev != torch.cuda.current_device():
+        with torch.cuda.device(dev):
+            return _fp8_quantize_impl(x, block_rows)
+    pitch = fp8_pitch(K)
+    codes = torch.empty(M, pitch, dtype=torch.float8_e4m3fn, device=x.device)
+    if pitch != K:
+        codes = codes[:, :K]
+    scale = torch.empty(-(-M // block_rows), fp8_groups(K), dtype=torch.float32, device=x.device)
+    check(load().llq_fp8_quantize(x.data_ptr(), _DT[x.dtype], M, K, x.stride(0) if M > 1 else K, block_rows,
+                                  codes.data_ptr(), pitch, scale.data_ptr(), _stream(x)), "fp8_quantize")
+    return codes, scale
+
+
+fp8_quantize = torch.library.custom_op("llada_quant::fp8_quantize", mutates_args=())(_fp8_quantize_impl)
+
+
+@fp8_quantize.register_fake
+def _(x, block_rows):
+    M, K = x.shape
+    return (x.new_empty(M, fp8_pitch(K), dtype=torch.float8_e4m3fn)[:, :K],
+            x.new_empty(-(-M // block_rows), fp8_groups(K), dtype=torch.float32))
+
+
+def fp8_operand(codes: torch.Tensor, what: str) -> torch.Tensor:
+    """e4m3 codes with 16-byte aligned rows (a copy where they are not)."""
+    if codes.dim() != 2 or codes.dtype != torch.float8_e4m3fn:
+        raise ValueError(f"{what} must be float8_e4m3fn [rows, K], got {codes.dtype} {tuple(codes.shape)}")
+    M, K = codes.shape
+    if codes.stride(1) == 1 and codes.data_ptr() % 16 == 0 and (M <= 1 or (codes.stride(0) >= K and codes.stride(0) % 16 == 0)):
+        return codes
+    held = torch.empty(M, fp8_pitch(K), dtype=torch.uint8, device=codes.device)[:, :K]
+    held.copy_(codes.view(torch.uint8) if codes.stride(1) == 1 else codes.contiguous().view(torch.uint8))
+    return held.view(torch.float8_e4m3fn)
+
+
+def _fp8_linear_impl(x: torch.Tensor, x_scale: Optional[torch.Tensor], w: torch.Tensor, w_scale: torch.Tensor,
+                     bias: Optional[torch.Tensor], out_dtype: torch.dtype) -> torch.Tensor:
+    """Rows times an e4m3 weight [N, K]: x fp32/fp16/bf16 values, or e4m3 codes with ``x_scale``."""
+    _need_cuda(x, x_scale, w, w_scale, bias)
+    _no_grad_through("the e4m3 product", x, bias)
+    if x.dim() != 2 or w.dim() != 2 or x.shape[1] != w.shape[1]:
+        raise ValueError(f"x [rows, K] and weight [N, K], got {tuple(x.shape)} and {tuple(w.shape)}")
+    M, K = x.shape
+    N = w.shape[0]
+    G = fp8_groups(K)
+    if out_dtype not in _DT:
+        raise ValueError(f"the e4m3 product gives fp32, fp16 or bf16, not {out_dtype}")
+    w = fp8_operand(w, "the weight")
+    if tuple(w_scale.shape) != (fp8_groups(N), G) or w_scale.dtype != torch.float32:
+        raise ValueError(f"the weight's scales must be float32 [{fp8_groups(N)}, {G}], got {w_scale.dtype} {tuple(w_scale.shape)}")
+    if x_scale is not None:
+        x = fp8_operand(x, "the rows")
+        if tuple(x_scale.shape) != (M, G) or x_scale.dtype != torch.float32:
+            raise ValueError(f"the rows' scales must be float32 [{M}, {G}], got {x_scale.dtype} {tuple(x_scale.shape)}")
+        x_scale = x_scale.contiguous()
+        kind = _lib.LLQ_E4M3
+    else:
+        if x.dtype not in _DT:
+            raise ValueError(f"rows must be fp32, fp16 or bf16, or e4m3 with their scales, got {x.dtype}")
+        if x.stride(1) != 1 or (M > 1 and x.stride(0) < K):
+            x = x.contiguous()
+        kind = _DT[x.dtype]
+    if bias is not None:
+        if tuple(bias.shape) != (N,):
+            raise ValueError(f"bias must be [{N}], got {tuple(bias.shape)}")
+        bias = bias.to(out_dtype).contiguous()
+    if any(t is not None and t.device != x.device for t in (x_scale, w, w_scale, bias)):
+        raise ValueError("the product's operands lie on several devices")
+    return fp8_call(x, kind, x_scale, w, w_scale.contiguous(), bias, out_dtype)
+
+
+def fp8_call(x, kind, x_scale, w, w_scale, bias, out_dtype) -> torch.Tensor:
+    """One ``llq_fp8_linear`` call on checked operands."""
+    dev = x.device.index
+    if dev != torch.cuda.current_device():
+        with torch.cuda.device(dev):
+            return fp8_call(x, kind, x_scale, w, w_scale, bias, out_dtype)
+    lib = load()
+    M, K = x.shape
+    N = w.shape[0]
+    out = torch.empty(M, N, dtype=out_dtype, device=x.device)
+    need = lib.llq_fp8_linear_workspace_size(M, K, N, kind)
+    ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
+    check(lib.llq_fp8_linear(x.data_ptr(), kind, _ptr(x_scale), M, K, x.stride(0) if M > 1 else fp8_pitch(K),
+                             w.data_ptr(), w_scale.data_ptr(), N, w.stride(0) if N > 1 else fp8_pitch(K), _ptr(bias),
+                             out.data_ptr(), _DT[out_dtype], _ptr(ws), need, _stream(x)), "fp8_linear")
+    return out
+
+
+fp8_linear = torch.library.custom_op("llada_quant::fp8_linear", mutates_args=())(_fp8_linear_impl)
+
+
+@fp8_linear.register_fake
+def _(x, x_scale, w, w_scale, bias, out_dtype):
+    return x.new_empty(x.shape[0], w.shape[0], dtype=out_dtype)
+
+
 def device_error() -> int:
     import ctypes
     code = ctypes.c_int32(0)
