@@ -2,7 +2,7 @@
 // the quantizer and the product of e4m3 rows with an e4m3 weight.
 #include <cuda_fp8.h>
 
-#include "llq_common.cuh"
+#include "fp8.cuh"
 #include "llq_internal.cuh"
 
 namespace llq {
@@ -10,6 +10,8 @@ namespace llq {
 namespace {
 
 constexpr int BLK = 128;
+// up to this many rows the product runs on fp8_few_rows_kernel, above on fp8_tc_kernel
+constexpr int64_t kFewRows = 16;
 // groups whose largest magnitude lies below 448 * 2^-60 are scaled as if it were this, so that the
 // product of two scales stays a normal fp32 number
 constexpr float kAmaxFloor = 448.f * 0x1p-60f;
@@ -371,13 +373,52 @@ int fp8_linear(const void* x, int x_dtype, const float* x_scale, int64_t M, int 
   if (K % 16 != 0) return fail(LLQ_EUNSUPPORTED, "the e4m3 product needs K in multiples of 16, got %d", K);
   if (ldw % 16 != 0 || (reinterpret_cast<uintptr_t>(w) & 15) != 0)
     return fail(LLQ_EINVAL, "the weight codes need a 16-byte aligned base and row pitch");
-  if (M > 65535 * 8) return fail(LLQ_EINVAL, "too many rows");
+  if (M > 0x7fffffff - 256) return fail(LLQ_EINVAL, "too many rows");
   if (M == 0) return LLQ_OK;
   if (x == nullptr || w == nullptr || w_scale == nullptr || out == nullptr) return fail(LLQ_EINVAL, "null pointer");
+  const int size = x_dtype == LLQ_E4M3 ? 1 : x_dtype == LLQ_F32 ? 4 : 2;
+  const bool vec = (reinterpret_cast<uintptr_t>(x) & 15) == 0 && (ldx * size) % 16 == 0;
+  if (x_dtype == LLQ_E4M3) {
+    if (x_scale == nullptr) return fail(LLQ_EINVAL, "e4m3 rows need their scales");
+    if (!vec) return fail(LLQ_EINVAL, "the row codes need a 16-byte aligned base and row pitch");
+  } else if (x_dtype != LLQ_F32 && x_dtype != LLQ_F16 && x_dtype != LLQ_BF16) {
+    return fail(LLQ_EUNSUPPORTED, "unknown dtype %d", x_dtype);
+  }
+  const int G = (K + BLK - 1) / BLK;
+  if (M > kFewRows) {
+    Fp8Operands p{};
+    p.x = static_cast<const uint8_t*>(x);
+    p.xs = x_scale;
+    p.ldx = ldx;
+    if (x_dtype != LLQ_E4M3) {  // quantized once into the workspace
+      const size_t need = fp8_linear_workspace(M, K, N, x_dtype);
+      if (workspace == nullptr || bytes < need) return fail(LLQ_ENOSPACE, "workspace needs %zu bytes, got %zu", need, bytes);
+      if (reinterpret_cast<uintptr_t>(workspace) & 15) return fail(LLQ_EINVAL, "the workspace needs 16-byte alignment");
+      uint8_t* codes = static_cast<uint8_t*>(workspace);
+      float* scale = reinterpret_cast<float*>(codes + static_cast<size_t>(M) * K);
+      const int rc = fp8_quantize(x, x_dtype, M, K, ldx, 1, codes, K, scale, st);
+      if (rc) return rc;
+      p.x = codes;
+      p.xs = scale;
+      p.ldx = K;
+    }
+    p.w = w;
+    p.ws = w_scale;
+    p.ldw = ldw;
+    p.bias = bias;
+    p.out = out;
+    p.out_type = out_dtype;
+    p.M = M;
+    p.N = N;
+    p.K = K;
+    p.G = G;
+    return fp8_gemm_tc(p, st);
+  }
   LinArgs a{};
   a.x = x;
   a.xs = x_scale;
   a.ldx = ldx;
+  a.vec = vec;
   a.w = w;
   a.ws = w_scale;
   a.ldw = ldw;
@@ -387,24 +428,21 @@ int fp8_linear(const void* x, int x_dtype, const float* x_scale, int64_t M, int 
   a.M = M;
   a.N = N;
   a.K = K;
-  a.G = (K + BLK - 1) / BLK;
-  const int size = x_dtype == LLQ_E4M3 ? 1 : x_dtype == LLQ_F32 ? 4 : 2;
-  a.vec = (reinterpret_cast<uintptr_t>(x) & 15) == 0 && (ldx * size) % 16 == 0;
+  a.G = G;
   const dim3 grid((N + 15) / 16, static_cast<unsigned>((M + 7) / 8));
   switch (x_dtype) {
-    case LLQ_E4M3:
-      if (x_scale == nullptr) return fail(LLQ_EINVAL, "e4m3 rows need their scales");
-      if (!a.vec) return fail(LLQ_EINVAL, "the row codes need a 16-byte aligned base and row pitch");
-      launch_pdl(fp8_few_rows_kernel<Raw>, grid, dim3(256), 0, st, a);
-      break;
+    case LLQ_E4M3: launch_pdl(fp8_few_rows_kernel<Raw>, grid, dim3(256), 0, st, a); break;
     case LLQ_F32: launch_pdl(fp8_few_rows_kernel<float>, grid, dim3(256), 0, st, a); break;
     case LLQ_F16: launch_pdl(fp8_few_rows_kernel<__half>, grid, dim3(256), 0, st, a); break;
-    case LLQ_BF16: launch_pdl(fp8_few_rows_kernel<__nv_bfloat16>, grid, dim3(256), 0, st, a); break;
-    default: return fail(LLQ_EUNSUPPORTED, "unknown dtype %d", x_dtype);
+    default: launch_pdl(fp8_few_rows_kernel<__nv_bfloat16>, grid, dim3(256), 0, st, a); break;
   }
   return check_launch("fp8_few_rows_kernel");
 }
 
-size_t fp8_linear_workspace(int64_t M, int K, int N, int x_dtype) { return 0; }
+// codes [M][K] (K is a multiple of 16) and scales [M][G] of rows that are quantized before the tensor-core product
+size_t fp8_linear_workspace(int64_t M, int K, int N, int x_dtype) {
+  if (M <= kFewRows || K < 1 || x_dtype == LLQ_E4M3) return 0;
+  return static_cast<size_t>(M) * K + static_cast<size_t>(M) * ((K + BLK - 1) / BLK) * 4;
+}
 
 }  // namespace llq

@@ -1,0 +1,446 @@
+// Product of e4m3 rows with an e4m3 weight, one fp32 scale per 128 of a row and per 128 x 128 of the
+// weight, on the tensor cores:
+//
+//   out[m, n] = sum over blocks g of xs[m, g] ws[n / 128, g] (sum_{k in g} x[m, k] w[n, k])  (+ bias[n])
+//
+// The scales are fp32, so no block sum may be added to another inside the tensor core: each 128-block of K
+// is its own tcgen05.mma group (four kind::f8f6f4 MMAs of K = 32) into its own TMEM buffer, and the
+// epilogue warps read it back, multiply by the block's scale and add in fp32 registers while the next
+// block is being multiplied into another buffer.
+//
+// A tile is 128 rows (TMEM lanes, so a row's scale is one number per thread) by BN weight rows.
+//   warp 0      TMA producer: per block the 128 x 128 and BN x 128 byte boxes (128-byte swizzle)
+//   warp 1      TMEM allocator and MMA issuer (one elected lane)
+//   warps 2-9   epilogue: one TMEM lane quarter each, half of the columns; BN / 2 sums per thread
+// Persistent over tiles when K is not split.  When the tiles do not cover the SMs, a cluster of `split`
+// CTAs shares one tile, each takes a part of K, and the parts meet in distributed shared memory and are
+// added in rank order.
+#include <cooperative_groups.h>
+
+#include "fp8.cuh"
+#include "tc_ptx.cuh"
+
+namespace llq {
+
+namespace {
+
+namespace cg = cooperative_groups;
+
+constexpr int BM = 128;
+constexpr int BK = 128;
+
+template <int BN>
+struct F8Cfg {
+  static constexpr int A_BYTES = BM * BK;
+  static constexpr int STAGE_BYTES = A_BYTES + BN * BK;
+  static constexpr int STAGES = 196608 / STAGE_BYTES;
+  static constexpr int ACC_BUFS = BN == 256 ? 2 : 4;
+  static constexpr int TMEM_COLS = ACC_BUFS * BN;
+  static constexpr int EPI_WARPS = 8;
+  static constexpr int COLS = BN / 2;  // columns of an epilogue thread
+  static constexpr int THREADS = (2 + EPI_WARPS) * 32;
+  static constexpr int OUT_BYTES = EPI_WARPS * 4096;  // per warp 32 rows of 128 bytes
+  static constexpr size_t SMEM_BYTES = 1024 + static_cast<size_t>(STAGES) * STAGE_BYTES + OUT_BYTES + 512;
+  static_assert(128 * BN * 4 <= STAGES * STAGE_BYTES, "the parts of a split tile reuse the stages");
+  static_assert(SMEM_BYTES <= 232448, "shared memory");
+};
+
+struct F8Args {
+  const float* xs;   // [M][G]
+  const float* ws;   // [ceil(N / 128)][G]
+  const void* bias;  // [N] of the output's type, or null
+  void* out;         // [M][N]
+  int64_t M;
+  int N, G;
+  int mtiles, tiles;
+  int split;
+  int tma_out;       // rows of out are 16-byte aligned
+};
+
+// instruction descriptor of kind::f8f6f4: D f32, A and B e4m3 (0), both K-major
+__device__ __forceinline__ uint32_t f8_idesc(int n) {
+  return (1u << 4) | (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(BM >> 4) << 24);
+}
+
+__device__ __forceinline__ void tc_mma_f8(uint32_t d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate,
+                                          uint32_t issue) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "setp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(issue)
+      : "memory");
+}
+
+// 32 consecutive fp32 columns of this thread's TMEM lane; complete after tc_wait_ld()
+__device__ __forceinline__ void tc_ld32(uint32_t taddr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr)
+      : "memory");
+}
+
+// two sums at once: acc = v * s + acc
+__device__ __forceinline__ void fma2(uint64_t& acc, uint32_t lo, uint32_t hi, uint64_t s) {
+  asm("{\n\t.reg .b64 v;\n\tmov.b64 v, {%1, %2};\n\tfma.rn.f32x2 %0, v, %3, %0;\n\t}" : "+l"(acc) : "r"(lo), "r"(hi), "l"(s));
+}
+
+__device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, const void* src, int x, int y) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];" ::"l"(
+                   reinterpret_cast<uint64_t>(map)),
+               "r"(x), "r"(y), "r"(smem_u32(src))
+               : "memory");
+  asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+
+template <typename O>
+__device__ __forceinline__ float bias_at(const void* b, int n) {
+  return to_f32(static_cast<const O*>(b)[n]);
+}
+
+// 16 bytes of outputs from consecutive sums
+__device__ __forceinline__ uint4 pack_out(const float* v, float) {
+  return make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+}
+__device__ __forceinline__ uint32_t pack2(float a, float b, __nv_bfloat16) {
+  __nv_bfloat162 p = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<uint32_t*>(&p);
+}
+__device__ __forceinline__ uint32_t pack2(float a, float b, __half) {
+  __half2 p = __floats2half2_rn(a, b);
+  return *reinterpret_cast<uint32_t*>(&p);
+}
+template <typename O>
+__device__ __forceinline__ uint4 pack_out(const float* v, O o) {
+  return make_uint4(pack2(v[0], v[1], o), pack2(v[2], v[3], o), pack2(v[4], v[5], o), pack2(v[6], v[7], o));
+}
+
+template <int BN, typename O>
+__global__ void __launch_bounds__(F8Cfg<BN>::THREADS, 1)
+    fp8_tc_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w,
+                  const __grid_constant__ CUtensorMap tm_o, const F8Args a) {
+  using C = F8Cfg<BN>;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* so = smem + C::STAGES * C::STAGE_BYTES;
+  uint64_t* full = reinterpret_cast<uint64_t*>(so + C::OUT_BYTES);
+  uint64_t* empty = full + C::STAGES;
+  uint64_t* acc_full = empty + C::STAGES;
+  uint64_t* acc_empty = acc_full + C::ACC_BUFS;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + C::ACC_BUFS);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < C::STAGES; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 1);
+    }
+    for (int i = 0; i < C::ACC_BUFS; ++i) {
+      mbar_init(&acc_full[i], 1);
+      mbar_init(&acc_empty[i], C::EPI_WARPS);
+    }
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                 "r"(C::TMEM_COLS)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  pdl_wait();
+  // the codes may come from generic stores of the kernel before
+  asm volatile("fence.proxy.async.global;" ::: "memory");
+
+  const int rank = blockIdx.x % a.split;
+  const int stride = gridDim.x / a.split;
+  const int g0 = static_cast<int>(static_cast<int64_t>(a.G) * rank / a.split);
+  const int g1 = static_cast<int>(static_cast<int64_t>(a.G) * (rank + 1) / a.split);
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int issued = 0, rs = 0;
+      uint32_t ph = 0;
+      bool ok = true;
+      for (int u = blockIdx.x / a.split; u < a.tiles && ok; u += stride) {
+        const int m0 = u % a.mtiles * BM, n0 = u / a.mtiles * BN;
+        for (int g = g0; g < g1; ++g) {
+          if (!mbar_wait(&empty[rs], ph ^ 1, abort_flag, 0x500 + rs)) { ok = false; break; }
+          mbar_expect_tx(&full[rs], C::STAGE_BYTES);
+          uint8_t* dst = smem + rs * C::STAGE_BYTES;
+          tma_load_2d(dst, &tm_x, g * BK, m0, &full[rs]);
+          tma_load_2d(dst + C::A_BYTES, &tm_w, g * BK, n0, &full[rs]);
+          ++issued;
+          if (++rs == C::STAGES) {
+            rs = 0;
+            ph ^= 1;
+          }
+        }
+      }
+      // never leave copies in flight into this CTA's shared memory
+      for (int i = (issued > C::STAGES ? issued - C::STAGES : 0); i < issued; ++i) {
+        const long long t0 = clock64();
+        while (!mbar_try_wait(&full[i % C::STAGES], (i / C::STAGES) & 1) && clock64() - t0 < kTimeoutCycles) {
+        }
+      }
+    }
+  } else if (warp == 1) {
+    const uint32_t leader = elect_one();
+    const uint32_t idesc = f8_idesc(BN);
+    int rs = 0, ab = 0;
+    uint32_t ph = 0, aph = 0;
+    bool ok = true;
+    for (int u = blockIdx.x / a.split; u < a.tiles && ok; u += stride) {
+      for (int g = g0; g < g1; ++g) {
+        if (!mbar_wait(&acc_empty[ab], aph ^ 1, abort_flag, 0x510 + ab)) { ok = false; break; }
+        if (!mbar_wait(&full[rs], ph, abort_flag, 0x520 + rs)) { ok = false; break; }
+        tc_fence_after();
+        const uint64_t ad = make_sdesc(smem_u32(smem + rs * C::STAGE_BYTES));
+        const uint64_t bd = make_sdesc(smem_u32(smem + rs * C::STAGE_BYTES + C::A_BYTES));
+#pragma unroll
+        for (int j = 0; j < 4; ++j)  // 32 bytes of K each: two 16-byte units of the descriptors
+          tc_mma_f8(tmem + ab * BN, ad + 2 * j, bd + 2 * j, idesc, j > 0 ? 1u : 0u, leader);
+        tc_commit(&empty[rs], leader);
+        tc_commit(&acc_full[ab], leader);
+        if (++rs == C::STAGES) {
+          rs = 0;
+          ph ^= 1;
+        }
+        if (++ab == C::ACC_BUFS) {
+          ab = 0;
+          aph ^= 1;
+        }
+      }
+    }
+  } else {
+    const int half = (warp - 2) >> 2;
+    const int q = warp & 3;  // the TMEM lanes a warp may read
+    const uint32_t lane_addr = tmem + (static_cast<uint32_t>(q * 32) << 16) + half * C::COLS;
+    uint8_t* stage = so + (warp - 2) * 4096;
+    int ab = 0;
+    uint32_t aph = 0;
+    bool ok = true;
+    for (int u = blockIdx.x / a.split; u < a.tiles && ok; u += stride) {
+      const int m0 = u % a.mtiles * BM, n0 = u / a.mtiles * BN + half * C::COLS;
+      const int64_t row = static_cast<int64_t>(m0) + q * 32 + lane;
+      const bool in = row < a.M;
+      const float* xs = a.xs + (in ? row : 0) * a.G;
+      const float* ws = a.ws + static_cast<int64_t>(min(n0, a.N - 1) / 128) * a.G;
+      uint64_t acc[C::COLS / 2];
+#pragma unroll
+      for (int i = 0; i < C::COLS / 2; ++i) acc[i] = 0;
+      float sx = in && g0 < g1 ? __ldg(xs + g0) : 0.f, sw = g0 < g1 ? __ldg(ws + g0) : 0.f;
+      for (int g = g0; g < g1; ++g) {
+        const float s = __fmul_rn(sx, sw);
+        uint64_t s2;
+        asm("mov.b64 %0, {%1, %1};" : "=l"(s2) : "f"(s));
+        if (g + 1 < g1) {  // the next block's scales ahead of the wait
+          sx = in ? __ldg(xs + g + 1) : 0.f;
+          sw = __ldg(ws + g + 1);
+        }
+        if (!mbar_wait(&acc_full[ab], aph, abort_flag, 0x530 + ab)) { ok = false; break; }
+        tc_fence_after();
+#pragma unroll
+        for (int c = 0; c < C::COLS / 32; ++c) {
+          uint32_t v[32];
+          tc_ld32(lane_addr + ab * BN + c * 32, v);
+          tc_wait_ld();
+#pragma unroll
+          for (int i = 0; i < 16; ++i) fma2(acc[c * 16 + i], v[2 * i], v[2 * i + 1], s2);
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&acc_empty[ab]);
+        if (++ab == C::ACC_BUFS) {
+          ab = 0;
+          aph ^= 1;
+        }
+      }
+      if (!ok) break;
+      if (a.split > 1) {  // this CTA's part of the tile, column by column, over the drained stages
+        float* part = reinterpret_cast<float*>(smem) + (half * C::COLS) * BM + q * 32 + lane;
+#pragma unroll
+        for (int i = 0; i < C::COLS / 2; ++i) {
+          part[(2 * i) * BM] = __uint_as_float(static_cast<uint32_t>(acc[i]));
+          part[(2 * i + 1) * BM] = __uint_as_float(static_cast<uint32_t>(acc[i] >> 32));
+        }
+        break;
+      }
+      // 128 bytes of every row at a time through this warp's shared memory
+      constexpr int PER = 16 / sizeof(O);                                      // outputs of 16 bytes
+      constexpr int CC = C::COLS * sizeof(O) < 128 ? C::COLS : 128 / sizeof(O);  // columns of a round
+#pragma unroll
+      for (int c = 0; c < C::COLS / CC; ++c) {
+        if (a.tma_out) {
+          if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+        }
+        __syncwarp();
+#pragma unroll
+        for (int j = 0; j < CC / PER; ++j) {
+          float v[PER];
+#pragma unroll
+          for (int i = 0; i < PER; i += 2) {
+            const uint64_t p = acc[(c * CC + j * PER + i) / 2];
+            v[i] = __uint_as_float(static_cast<uint32_t>(p));
+            v[i + 1] = __uint_as_float(static_cast<uint32_t>(p >> 32));
+          }
+          if (a.bias != nullptr) {
+#pragma unroll
+            for (int i = 0; i < PER; ++i)
+              v[i] = __fadd_rn(v[i], bias_at<O>(a.bias, min(n0 + c * CC + j * PER + i, a.N - 1)));
+          }
+          *reinterpret_cast<uint4*>(stage + lane * 128 + ((j ^ (lane & 7)) * 16)) = pack_out(v, O());
+        }
+        if (a.tma_out) {
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          __syncwarp();
+          if (lane == 0 && n0 + c * CC < a.N && m0 + q * 32 < a.M) tma_store_2d(&tm_o, stage, n0 + c * CC, m0 + q * 32);
+        } else {
+          __syncwarp();
+          for (int r = 0; r < 32 && m0 + q * 32 + r < a.M; ++r) {
+            O* dst = static_cast<O*>(a.out) + (static_cast<int64_t>(m0) + q * 32 + r) * a.N;
+            for (int i = lane; i < CC; i += 32) {
+              const int n = n0 + c * CC + i;
+              if (n < a.N)
+                dst[n] = *reinterpret_cast<const O*>(stage + r * 128 + (((i / PER) ^ (r & 7)) * 16) + i % PER * sizeof(O));
+            }
+          }
+          __syncwarp();
+        }
+      }
+    }
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+  }
+  if (a.split > 1) {
+    cg::cluster_group cluster = cg::this_cluster();
+    cluster.sync();
+    // BN / split columns each: a thread adds 8 of one row over the ranks, in rank order
+    const int u = blockIdx.x / a.split;
+    const int m0 = u % a.mtiles * BM, n0 = u / a.mtiles * BN;
+    const int mine = BN / a.split, c0 = rank * mine;
+    for (int i = threadIdx.x; i < BM * mine / 8; i += C::THREADS) {
+      const int r = i % BM, c = c0 + i / BM * 8;
+      float v[8] = {};
+      for (int k = 0; k < a.split; ++k) {
+        const float* part = cluster.map_shared_rank(reinterpret_cast<float*>(smem), k) + c * BM + r;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = __fadd_rn(v[j], part[j * BM]);
+      }
+      const int64_t m = static_cast<int64_t>(m0) + r;
+      if (m < a.M) {
+        O* dst = static_cast<O*>(a.out) + m * a.N + n0 + c;
+        if (a.bias != nullptr) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) v[j] = __fadd_rn(v[j], bias_at<O>(a.bias, min(n0 + c + j, a.N - 1)));
+        }
+        constexpr int PER = 16 / sizeof(O);
+        if (a.tma_out && n0 + c + 8 <= a.N) {
+#pragma unroll
+          for (int j = 0; j < 8; j += PER) *reinterpret_cast<uint4*>(dst + j) = pack_out(v + j, O());
+        } else {
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if (n0 + c + j < a.N) dst[j] = from_f32<O>(v[j]);
+        }
+      }
+    }
+    cluster.sync();  // the others may still read this CTA's part
+  }
+  tc_fence_before();
+  __syncthreads();
+  pdl_trigger();
+  if (warp == 1) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(C::TMEM_COLS) : "memory");
+  }
+}
+
+template <int BN, typename O>
+int launch_tc(const Fp8Operands& p, const F8Args& in, CUtensorMapDataType ot, cudaStream_t st) {
+  using C = F8Cfg<BN>;
+  F8Args a = in;
+  CUtensorMap tx, tw, to;
+  int rc = make_map(&tx, p.x, CU_TENSOR_MAP_DATA_TYPE_UINT8, p.K, p.M, p.ldx, BK, BM, CU_TENSOR_MAP_SWIZZLE_128B);
+  if (rc) return rc;
+  rc = make_map(&tw, p.w, CU_TENSOR_MAP_DATA_TYPE_UINT8, p.K, p.N, p.ldw, BK, BN, CU_TENSOR_MAP_SWIZZLE_128B);
+  if (rc) return rc;
+  to = tx;
+  const bool aligned = (reinterpret_cast<uintptr_t>(p.out) & 15) == 0 && (static_cast<size_t>(p.N) * sizeof(O)) % 16 == 0;
+  a.tma_out = aligned && (a.split > 1 || C::COLS * sizeof(O) >= 128);
+  if (a.tma_out && a.split == 1) {
+    rc = make_map(&to, p.out, ot, p.N, p.M, static_cast<uint64_t>(p.N) * sizeof(O), 128 / sizeof(O), 32,
+                  CU_TENSOR_MAP_SWIZZLE_128B);
+    if (rc) return rc;
+  }
+  // set on every call: a first call elsewhere may not have set it yet
+  cudaError_t e = cudaFuncSetAttribute(fp8_tc_kernel<BN, O>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                       static_cast<int>(C::SMEM_BYTES));
+  if (e != cudaSuccess) return fail(LLQ_ECUDA, "fp8_tc_kernel: %s", cudaGetErrorString(e));
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(a.split > 1 ? a.tiles * a.split : std::min(a.tiles, num_sms()));
+  cfg.blockDim = dim3(C::THREADS);
+  cfg.dynamicSmemBytes = C::SMEM_BYTES;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = a.split;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = a.split > 1 ? 2 : 1;
+  e = cudaLaunchKernelEx(&cfg, fp8_tc_kernel<BN, O>, tx, tw, to, a);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return fail(LLQ_ECUDA, "fp8_tc_kernel: %s", cudaGetErrorString(e));
+  }
+  return LLQ_OK;
+}
+
+template <int BN>
+int launch_out(const Fp8Operands& p, const F8Args& a, cudaStream_t st) {
+  switch (p.out_type) {
+    case LLQ_F32: return launch_tc<BN, float>(p, a, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, st);
+    case LLQ_F16: return launch_tc<BN, __half>(p, a, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, st);
+    default: return launch_tc<BN, __nv_bfloat16>(p, a, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, st);
+  }
+}
+
+}  // namespace
+
+int fp8_gemm_tc(const Fp8Operands& p, cudaStream_t st) {
+  const int64_t mt = (p.M + BM - 1) / BM;
+  const int sms = num_sms();
+  auto tiles = [&](int bn) { return mt * ((p.N + bn - 1) / bn); };
+  int bn = 256;
+  if (tiles(256) < sms) bn = tiles(128) < sms ? 64 : 128;
+  F8Args a{};
+  a.xs = p.xs;
+  a.ws = p.ws;
+  a.bias = p.bias;
+  a.out = p.out;
+  a.M = p.M;
+  a.N = p.N;
+  a.G = p.G;
+  if (tiles(bn) > 0x7fffffff) return fail(LLQ_EINVAL, "too many tiles");
+  a.mtiles = static_cast<int>(mt);
+  a.tiles = static_cast<int>(tiles(bn));
+  a.split = 1;
+  if (bn == 64)
+    while (a.split < 8 && a.tiles * a.split * 2 <= sms && a.split * 4 <= a.G) a.split *= 2;
+  return bn == 256 ? launch_out<256>(p, a, st) : bn == 128 ? launch_out<128>(p, a, st) : launch_out<64>(p, a, st);
+}
+
+}  // namespace llq
