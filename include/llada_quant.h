@@ -341,12 +341,12 @@ typedef struct llq_few_layer {
  * tokens, which round logits, weights and h to bf16.  logits float32 [T, E]
  * or NULL.  Ids outside [0, E) contribute nothing (experts of other ranks); an
  * expert that appears twice in a token counts with the sum of its weights.
- * T <= 32, E <= 256, k <= 32, H and I in multiples of 32 up to 32768, a group
+ * T <= 32, E <= 256, k <= 32, H and I in multiples of 32 up to 8192, a group
  * size in multiples of 128 or one scale per row (others: LLQ_EUNSUPPORTED).
  * workspace: llq_moe_few_workspace_size bytes, of this call alone until it is
  * done on the stream.
  */
-size_t llq_moe_few_workspace_size(int64_t T, int k, int I);
+size_t llq_moe_few_workspace_size(int64_t T, int k, int E, int I);
 int llq_moe_few(const llq_few_layer* layer, const void* x, int64_t T, float* logits, float* topk_w,
                 int32_t* topk_ids, void* out, void* workspace, size_t workspace_bytes,
                 void* stream);

@@ -384,9 +384,11 @@ int launch_tc(const Fp8Operands& p, const F8Args& in, CUtensorMapDataType ot, cu
                   CU_TENSOR_MAP_SWIZZLE_128B);
     if (rc) return rc;
   }
-  // set on every call: a first call elsewhere may not have set it yet
-  cudaError_t e = cudaFuncSetAttribute(fp8_tc_kernel<BN, O>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       static_cast<int>(C::SMEM_BYTES));
+  static std::atomic<uint64_t> ready{0};
+  cudaError_t e = once_per_device(ready, [] {
+    return cudaFuncSetAttribute(fp8_tc_kernel<BN, O>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                static_cast<int>(C::SMEM_BYTES));
+  });
   if (e != cudaSuccess) return fail(LLQ_ECUDA, "fp8_tc_kernel: %s", cudaGetErrorString(e));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(a.split > 1 ? a.tiles * a.split : std::min(a.tiles, num_sms()));

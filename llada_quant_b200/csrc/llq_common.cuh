@@ -57,6 +57,19 @@ inline bool first_use_on_device(std::atomic<uint64_t>& seen_mask) {
   return (seen_mask.fetch_or(bit) & bit) == 0;
 }
 
+// `set` once per device: the device is marked after `set` succeeded, so that no other
+// thread launches before the attribute is there
+template <typename F>
+inline cudaError_t once_per_device(std::atomic<uint64_t>& done, F&& set) {
+  int dev = 0;
+  const bool known = cudaGetDevice(&dev) == cudaSuccess && dev >= 0 && dev < 64;
+  const uint64_t bit = known ? 1ull << dev : 0;
+  if (done.load(std::memory_order_acquire) & bit) return cudaSuccess;
+  const cudaError_t e = set();
+  if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_release);
+  return e;
+}
+
 // ---------------------------------------------------------------------------
 // programmatic dependent launch: the layer's kernels are launched so that the
 // next one is scheduled while the previous one drains; each waits for its

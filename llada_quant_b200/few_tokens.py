@@ -48,18 +48,22 @@ class FewTokenMoE:
 
     def __call__(self, x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
         """x bf16 ``[T <= 32, H]`` -> (out bf16 ``[T, H]``, weights fp32 ``[T, k]``, ids int32 ``[T, k]``)."""
-        return self.with_logits(x, False)[:3]
+        x, weights, ids = self._outputs(x)
+        return ops.few_call(self._layer, x, weights, ids), weights, ids
 
-    def with_logits(self, x: torch.Tensor, want: bool = True):
+    def with_logits(self, x: torch.Tensor):
         """As a call, with the router's logits (bias added) fp32 ``[T, E]`` as the fourth."""
+        x, weights, ids = self._outputs(x)
+        logits = torch.empty(x.shape[0], self.num_experts, dtype=torch.float32, device=self.device)
+        return ops.few_call(self._layer, x, weights, ids, logits), weights, ids, logits
+
+    def _outputs(self, x: torch.Tensor):
         if self._layer is None:
             raise ValueError("this layer was made without gate_w: call routed(x, weights, ids)")
         x = ops.few_rows(x, self.hidden, self.device)
         T = x.shape[0]
-        weights = torch.empty(T, self.top_k, dtype=torch.float32, device=x.device)
-        ids = torch.empty(T, self.top_k, dtype=torch.int32, device=x.device)
-        logits = torch.empty(T, self.num_experts, dtype=torch.float32, device=x.device) if want else None
-        return ops.few_call(self._layer, x, weights, ids, logits), weights, ids, logits
+        return (x, torch.empty(T, self.top_k, dtype=torch.float32, device=self.device),
+                torch.empty(T, self.top_k, dtype=torch.int32, device=self.device))
 
     def routed(self, x: torch.Tensor, topk_weights: torch.Tensor, topk_ids: torch.Tensor) -> torch.Tensor:
         """The experts alone, with the caller's routing ``[T, k]``.  Ids outside ``[0, E)`` contribute

@@ -57,13 +57,21 @@ def fp8_linear(x: Union[torch.Tensor, Fp8Tensor], weight: Fp8Tensor, bias: Optio
                out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """``x . weight^T + bias``: x ``[M, K]`` values (quantized on the way as by :func:`quantize_fp8`) or an
     :class:`Fp8Tensor` of rows; weight ``[N, K]`` in 128 x 128 blocks; K a multiple of 16."""
-    if weight.block_rows != BLOCK:
+    return _multiply(ops.Fp8Weight(_weight(weight).codes, weight.scale, bias, out_dtype), x)
+
+
+def _weight(w: Fp8Tensor) -> Fp8Tensor:
+    if w.block_rows != BLOCK:
         raise ValueError("the weight needs one scale per 128 x 128 block")
-    if isinstance(x, Fp8Tensor):
-        if x.block_rows != 1:
-            raise ValueError("the rows need one scale per 128 values of a row")
-        return ops._fp8_linear_impl(x.codes, x.scale, weight.codes, weight.scale, bias, out_dtype)
-    return ops._fp8_linear_impl(x, None, weight.codes, weight.scale, bias, out_dtype)
+    return w
+
+
+def _multiply(w: ops.Fp8Weight, x: Union[torch.Tensor, Fp8Tensor]) -> torch.Tensor:
+    if not isinstance(x, Fp8Tensor):
+        return w.multiply(x)
+    if x.block_rows != 1:
+        raise ValueError("the rows need one scale per 128 values of a row")
+    return w.multiply(x.codes, x.scale)
 
 
 class Fp8Linear(nn.Module):
@@ -76,6 +84,12 @@ class Fp8Linear(nn.Module):
     def __init__(self, in_features: int, out_features: int, bias: bool = False,
                  compute_dtype: torch.dtype = torch.bfloat16) -> None:
         super().__init__()
+        self._sizes(in_features, out_features, compute_dtype)
+        self.register_buffer("qweight", torch.zeros(out_features, in_features, dtype=torch.uint8))
+        self.register_buffer("scale", torch.ones(ops.fp8_groups(out_features), ops.fp8_groups(in_features)))
+        self.register_buffer("bias", torch.zeros(out_features, dtype=compute_dtype) if bias else None)
+
+    def _sizes(self, in_features: int, out_features: int, compute_dtype: torch.dtype) -> None:
         if in_features < 16 or in_features % 16 != 0 or out_features < 1:
             raise ValueError(f"Fp8Linear needs in_features in multiples of 16, got {in_features} -> {out_features}")
         if compute_dtype not in (torch.float32, torch.float16, torch.bfloat16):
@@ -83,26 +97,20 @@ class Fp8Linear(nn.Module):
         self.in_features = in_features
         self.out_features = out_features
         self.compute_dtype = compute_dtype
-        self.register_buffer("qweight", torch.zeros(out_features, in_features, dtype=torch.uint8))
-        self.register_buffer("scale", torch.ones(ops.fp8_groups(out_features), ops.fp8_groups(in_features)))
-        self.register_buffer("bias", torch.zeros(out_features, dtype=compute_dtype) if bias else None)
+        self._ready = None
 
     @classmethod
     def from_codes(cls, weight: Fp8Tensor, bias: Optional[torch.Tensor] = None,
                    compute_dtype: torch.dtype = torch.bfloat16) -> "Fp8Linear":
         """A layer over codes that are there already (no copy where their rows are whole and aligned)."""
-        if weight.block_rows != BLOCK:
-            raise ValueError("the weight needs one scale per 128 x 128 block")
-        N, K = weight.shape
-        m = cls(K, N, bias is not None, compute_dtype)
-        m.qweight = ops.fp8_operand(weight.codes, "the weight").view(torch.uint8).contiguous()
-        if tuple(weight.scale.shape) != tuple(m.scale.shape) or weight.scale.dtype != torch.float32:
-            raise ValueError(f"scales must be float32 {tuple(m.scale.shape)}, got {weight.scale.dtype} {tuple(weight.scale.shape)}")
-        m.scale = weight.scale.contiguous()
-        if bias is not None:
-            if tuple(bias.shape) != (N,):
-                raise ValueError(f"bias must be [{N}], got {tuple(bias.shape)}")
-            m.bias = bias.detach().to(compute_dtype).contiguous()
+        N, K = _weight(weight).shape
+        m = cls.__new__(cls)
+        nn.Module.__init__(m)
+        m._sizes(K, N, compute_dtype)
+        held = ops.Fp8Weight(weight.codes, weight.scale, bias, compute_dtype)
+        m.register_buffer("qweight", held.codes.view(torch.uint8).contiguous())
+        m.register_buffer("scale", held.scale)
+        m.register_buffer("bias", held.bias)
         return m
 
     @classmethod
@@ -128,10 +136,19 @@ class Fp8Linear(nn.Module):
     def extra_repr(self) -> str:
         return f"{self.in_features} -> {self.out_features}, e4m3 codes, blocks of {BLOCK}"
 
+    def _multiplier(self) -> ops.Fp8Weight:
+        """The checked operand of the buffers as they are now (checked again when one was replaced)."""
+        b, r = self._buffers, self._ready
+        q, s, bias = b["qweight"], b["scale"], b["bias"]
+        at = (q.data_ptr(), s.data_ptr(), 0 if bias is None else bias.data_ptr())
+        if r is None or r[0] is not q or r[1] is not s or r[2] is not bias or r[3] != at:
+            w = ops.Fp8Weight(q.view(torch.float8_e4m3fn), s, bias, self.compute_dtype)
+            self._ready = r = (q, s, bias, at, w)
+        return r[4]
+
     def forward(self, x: Union[torch.Tensor, Fp8Tensor]) -> torch.Tensor:
         """x ``[..., in]`` (any of fp32, fp16, bf16) or an :class:`Fp8Tensor` ``[M, in]`` -> ``[..., out]``."""
-        if isinstance(x, Fp8Tensor):
-            return fp8_linear(x, self.weight, self.bias, self.compute_dtype)
-        lead = x.shape[:-1]
-        y = fp8_linear(x.reshape(-1, x.shape[-1]), self.weight, self.bias, self.compute_dtype)
-        return y.reshape(*lead, self.out_features)
+        w = self._multiplier()
+        if isinstance(x, Fp8Tensor) or x.dim() == 2:
+            return _multiply(w, x)
+        return w.multiply(x.reshape(-1, x.shape[-1])).reshape(*x.shape[:-1], self.out_features)
