@@ -346,7 +346,7 @@ typedef struct llq_few_layer {
  * workspace: llq_moe_few_workspace_size bytes, of this call alone until it is
  * done on the stream.
  */
-size_t llq_moe_few_workspace_size(int64_t T, int k, int E, int I);
+size_t llq_moe_few_workspace_size(int64_t T, int k, int E, int H, int I);
 int llq_moe_few(const llq_few_layer* layer, const void* x, int64_t T, float* logits, float* topk_w,
                 int32_t* topk_ids, void* out, void* workspace, size_t workspace_bytes,
                 void* stream);

@@ -69,7 +69,7 @@ SIGNATURES = {
     "llq_ep_experts_workspace_size": (c_size_t, [I, I, I, I, I]),
     "llq_ep_experts": (I, [P, P, I, I, I, ctypes.c_uint32, P, P, P, P, I, I, I, I, I, L, P, c_size_t, I, P]),
     "llq_ep_combine_wait": (I, [P, I, I, I, ctypes.c_uint32, P, L, I, I, P, P]),
-    "llq_moe_few_workspace_size": (c_size_t, [L, I, I, I]),
+    "llq_moe_few_workspace_size": (c_size_t, [L, I, I, I, I]),
     "llq_moe_few": (I, [P, P, L, P, P, P, P, P, c_size_t, P]),
     "llq_fp8_quantize": (I, [P, I, L, L, L, I, P, L, P, P]),
     "llq_fp8_linear_workspace_size": (c_size_t, [L, I, I, I]),

@@ -346,7 +346,9 @@ int llq_moe_block_packed(const void* x, const void* gate_w, const float* bias, i
   return experts_after_align(ws, x, qw1, sw1, qw2, sw2, topk_w, T, E, H, I, k, bits, group_size, out, impl, st);
 }
 
-size_t llq_moe_few_workspace_size(int64_t T, int k, int E, int I) { return moe_few_workspace(T, k, E, I); }
+size_t llq_moe_few_workspace_size(int64_t T, int k, int E, int H, int I) {
+  return moe_few_workspace(T, k, E, H, I);
+}
 
 int llq_moe_few(const llq_few_layer* layer, const void* x, int64_t T, float* logits, float* topk_w,
                 int32_t* topk_ids, void* out, void* workspace, size_t workspace_bytes, void* stream) {

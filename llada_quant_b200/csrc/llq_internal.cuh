@@ -51,7 +51,7 @@ int gemm12_fused_bf16_tc(const void* x_sorted, const int32_t* offsets, const int
 constexpr int64_t kPrefillRowsPerExpert = 512;
 int dense_linear_tc(const void* x, int64_t M, int K, int N, const int8_t* q, const float* scale, int bits,
                     int group_size, void* out, void* workspace, size_t ws_bytes, cudaStream_t st);
-size_t moe_few_workspace(int64_t T, int k, int E, int I);
+size_t moe_few_workspace(int64_t T, int k, int E, int H, int I);
 int moe_few(const llq_few_layer& L, const void* x, int64_t T, float* logits, float* topk_w, int32_t* topk_ids,
             void* out, void* workspace, size_t bytes, cudaStream_t st);
 int fp8_quantize(const void* x, int x_dtype, int64_t M, int64_t K, int64_t ldx, int block_rows, uint8_t* codes,

@@ -11,25 +11,30 @@
 // too few tokens to fill a tcgen05 tile (8 of 64 experts get one token each), so the products run
 // on mma.sync m16n8k16 with the weights as the 16 rows and up to 8 tokens as the columns: a lane's
 // 16 (INT4) or 32 (INT8) contiguous bytes of a row are its k slots of the 8 MMAs of one 128-group,
-// so nothing is transposed or repacked between memory and MMA.  The integer codes are exact in
-// bf16; each group's partial sum is multiplied by the group's scale in fp32.
+// so nothing is transposed or repacked between memory and MMA.  The integer codes become exact
+// 16-bit numbers; each group's partial sum is multiplied by the group's scale in fp32.
 //
-// Kernel 1 (router, GEMM1): each cluster of 2 CTAs computes the whole router (half per CTA, exchanged
-// through distributed shared memory), so no grid-wide wait stands between router and experts.  The
-// work is a list of segments (expert, up to 8 of its tokens), each of I / 8 jobs: 8 gate and the 8 up
-// rows, so that SiLU(a) * b is local to a thread.  The CTAs take equal runs of jobs.
-// Kernel 2 (GEMM2, combine): a cluster of 4 CTAs owns 64 output features and splits the list of
-// (segment, 128-group) steps evenly over its 16 warp groups; the partial outputs meet in distributed
-// shared memory and are added in the order of the steps: no atomics, a fixed order of sums.
-// h travels between them as two bf16 numbers, hi + lo (16 significant bits), in the order in which
-// kernel 2's lanes want it, so that the bf16 MMAs add no visible rounding: the layer rounds once, at
-// its end.
+// Kernel 1 (router, GEMM1): each cluster of 2 CTAs computes the whole router (half of K per CTA,
+// exchanged through distributed shared memory), so no grid-wide wait stands between router and
+// experts.  The work is a list of segments (expert, up to 8 of its tokens), each of I / 8 jobs: 8
+// gate and the 8 up rows, so that SiLU(a) * b is local to a thread.  The CTAs take equal runs of jobs.
+// Kernel 2 (GEMM2, combine): the CTAs of a panel of 128 output features split the list of (segment,
+// 128-group) steps evenly; each stores its partial outputs, and the one that finishes last adds them
+// in the order of the steps: no waits, and a fixed order of sums.
+// The tokens enter kernel 1 as fp16, each 128-group scaled by a power of two so that its largest
+// magnitude lies in [2^14, 2^15): exact for every bf16 value within 2^-31 of the largest, and what is
+// lost below is 2^-40 of it.  (fp16 rather than bf16 because its ten mantissa bits take an INT8 code, or
+// the upper nibble of a byte, where it lies: 40 instead of 56 logic instructions per lane and 128-group at
+// INT4, 48 instead of 96 at INT8; the logic pipe is what bounds the arithmetic.)  h travels between the
+// kernels as two bf16 numbers, hi + lo (16 significant bits).  So no MMA adds a visible rounding: the
+// layer rounds once, at its end.
 //
 // The packed bytes and their scales reach shared memory by TMA (swizzled) into rings that are deep
 // enough for HBM's latency; the tokens lie in shared memory in MMA order.  Measured on the way
 // (32 tokens, INT4, both kernels): lanes loading their own bytes with cp.async and their tokens from L1,
 // 132 us, bound by the L1 wavefronts that eight scattered rows per instruction cost; a register ring
-// unrolled over its slots, 527 us, its code larger than the instruction cache.
+// unrolled over its slots, 527 us, its code larger than the instruction cache; TMA rings whose refill one
+// lane computed while its warp waited, 94 us.
 #include <algorithm>
 
 #include <cooperative_groups.h>
@@ -49,16 +54,25 @@ constexpr int MAX_K = 32;
 constexpr int MAX_SEG = MAX_EXP + MAX_T * MAX_K / 8;
 constexpr int CL1 = 2;        // CTAs of a cluster of kernel 1: all 148 SMs hold one (of 8, with this much
                               // shared memory, only 120 CTAs fit at once)
-constexpr int CL2 = 4;        // of kernel 2: 132 fit
 constexpr int WARPS = 16;
 constexpr int THREADS = WARPS * 32;
 constexpr int KG = 128;       // K elements of a step: 32 for each of a quad's four lanes
 
-// what kernel 1 tells kernel 2 about the routing: the segments
+constexpr int MAX_SPLIT = 16;  // CTAs of a panel in kernel 2
+constexpr int MAX_PANELS = 64;
+
+// an expert and up to 8 of its tokens, ascending: the columns of its MMAs
+struct Segment {
+  int32_t expert, n;
+  uint64_t tokens;  // a byte each
+  __device__ __forceinline__ int token(int c) const { return static_cast<int>(tokens >> (8 * c)) & 0xff; }
+};
+
+// what kernel 1 tells kernel 2 about the routing
 struct FewPlan {
+  Segment seg[MAX_SEG];
   int32_t n;
-  int32_t expert[MAX_SEG];
-  uint32_t mask[MAX_SEG];     // tokens, at most 8: the columns of the segment, ascending
+  int32_t done[MAX_PANELS];  // kernel 2's CTAs that have stored their part of a panel
 };
 
 struct FewArgs {
@@ -83,6 +97,8 @@ struct FewArgs {
   // segment's tokens; plane 0 holds the hi parts, plane 1 the lo parts, but with at most 4 tokens the lo parts are
   // columns 4 to 7 of plane 0 and half of the bytes and MMAs fall away.
   uint4* h;
+  float* partial;        // [panel][split][128 features][T]
+  int split;             // CTAs of a panel in kernel 2
   __nv_bfloat16* out;
 };
 
@@ -92,6 +108,13 @@ struct FewArgs {
 __device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                          uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                        uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
@@ -107,37 +130,66 @@ __device__ __forceinline__ float lds4(uint32_t a) {
   return v;
 }
 
-// two int4 codes of a word (its nibbles 0 and 4) as a bf16 pair, 136 too large: the xor puts q + 8 into the low
-// mantissa bits of 128
-constexpr float kBias4 = 136.f;
-__device__ __forceinline__ uint32_t int4_biased(uint32_t w) {
-  uint32_t t;
-  asm("lop3.b32 %0, %1, 0x000F000F, 0x43084308, 0x6A;" : "=r"(t) : "r"(w));
-  return t;
+__device__ __forceinline__ uint32_t and_xor(uint32_t x, uint32_t mask, uint32_t k) {
+  uint32_t r;
+  asm("lop3.b32 %0, %1, %2, %3, 0x6A;" : "=r"(r) : "r"(x), "r"(mask), "r"(k));
+  return r;
 }
-// and exactly
-__device__ __forceinline__ uint32_t int4_pair(uint32_t w) {
-  uint32_t o;
-  asm("add.rn.bf16x2 %0, %1, %2;" : "=r"(o) : "r"(int4_biased(w)), "r"(0xC308C308u));
-  return o;
+__device__ __forceinline__ uint32_t add_bf16x2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("add.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
 }
-
-// two int8 codes, one in the low byte of each half: the low seven bits in the mantissa of 128, minus
-// 128 (code >= 0) or 256 (code < 0: its sign bit is the exponent step between the two)
-__device__ __forceinline__ uint32_t int8_pair(uint32_t b) {
-  uint32_t m, c, o;
-  asm("lop3.b32 %0, %1, 0x007F007F, 0x43004300, 0xEA;" : "=r"(m) : "r"(b));
-  asm("lop3.b32 %0, %1, 0x00800080, 0xC300C300, 0xEA;" : "=r"(c) : "r"(b));
-  asm("add.rn.bf16x2 %0, %1, %2;" : "=r"(o) : "r"(m), "r"(c));
-  return o;
+__device__ __forceinline__ uint32_t add_f16x2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("add.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+__device__ __forceinline__ uint32_t fma_f16x2(uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t r;
+  asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+  return r;
 }
 
-// A lane's 32 codes of a row for one step, from rows of 128 bytes (128-byte swizzle) or 64 bytes (64-byte swizzle).
+// Eight codes as four pairs of 16-bit numbers, exactly: INT4 (0,4) (1,5) (2,6) (3,7), INT8 (0,2) (1,3) (4,6) (5,7).
+// fp16, for kernel 1.  INT4: the xor puts q + 8 into the low mantissa bits of 1024 (one is 1) or the next four (one is
+// 16), and 1032, or a sixteenth and 72, bring it back.  INT8: the byte xor 128 is q + 128 in the mantissa of 1024.
+__device__ __forceinline__ void pairs4_f16(uint32_t w, uint32_t (&p)[4]) {
+  const uint32_t y = w >> 8;
+  p[0] = add_f16x2(and_xor(w, 0x000F000Fu, 0x64086408u), 0xE408E408u);
+  p[1] = fma_f16x2(and_xor(w, 0x00F000F0u, 0x64806480u), 0x2C002C00u, 0xD480D480u);
+  p[2] = add_f16x2(and_xor(y, 0x000F000Fu, 0x64086408u), 0xE408E408u);
+  p[3] = fma_f16x2(and_xor(y, 0x00F000F0u, 0x64806480u), 0x2C002C00u, 0xD480D480u);
+}
+__device__ __forceinline__ void pairs8_f16(uint32_t w, uint32_t& p0, uint32_t& p1) {
+  const uint32_t x = w ^ 0x80808080u;
+  p0 = add_f16x2(__byte_perm(x, 0x64646464u, 0x4240u), 0xE480E480u);
+  p1 = add_f16x2(__byte_perm(x, 0x64646464u, 0x4341u), 0xE480E480u);
+}
+// bf16, for kernel 2, whose h has no bound that fp16 could be scaled by.  INT4: q + 8 in the low mantissa bits of 128.
+// INT8: the low seven bits in the mantissa of 128, minus 128 (code >= 0) or 256 (code < 0: its sign bit is the
+// exponent step between the two).
+__device__ __forceinline__ void pairs4_bf16(uint32_t w, uint32_t (&p)[4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) p[i] = add_bf16x2(and_xor(w >> (4 * i), 0x000F000Fu, 0x43084308u), 0xC308C308u);
+}
+__device__ __forceinline__ uint32_t and_or(uint32_t x, uint32_t mask, uint32_t k) {
+  uint32_t r;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(x), "r"(mask), "r"(k));
+  return r;
+}
+__device__ __forceinline__ void pairs8_bf16(uint32_t w, uint32_t& p0, uint32_t& p1) {
+  const uint32_t y = w >> 8;
+  p0 = add_bf16x2(and_or(w, 0x007F007Fu, 0x43004300u), and_or(w, 0x00800080u, 0xC300C300u));
+  p1 = add_bf16x2(and_or(y, 0x007F007Fu, 0x43004300u), and_or(y, 0x00800080u, 0xC300C300u));
+}
+
+// A lane's 32 codes of a row for one step, from rows of 128 bytes (128-byte swizzle).
 template <int BITS>
 struct Codes {
   static constexpr int STEPS = BITS == 4 ? 2 : 1;  // steps in 128 bytes
   uint4 v[BITS == 4 ? 1 : 2];
-  // Rows of 128 bytes; `row` is the address of row r (mod 8), `step` the step in it.  With row_of(g) as lane g's row
+  // `row` is the address of row r (mod 8), `step` the step in it.  With row_of(g) as lane g's row
   // the eight lanes that a shared-memory access serves at a time (two rows) meet eight different 16-byte columns.
   static __device__ __forceinline__ int row_of(int g) { return BITS == 4 ? ((g & 1) << 2) | (g >> 1) : g; }
   __device__ __forceinline__ void load128(uint32_t row, int r, int step, int t) {
@@ -148,58 +200,36 @@ struct Codes {
       v[1] = lds16(row + (((2 * t + 1) ^ r) << 4));
     }
   }
-  // rows of one step, 64 bytes at INT4; lane g's row is g
-  __device__ __forceinline__ void load_step(uint32_t row, int g, int t) {
-    if (BITS == 4) v[0] = lds16(row + ((t ^ (g >> 1)) << 4));
-    else load128(row, g, 0, t);
-  }
-  // codes 8j .. 8j + 7 as four bf16 pairs: INT4 (0,4) (1,5) (2,6) (3,7), INT8 (0,1) (2,3) (4,5) (6,7)
-  // (BIASED: INT4 ones 136 too large)
-  template <bool BIASED>
+  // codes 8j .. 8j + 7
+  template <bool F16>
   __device__ __forceinline__ void pairs(int j, uint32_t (&p)[4]) const {
     if (BITS == 4) {
       const uint32_t w = j == 0 ? v[0].x : j == 1 ? v[0].y : j == 2 ? v[0].z : v[0].w;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) p[i] = BIASED ? int4_biased(w >> (4 * i)) : int4_pair(w >> (4 * i));
+      if (F16) pairs4_f16(w, p);
+      else pairs4_bf16(w, p);
     } else {
       const uint4 u = v[j >> 1];
       const uint32_t w0 = (j & 1) ? u.z : u.x, w1 = (j & 1) ? u.w : u.y;
-      p[0] = int8_pair(__byte_perm(w0, 0, 0x4140));
-      p[1] = int8_pair(__byte_perm(w0, 0, 0x4342));
-      p[2] = int8_pair(__byte_perm(w1, 0, 0x4140));
-      p[3] = int8_pair(__byte_perm(w1, 0, 0x4342));
+      if (F16) {
+        pairs8_f16(w0, p[0], p[1]);
+        pairs8_f16(w1, p[2], p[3]);
+      } else {
+        pairs8_bf16(w0, p[0], p[1]);
+        pairs8_bf16(w1, p[2], p[3]);
+      }
     }
   }
 };
 
-// 8 bf16 of a token in natural order -> the pairs of Codes::pairs
+// the element of 8 that stands at place i of the pairs, and the place of element n of h
 template <int BITS>
-__device__ __forceinline__ void token_pairs(uint4 x, uint32_t (&p)[4]) {
-  if (BITS == 4) {
-    p[0] = __byte_perm(x.x, x.z, 0x5410);
-    p[1] = __byte_perm(x.x, x.z, 0x7632);
-    p[2] = __byte_perm(x.y, x.w, 0x5410);
-    p[3] = __byte_perm(x.y, x.w, 0x7632);
-  } else {
-    p[0] = x.x;
-    p[1] = x.y;
-    p[2] = x.z;
-    p[3] = x.w;
-  }
+__device__ __forceinline__ constexpr int pair_element(int i) {
+  return BITS == 4 ? (i >> 1) + 4 * (i & 1) : (i & 4) + ((i >> 1) & 1) + 2 * (i & 1);
 }
-
-// position of feature n of h in the order of Codes::pairs
 template <int BITS>
-__device__ __forceinline__ int pair_pos(int n) {
-  if (BITS != 4) return n;
+__device__ __forceinline__ int pair_place(int n) {
   const int j = n & 7;
-  return (n & ~7) | (j < 4 ? 2 * j : 2 * j - 7);
-}
-
-// the i-th set bit of m (i below the number of its bits, at most 8 here)
-__device__ __forceinline__ int nth_bit(uint32_t m, int i) {
-  for (; i > 0; --i) m &= m - 1;
-  return __ffs(m) - 1;
+  return BITS == 4 ? (j < 4 ? 2 * j : 2 * j - 7) : (j & 4) + 2 * (j & 1) + ((j >> 1) & 1);
 }
 
 // The scale of step s of a row: where a row has a multiple of 4 of them, a copy brings the aligned four that hold it
@@ -229,28 +259,28 @@ constexpr int TILE1 = 2048;      // 8 gate and 8 up rows of 128 bytes: one copy
 constexpr int SLOT1 = 2 * TILE1;
 constexpr int SCALE1 = 256;      // the same 16 rows' four scales
 constexpr int RED_SLICES = 8;
-constexpr int RED_BYTES = RED_SLICES * 64 * MAX_T * 4;
+constexpr int RED_PITCH = MAX_T + 1;
+constexpr int RED_BYTES = RED_SLICES * 64 * RED_PITCH * 4;
 constexpr int ROUTER_BYTES = RED_BYTES + CL1 * MAX_EXP * MAX_T * 4;  // over the rings and tokens, before they are used
 
 struct Smem1 {
   float w[MAX_T][MAX_K];         // the routing, as the caller brings it or gets it
   int16_t ids[MAX_T][MAX_K];     // (experts out of range as -1)
   uint32_t mask[MAX_EXP];        // tokens of every expert
-  int32_t expert[MAX_SEG];       // the segments
-  uint32_t seg_mask[MAX_SEG];
+  Segment seg[MAX_SEG];
   float col_w[2][8];             // the columns' weights of the segments at hand
-  float sum[2][64][8];           // and 136 times the sums of the steps of their tokens
+  float col_scale[2][64][8];     // what undoes the scaling of a step of a column's token
   float4 head[WARPS][32];        // a warp's part of a job that an earlier warp began
   uint64_t full[WARPS][MAX_DEPTH1];  // a slot of a warp's ring has landed
   int32_t nseg;
   int abort_flag;
 };
 
-using LogitPart = float[MAX_EXP][MAX_T];
+using LogitPart = float[MAX_T][MAX_EXP];
 
 // The router: K is split over the CTAs of the cluster and eight slices of warps in each; half of the warps take 32 of
 // 64 experts at a time, the others the next 32.  A slice's sums meet in `red`, a CTA's in parts[rank] of both CTAs.
-__device__ void router_logits(const FewArgs& a, float (*red)[64][MAX_T], LogitPart* parts, cg::cluster_group& cluster) {
+__device__ void router_logits(const FewArgs& a, float (*red)[64][RED_PITCH], LogitPart* parts, cg::cluster_group& cluster) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int ntiles = (a.T + 7) / 8;
   const int rank = static_cast<int>(cluster.block_rank());
@@ -298,19 +328,18 @@ __device__ void router_logits(const FewArgs& a, float (*red)[64][MAX_T], LogitPa
           float* r = &red[slice][half * 32 + m * 16 + g][n * 8 + 2 * t];
           r[0] = d[m][n][0];
           r[1] = d[m][n][1];
-          r[8 * MAX_T] = d[m][n][2];
-          r[8 * MAX_T + 1] = d[m][n][3];
+          r[8 * RED_PITCH] = d[m][n][2];
+          r[8 * RED_PITCH + 1] = d[m][n][3];
         }
     __syncthreads();
-    const int tw = ntiles * 8;
-    for (int i = threadIdx.x; i < 64 * tw; i += THREADS) {
-      const int r = i / tw, tok = i - r * tw;
+    for (int i = threadIdx.x; i < 64 * a.T; i += THREADS) {
+      const int r = i & 63, tok = i >> 6;
       if (eg + r < a.E) {
         float z = 0.f;
 #pragma unroll
         for (int k = 0; k < RED_SLICES; ++k) z = __fadd_rn(z, red[k][r][tok]);
 #pragma unroll
-        for (int c = 0; c < CL1; ++c) *cluster.map_shared_rank(&parts[rank][eg + r][tok], c) = z;
+        for (int c = 0; c < CL1; ++c) *cluster.map_shared_rank(&parts[rank][tok][eg + r], c) = z;
       }
     }
     if (eg + 64 < a.E) __syncthreads();
@@ -318,7 +347,7 @@ __device__ void router_logits(const FewArgs& a, float (*red)[64][MAX_T], LogitPa
 }
 
 __device__ __forceinline__ float logit_of(const FewArgs& a, const LogitPart* parts, int e, int tok) {
-  float z = __fadd_rn(parts[0][e][tok], parts[1][e][tok]);
+  float z = __fadd_rn(parts[0][tok][e], parts[1][tok][e]);
   if (a.bias != nullptr) z = __fadd_rn(z, __ldg(a.bias + e));
   return z;
 }
@@ -412,10 +441,6 @@ __device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
 }
 
-__device__ __forceinline__ void prefetch_l2(const void* p, uint32_t bytes) {
-  asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p), "r"(bytes) : "memory");
-}
-
 // TS: scales by copies
 template <int BITS, bool TS>
 __global__ void __launch_bounds__(THREADS, 1)
@@ -446,7 +471,7 @@ __global__ void __launch_bounds__(THREADS, 1)
 
   if (a.gate != nullptr) {
     LogitPart* parts = reinterpret_cast<LogitPart*>(base + RED_BYTES);
-    router_logits(a, reinterpret_cast<float (*)[64][MAX_T]>(base), parts, cluster);
+    router_logits(a, reinterpret_cast<float (*)[64][RED_PITCH]>(base), parts, cluster);
     cluster.sync();  // every CTA's sums are in every CTA
     if (a.E > 64) {
       for (int tok = warp; tok < a.T; tok += WARPS) choose<MAX_EXP / 32, 1>(a, sm, parts, tok);
@@ -487,14 +512,9 @@ __global__ void __launch_bounds__(THREADS, 1)
         if (lane >= o) incl += v;
       }
       for (int i = n + incl - mine; m != 0; ++i) {
-        uint32_t rest = 0;
-        if (__popc(m) > 8) {  // the lowest 8 tokens, then the others
-          rest = m;
-          for (int b = 0; b < 8; ++b) rest &= rest - 1;
-        }
-        sm.expert[i] = e0 + lane;
-        sm.seg_mask[i] = m ^ rest;
-        m = rest;
+        Segment g1{e0 + lane, 0, 0};
+        for (; m != 0 && g1.n < 8; m &= m - 1) g1.tokens |= static_cast<uint64_t>(__ffs(m) - 1) << (8 * g1.n++);
+        sm.seg[i] = g1;
       }
       n += __shfl_sync(0xffffffffu, incl, 31);
     }
@@ -523,74 +543,54 @@ __global__ void __launch_bounds__(THREADS, 1)
   uint8_t* sring = base + WARPS * a.depth1 * SLOT1 + warp * a.depth1 * SCALE1;
   volatile int* abort_flag = &sm.abort_flag;
   auto window_end = [&](int wb) { return min(end, (wb / tiles + a.nbuf) * tiles); };
-  // this warp's units of window [wb, we): [first, last)
+  // the units (slots of jobs, in order) of window [wb, we) that warp w begins at
   auto unit = [&](int wb, int we, int w) { return static_cast<int>(static_cast<int64_t>(we - wb) * slots * w / WARPS); };
 
   // what is copied next: slot lz of row block lrow of expert half lhalf; lleft units are left in the window at lwb
-  int lwb = begin, lu = 0, lleft = 0, lz = 0, lrow = 0, lhalf = 0, lslot = 0;
-  auto place = [&]() {
-    const int job = lwb + lu / slots, seg = job / tiles;
-    lz = lu % slots;
-    lrow = (job - seg * tiles) * 8;
-    lhalf = sm.expert[seg] * 2;
-  };
+  int lwb = begin, lleft = 0, lz = 0, lseg = 0, lrow = 0, lhalf = 0, lslot = 0;
   auto open = [&]() {  // the first window from lwb on in which this warp has units
     for (; lwb < end; lwb = window_end(lwb)) {
-      const int we = window_end(lwb);
-      lu = unit(lwb, we, warp);
-      lleft = unit(lwb, we, warp + 1) - lu;
+      const int we = window_end(lwb), u = unit(lwb, we, warp);
+      lleft = unit(lwb, we, warp + 1) - u;
       if (lleft > 0) {
-        place();
+        const int job = lwb + u / slots;
+        lz = u % slots;
+        lseg = job / tiles;
+        lrow = (job - lseg * tiles) * 8;
+        lhalf = sm.seg[lseg].expert * 2;
         return;
       }
     }
   };
-  auto fetch = [&]() {  // (lane 0; lwb < end)
+  // The whole warp follows the cursor and three lanes issue a copy each (two tiles, the scales): one lane doing it all
+  // held the warp up for 950 cycles a slot.
+  const CUtensorMap* lmap = lane == 2 ? &tm_s : &tm_w;
+  auto fetch = [&]() {
     uint64_t* bar = &sm.full[warp][lslot];
-    uint8_t* dst = ring + lslot * SLOT1;
     const bool two = lz * 256 + 128 < kb;
-    mbar_expect_tx(bar, SLOT1 - (two ? 0 : TILE1) + (TS ? SCALE1 : 0));
-    tma_load_3d(dst, &tm_w, lz * 256, lrow, lhalf, bar);
-    if (two) tma_load_3d(dst + TILE1, &tm_w, lz * 256 + 128, lrow, lhalf, bar);
-    if (TS) tma_load_3d(sring + lslot * SCALE1, &tm_s, scale_index(lz * 2 * SS, a.gsteps1) & ~3, lrow, lhalf, bar);
+    if (lane == 0) mbar_expect_tx(bar, SLOT1 - (two ? 0 : TILE1) + (TS ? SCALE1 : 0));
+    __syncwarp();
+    uint8_t* dst = lane == 2 ? sring + lslot * SCALE1 : ring + lslot * SLOT1 + lane * TILE1;
+    const int x = lane == 2 ? scale_index(lz * 2 * SS, a.gsteps1) & ~3 : lz * 256 + lane * 128;
+    if (lane == 0 || (lane == 1 && two) || (lane == 2 && TS)) tma_load_3d(dst, lmap, x, lrow, lhalf, bar);
     if (++lslot == a.depth1) lslot = 0;
     if (--lleft == 0) {
       lwb = window_end(lwb);
       open();
-    } else {
-      ++lu;
-      if (++lz == slots) place();
+    } else if (++lz == slots) {
+      lz = 0;
+      lrow += 8;
+      if (lrow == a.I) {
+        lrow = 0;
+        lhalf = sm.seg[++lseg].expert * 2;
+      }
     }
   };
-  // once its own copies are on their way, every warp asks for its share of w2 and its scales: HBM stays busy until
-  // kernel 2 runs, which then finds them in L2 (while they fit: half of it)
-  bool asked = lane != 0 || static_cast<int64_t>(nseg) * a.H * a.I * BITS / 8 > (64 << 20);
-  auto ask = [&]() {
-    asked = true;
-    const int64_t wbytes = static_cast<int64_t>(a.H) * a.I * BITS / 8, sbytes = static_cast<int64_t>(a.H) * a.groups2 * 4;
-    constexpr int PIECE = 8192;
-    const int wp = static_cast<int>((wbytes + PIECE - 1) / PIECE);
-    const int sp = (reinterpret_cast<uintptr_t>(a.s2) & 15) ? 0 : static_cast<int>((sbytes + PIECE - 1) / PIECE);
-    for (int64_t i = static_cast<int64_t>(cta) * WARPS + warp; i < static_cast<int64_t>(nseg) * (wp + sp); i += grid * WARPS) {
-      const int s = static_cast<int>(i / (wp + sp)), p = static_cast<int>(i - static_cast<int64_t>(s) * (wp + sp));
-      const int64_t e = sm.expert[s];
-      if (s > 0 && sm.expert[s - 1] == e) continue;
-      const int64_t off = static_cast<int64_t>(p < wp ? p : p - wp) * PIECE, all = p < wp ? wbytes : sbytes;
-      const char* at = p < wp ? reinterpret_cast<const char*>(a.q2) + e * wbytes : reinterpret_cast<const char*>(a.s2) + e * sbytes;
-      prefetch_l2(at + off, static_cast<uint32_t>(min(static_cast<int64_t>(PIECE), all - off)) & ~15u);
-    }
-  };
-  if (lane == 0) {
-    open();
-    for (int i = 0; i < a.depth1 && lwb < end; ++i) fetch();
-    if (lwb >= end && !asked) ask();
-  }
-  __syncwarp();
+  open();
+  for (int i = 0; i < a.depth1 && lwb < end; ++i) fetch();
   if (cta == 0) {
-    for (int i = threadIdx.x; i < nseg; i += THREADS) {
-      a.plan->expert[i] = sm.expert[i];
-      a.plan->mask[i] = sm.seg_mask[i];
-    }
+    for (int i = threadIdx.x; i < nseg; i += THREADS) a.plan->seg[i] = sm.seg[i];
+    if (threadIdx.x < MAX_PANELS) a.plan->done[threadIdx.x] = 0;
     if (threadIdx.x == 0) a.plan->n = nseg;
   }
 
@@ -601,44 +601,64 @@ __global__ void __launch_bounds__(THREADS, 1)
   bool ok = true;
   for (int wb = begin; wb < end; wb = window_end(wb)) {
     const int we = window_end(wb), seg0 = wb / tiles, nsegs = (we - 1) / tiles - seg0 + 1;
-    __syncthreads();  // the tokens of the window before are done with
-    for (int b = 0; b < nsegs; ++b) {
-      const int e = sm.expert[seg0 + b];
-      const uint32_t mask = sm.seg_mask[seg0 + b];
-      const int ntok = __popc(mask), row = xf_pieces / 8;  // 16-byte pieces of a token, a multiple of 16
-      for (int i0 = warp * 32; i0 < row * ntok; i0 += THREADS) {
-        const int i = i0 + lane;
-        const int c = i / row, p = i - c * row;               // column, piece of its row
+    if (wb > begin) __syncthreads();  // the tokens of the window before are done with
+    // the segments' tokens to fp16 in MMA order, eight 16-byte pieces in flight per thread
+    const int row = xf_pieces / 8;  // pieces of a token with the zeros behind it, a multiple of 16
+    const int n0 = sm.seg[seg0].n, cols = n0 + (nsegs > 1 ? sm.seg[seg0 + 1].n : 0);
+    for (int i0 = 0; i0 < row * cols; i0 += 8 * THREADS) {
+      uint4 v[8];
+#pragma unroll
+      for (int q = 0; q < 8; ++q) {
+        const int i = i0 + q * THREADS + static_cast<int>(threadIdx.x), cc = i / row, p = i - cc * row;
+        const int b = cc >= n0;
+        v[q] = make_uint4(0, 0, 0, 0);
+        if (cc < cols && p * 8 < a.H)
+          v[q] = __ldg(reinterpret_cast<const uint4*>(a.x + static_cast<int64_t>(sm.seg[seg0 + b].token(cc - b * n0)) * a.H) + p);
+      }
+#pragma unroll
+      for (int q = 0; q < 8; ++q) {
+        const int i = i0 + q * THREADS + static_cast<int>(threadIdx.x), cc = i / row, p = i - cc * row;
+        const int b = cc >= n0, c = cc - b * n0;
         const int s = p >> 4, pt = (p >> 2) & 3, pj = p & 3;  // step, lane of the quad, piece of the lane
-        uint4 v = make_uint4(0, 0, 0, 0);
-        if (c < ntok && p * 8 < a.H)
-          v = __ldg(reinterpret_cast<const uint4*>(a.x + static_cast<int64_t>(nth_bit(mask, c)) * a.H) + p);
-        uint32_t q[4];
-        token_pairs<BITS>(v, q);
-        if (c < ntok) xf[b * xf_pieces + (s * 4 + pj) * 32 + c * 4 + pt] = make_uint4(q[0], q[1], q[2], q[3]);
-        if (BITS == 4) {  // the token's sum over the step, for the bias of the codes
-          float sum = 0.f;
+        const uint32_t w[4] = {v[q].x, v[q].y, v[q].z, v[q].w};
+        float f[8];
+        uint32_t m = 0;
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            sum = __fadd_rn(sum, __fadd_rn(__uint_as_float(q[k] << 16), __uint_as_float(q[k] & 0xffff0000u)));
+        for (int k = 0; k < 4; ++k) {
+          f[2 * k] = __uint_as_float(w[k] << 16);
+          f[2 * k + 1] = __uint_as_float(w[k] & 0xffff0000u);
+          m = max(m, max(w[k] & 0x7fff0000u, (w[k] << 16) & 0x7fffffffu));
+        }
 #pragma unroll
-          for (int o = 8; o > 0; o >>= 1) sum = __fadd_rn(sum, __shfl_xor_sync(0xffffffffu, sum, o));
-          if ((lane & 15) == 0 && c < ntok) sm.sum[b][s][c] = sum * kBias4;
+        for (int o = 8; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));  // the step's 16 pieces
+        const uint32_t e = min(max(m >> 23, 15u), 254u);  // largest magnitude in [2^(e-127), 2^(e-126))
+        const float up = __uint_as_float((268u - e) << 23);
+        uint32_t h[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const __half2 pr = __floats2half2_rn(f[pair_element<BITS>(2 * k)] * up, f[pair_element<BITS>(2 * k + 1)] * up);
+          h[k] = *reinterpret_cast<const uint32_t*>(&pr);
+        }
+        if (cc < cols) {
+          xf[b * xf_pieces + (s * 4 + pj) * 32 + c * 4 + pt] = make_uint4(h[0], h[1], h[2], h[3]);
+          if ((p & 15) == 0) sm.col_scale[b][s][c] = __uint_as_float((e - 14u) << 23);
         }
       }
-      if (threadIdx.x < ntok) {
-        const int tok = nth_bit(mask, threadIdx.x);
-        float w = 0.f;
-        for (int i = 0; i < a.k; ++i)
-          if (sm.ids[tok][i] == e) w = __fadd_rn(w, sm.w[tok][i]);
-        sm.col_w[b][threadIdx.x] = w;
-      }
+    }
+    if (threadIdx.x < cols) {
+      const int b = static_cast<int>(threadIdx.x) >= n0, c = static_cast<int>(threadIdx.x) - b * n0;
+      const Segment sg = sm.seg[seg0 + b];
+      const int tok = sg.token(c);
+      float w = 0.f;
+      for (int i = 0; i < a.k; ++i)
+        if (sm.ids[tok][i] == sg.expert) w = __fadd_rn(w, sm.w[tok][i]);
+      sm.col_w[b][c] = w;
     }
     __syncthreads();
 
     // h of a finished job
     auto emit = [&](int job, const float (&acc)[4]) {
-      const int seg = job / tiles, rb = job - seg * tiles, ntok = __popc(sm.seg_mask[seg]);
+      const int seg = job / tiles, rb = job - seg * tiles, ntok = sm.seg[seg].n;
       const bool packed = ntok <= 4;
       // feature n = 8 rb + r of columns 2t and 2t + 1: its place in the 16 bytes of 8 features that rb is
       const int n = rb * 8 + r, s = n / KG, pt = (n % KG) / 32, pj = (n % 32) / 8;
@@ -650,7 +670,7 @@ __global__ void __launch_bounds__(THREADS, 1)
           const float ga = acc[i], up = acc[2 + i];
           const float h = __fdiv_rn(ga, 1.f + expf(-ga)) * up * sm.col_w[seg - seg0][col];
           const __nv_bfloat16 hi = __float2bfloat16_rn(h);
-          __nv_bfloat16* at = reinterpret_cast<__nv_bfloat16*>(step + col * 4) + (pair_pos<BITS>(n) & 7);
+          __nv_bfloat16* at = reinterpret_cast<__nv_bfloat16*>(step + col * 4) + pair_place<BITS>(n);
           at[0] = hi;
           at[(packed ? 16 : 128) * 8] = __float2bfloat16_rn(h - __bfloat162float(hi));  // four columns, or a plane, further
         }
@@ -662,59 +682,58 @@ __global__ void __launch_bounds__(THREADS, 1)
         }
       }
     };
-    const int first = unit(wb, we, warp), last = unit(wb, we, warp + 1);
+    int left = unit(wb, we, warp + 1) - unit(wb, we, warp);
+    int job = wb + unit(wb, we, warp) / slots, za = unit(wb, we, warp) % slots;
     float acc[4] = {0.f, 0.f, 0.f, 0.f};
     int open_job = -1;  // a job that this warp began and a later one ends
-    for (int u = first; u < last && ok;) {
-      const int job = wb + u / slots, za = u % slots, zb = min(slots, za + last - u);
-      const int seg = job / tiles, b = seg - seg0;
-      const int64_t row = static_cast<int64_t>(sm.expert[seg]) * 2 * a.I + (job - seg * tiles) * 8 + r;
-      const float* fg = a.s1 + row * a.groups1;
+    while (left > 0 && ok) {
+      const int zb = min(slots, za + left), seg = job / tiles, b = seg - seg0;
+      left -= zb - za;
+      const int64_t wrow = static_cast<int64_t>(sm.seg[seg].expert) * 2 * a.I + (job - seg * tiles) * 8 + r;
+      const float* fg = a.s1 + wrow * a.groups1;
       const float* fu = fg + static_cast<int64_t>(a.I) * a.groups1;
       float sc = TS ? 0.f : load_scale(fg, fu, za * 2 * SS, steps, a.gsteps1, t);
       acc[0] = acc[1] = acc[2] = acc[3] = 0.f;
-      const uint32_t xb = smem_u32(xf + b * xf_pieces + lane), sb = smem_u32(&sm.sum[b][0][2 * t]);
+      uint32_t xb = smem_u32(xf + b * xf_pieces + lane) + za * (2 * SS * 2048);
+      uint32_t cb = smem_u32(&sm.col_scale[b][za * 2 * SS][2 * t]);
       for (int z = za; z < zb && ok; ++z) {
         ok = mbar_wait(&sm.full[warp][slot], phase, abort_flag, 0x600 + warp);
         const uint32_t tile = smem_u32(ring + slot * SLOT1) + r * 128, sa = smem_u32(sring + slot * SCALE1) + r * 16;
 #pragma unroll
         for (int h = 0; h < 2 * SS; ++h) {  // behind the last step codes and tokens are zero
-          const int s = z * 2 * SS + h;
           float f, v;
           if (TS) {
-            const uint32_t at = sa + (scale_index(s, a.gsteps1) & 3) * 4;
+            const uint32_t at = sa + (scale_index(z * 2 * SS + h, a.gsteps1) & 3) * 4;
             f = lds4(at);
             v = lds4(at + SCALE1 / 2);
           } else {
             quad_scales(sc, f, v);
-            sc = load_scale(fg, fu, s + 1, steps, a.gsteps1, t);
+            sc = load_scale(fg, fu, z * 2 * SS + h + 1, steps, a.gsteps1, t);
           }
+          const float c0 = lds4(cb + h * 32), c1 = lds4(cb + h * 32 + 4);
           Codes<BITS> wg, wu;
           wg.load128(tile + h / SS * TILE1, r, h % SS, t);
           wu.load128(tile + h / SS * TILE1 + TILE1 / 2, r, h % SS, t);
           float d0[4] = {0.f, 0.f, 0.f, 0.f}, d1[4] = {0.f, 0.f, 0.f, 0.f};  // two chains of MMAs
-          if (BITS == 4) {
-            d0[0] = d0[2] = -lds4(sb + s * 32);
-            d0[1] = d0[3] = -lds4(sb + s * 32 + 4);
-          }
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            const uint4 x = lds16(xb + s * 2048 + j * 512);
+            const uint4 x = lds16(xb + h * 2048 + j * 512);
             uint32_t ag[4], au[4];
             wg.template pairs<true>(j, ag);
             wu.template pairs<true>(j, au);
-            mma_bf16(d0, ag[0], au[0], ag[1], au[1], x.x, x.y);
-            mma_bf16(d1, ag[2], au[2], ag[3], au[3], x.z, x.w);
+            mma_f16(d0, ag[0], au[0], ag[1], au[1], x.x, x.y);
+            mma_f16(d1, ag[2], au[2], ag[3], au[3], x.z, x.w);
           }
-#pragma unroll
-          for (int i = 0; i < 4; ++i) acc[i] = __fmaf_rn(i < 2 ? f : v, __fadd_rn(d0[i], d1[i]), acc[i]);
+          acc[0] = __fmaf_rn(f * c0, __fadd_rn(d0[0], d1[0]), acc[0]);
+          acc[1] = __fmaf_rn(f * c1, __fadd_rn(d0[1], d1[1]), acc[1]);
+          acc[2] = __fmaf_rn(v * c0, __fadd_rn(d0[2], d1[2]), acc[2]);
+          acc[3] = __fmaf_rn(v * c1, __fadd_rn(d0[3], d1[3]), acc[3]);
         }
+        xb += 2 * SS * 2048;
+        cb += 2 * SS * 32;
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // our reads of the slot before its refill
         __syncwarp();
-        if (lane == 0 && ok) {
-          if (lwb < end) fetch();
-          else if (!asked) ask();
-        }
+        if (lwb < end && ok) fetch();
         if (++slot == a.depth1) {
           slot = 0;
           phase ^= 1;
@@ -727,7 +746,8 @@ __global__ void __launch_bounds__(THREADS, 1)
       } else {
         open_job = job;
       }
-      u += zb - za;
+      ++job;
+      za = 0;
     }
     __syncthreads();
     if (open_job >= 0) {  // its parts in the order of K
@@ -754,41 +774,42 @@ __global__ void __launch_bounds__(THREADS, 1)
   }
 }
 
-constexpr int MT = 4;                  // 16-row tiles of a panel, one warp of a group each
-constexpr int PANEL = MT * 16;         // output features of a cluster of kernel 2
+constexpr int MT = 8;                  // 16-row tiles of a panel, one warp of a group each
+constexpr int PANEL = MT * 16;         // output features of a CTA of kernel 2
 constexpr int GROUPS = WARPS / MT;     // groups of a CTA, each with a part of the steps
-constexpr int MAX_DEPTH2 = 6;
+constexpr int MAX_DEPTH2 = 4;
+constexpr int THREADS2 = THREADS + 32;  // and a warp that issues the copies
 
 template <int BITS>
-struct Stage2 {  // one step: the panel's packed rows, h, four scales of the rows
-  static constexpr int W = PANEL * KG * BITS / 8;
-  static constexpr int H = 4096;
+struct Stage2 {  // 128 bytes of the panel's packed rows (two steps at INT4, one at INT8), h, four scales of the rows
+  static constexpr int STEPS = Codes<BITS>::STEPS;
+  static constexpr int W = PANEL * 128;
+  static constexpr int H = STEPS * 4096;
   static constexpr int S = PANEL * 16;
   static constexpr int BYTES = W + H + S;
 };
 
 struct Smem2 {
-  int32_t expert[MAX_SEG];
-  uint32_t mask[MAX_SEG];
+  Segment seg[MAX_SEG];
   uint64_t full[GROUPS][MAX_DEPTH2];
   uint64_t empty[GROUPS][MAX_DEPTH2];
   int abort_flag;
+  int last;
 };
 
 template <int BITS, bool TS>
-__global__ void __launch_bounds__(THREADS, 1)
+__global__ void __launch_bounds__(THREADS2, 1)
     few_gemm2_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_s, const FewArgs a) {
   extern __shared__ __align__(1024) uint8_t raw[];
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
   using S = Stage2<BITS>;
+  constexpr int SS = S::STEPS;
   const int depth = a.depth2;
   Smem2& sm = *reinterpret_cast<Smem2*>(base + GROUPS * depth * S::BYTES);
   float* parts = reinterpret_cast<float*>(base + GROUPS * depth * S::BYTES + sizeof(Smem2));  // [GROUPS][PANEL][pitch]
   const int pitch = a.T | 1;
-  cg::cluster_group cluster = cg::this_cluster();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int rank = static_cast<int>(cluster.block_rank());
-  const int panel = blockIdx.x / CL2, tile = warp % MT, group = warp / MT;
+  const int panel = blockIdx.x / a.split, rank = blockIdx.x % a.split, tile = warp % MT, group = warp / MT;
   if (threadIdx.x < GROUPS * MAX_DEPTH2) {
     mbar_init(&sm.full[threadIdx.x / MAX_DEPTH2][threadIdx.x % MAX_DEPTH2], 1);
     mbar_init(&sm.empty[threadIdx.x / MAX_DEPTH2][threadIdx.x % MAX_DEPTH2], MT);
@@ -798,177 +819,207 @@ __global__ void __launch_bounds__(THREADS, 1)
     prefetch_map(&tm_w);
     if (TS) prefetch_map(&tm_s);
   }
-  for (int i = threadIdx.x; i < GROUPS * PANEL * pitch; i += THREADS) parts[i] = 0.f;
+  for (int i = threadIdx.x; i < GROUPS * PANEL * pitch; i += THREADS2) parts[i] = 0.f;
   asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   pdl_wait();
   asm volatile("fence.proxy.async.global;" ::: "memory");  // kernel 1's stores of h before the copies read them
   const int nseg = a.plan->n;
-  if (threadIdx.x < MAX_SEG) {  // what lies behind the last segment is not looked at
-    sm.expert[threadIdx.x] = a.plan->expert[threadIdx.x];
-    sm.mask[threadIdx.x] = a.plan->mask[threadIdx.x];
-  }
+  if (threadIdx.x < MAX_SEG) sm.seg[threadIdx.x] = a.plan->seg[threadIdx.x];  // (those behind the last are not looked at)
   __syncthreads();
 
-  // the steps of all segments in a row; this group has [begin, end) of them
-  const int steps = (a.I + KG - 1) / KG;
-  const int64_t total = static_cast<int64_t>(nseg) * steps;
-  const int piece = rank * GROUPS + group;
-  const int begin = static_cast<int>(total * piece / (CL2 * GROUPS)), end = static_cast<int>(total * (piece + 1) / (CL2 * GROUPS));
-  uint8_t* ring = base + group * depth * S::BYTES;
+  // the slots (a stage each) of all segments in a row; a group has [begin, end) of them
+  const int steps = (a.I + KG - 1) / KG, slots = (steps + SS - 1) / SS;
+  const int64_t total = static_cast<int64_t>(nseg) * slots;
+  auto bound = [&](int grp) { return static_cast<int>(total * (rank * GROUPS + grp) / (a.split * GROUPS)); };
   volatile int* abort_flag = &sm.abort_flag;
-  int lat = begin, lseg = begin / steps, ls = begin - lseg * steps, lst = 0, lrow = 0, lh = 0;  // the step to be copied next
-  auto place = [&]() {
-    lrow = sm.expert[lseg] * a.H + panel * PANEL;
-    lh = __popc(sm.mask[lseg]) <= 4 ? S::H / 2 : S::H;
-  };
-  if (begin < end) place();
-  auto fetch = [&]() {  // (one lane of the group)
-    uint64_t* bar = &sm.full[group][lst];
-    uint8_t* dst = ring + lst * S::BYTES;
-    mbar_expect_tx(bar, S::W + lh + (TS ? S::S : 0));
-    tma_load_2d(dst, &tm_w, ls * (KG * BITS / 8), lrow, bar);
-    bulk_load(dst + S::W, a.h + static_cast<int64_t>(lat) * 256, lh, bar);
-    if (TS) tma_load_2d(dst + S::W + S::H, &tm_s, scale_index(ls, a.gsteps2) & ~3, lrow, bar);
-    if (++lst == depth) lst = 0;
-    ++lat;
-    if (++ls == steps) {
-      ls = 0;
-      if (++lseg < nseg) place();
-    }
-  };
-  if (tile == 0 && lane == 0)
-    for (int i = 0; i < depth && lat < end; ++i) fetch();
 
-  const int r0 = tile * 16 + g;  // this lane's rows of the panel: r0 and r0 + 8
-  const int n0 = min(panel * PANEL + r0, a.H - 1), n1 = min(panel * PANEL + r0 + 8, a.H - 1);
-  bool ok = true;
-  int st = 0, prev = 0;  // the stage to be read, and the one read before
-  uint32_t phase = 0, pphase = 0;
-  for (int at = begin; at < end && ok;) {
-    const int seg = at / steps, sa = at - seg * steps, sb = min(steps, sa + end - at);
-    const int64_t e = sm.expert[seg];
-    const uint32_t mask = sm.mask[seg];
-    const int ntok = __popc(mask);
-    const bool packed = ntok <= 4;
-    const float* f0 = a.s2 + (e * a.H + n0) * a.groups2;
-    const float* f1 = a.s2 + (e * a.H + n1) * a.groups2;
-    float acc[4] = {0.f, 0.f, 0.f, 0.f};
-    float sc = TS ? 0.f : load_scale(f0, f1, sa, sb, a.gsteps2, t);
-    for (int s = sa; s < sb; ++s, ++at) {
-      const float scn = TS ? 0.f : load_scale(f0, f1, s + 1, sb, a.gsteps2, t);
-      // the stage read before takes the next step once the group's four warps have read it
-      if (tile == 0 && lane == 0 && at > begin && lat < end &&
-          mbar_wait(&sm.empty[group][prev], pphase, abort_flag, 0x620 + group))
-        fetch();
-      __syncwarp();
-      ok = mbar_wait(&sm.full[group][st], phase, abort_flag, 0x610 + group);
-      if (!ok) break;
-      const uint32_t w = smem_u32(ring + st * S::BYTES) + r0 * (KG * BITS / 8);
-      const uint32_t ha = smem_u32(ring + st * S::BYTES + S::W) + lane * 16;
-      Codes<BITS> w0, w1;
-      w0.load_step(w, g, t);
-      w1.load_step(w + 8 * (KG * BITS / 8), g, t);
-      float f, v;
-      if (TS) {
-        const uint32_t fa = smem_u32(ring + st * S::BYTES + S::W + S::H) + r0 * 16 + (scale_index(s, a.gsteps2) & 3) * 4;
-        f = lds4(fa);
-        v = lds4(fa + 128);
-      } else {
-        quad_scales(sc, f, v);
-        sc = scn;
-      }
-      float d0[4] = {0.f, 0.f, 0.f, 0.f}, d1[4] = {0.f, 0.f, 0.f, 0.f};  // chains of MMAs
-      if (packed) {
+  if (warp == WARPS) {
+    // ---- copies: the groups' next slots in turn
+    int at[GROUPS], seg[GROUPS], z[GROUPS], st[GROUPS], issued[GROUPS];
+    uint32_t ph[GROUPS];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const uint4 hv = lds16(ha + j * 512);
-          uint32_t p0[4], p1[4];
-          w0.template pairs<false>(j, p0);
-          w1.template pairs<false>(j, p1);
-          mma_bf16(d0, p0[0], p1[0], p0[1], p1[1], hv.x, hv.y);
-          mma_bf16(d1, p0[2], p1[2], p0[3], p1[3], hv.z, hv.w);
+    for (int q = 0; q < GROUPS; ++q) {
+      at[q] = bound(q);
+      seg[q] = at[q] / slots;
+      z[q] = at[q] - seg[q] * slots;
+      st[q] = issued[q] = 0;
+      ph[q] = 1;
+    }
+    bool ok = true;
+    while (ok && (at[0] < bound(1) || at[GROUPS - 1] < bound(GROUPS))) {
+#pragma unroll
+      for (int q = 0; q < GROUPS; ++q) {
+        if (ok && at[q] < bound(q + 1)) {
+          ok = mbar_wait(&sm.empty[q][st[q]], ph[q], abort_flag, 0x620 + q);
+          if (!ok) break;
+          const Segment sg = sm.seg[seg[q]];
+          uint64_t* bar = &sm.full[q][st[q]];
+          uint8_t* dst = base + (q * depth + st[q]) * S::BYTES;
+          const int n = min(SS, steps - z[q] * SS);
+          const int hb = sg.n <= 4 ? 2048 : 4096;  // of a step
+          const int y = sg.expert * a.H + panel * PANEL;
+          if (lane == 0) mbar_expect_tx(bar, S::W + n * hb + (TS ? S::S : 0));
+          __syncwarp();
+          if (lane == 0) {
+            tma_load_2d(dst, &tm_w, z[q] * 128, y, bar);
+            if (TS) tma_load_2d(dst + S::W + S::H, &tm_s, scale_index(z[q] * SS, a.gsteps2) & ~3, y, bar);
+          } else if (lane <= n) {
+            bulk_load(dst + S::W + (lane - 1) * 4096, a.h + (static_cast<int64_t>(seg[q]) * steps + z[q] * SS + lane - 1) * 256,
+                      hb, bar);
+          }
+          ++at[q];
+          ++issued[q];
+          if (++z[q] == slots) {
+            z[q] = 0;
+            ++seg[q];
+          }
+          if (++st[q] == depth) {
+            st[q] = 0;
+            ph[q] ^= 1;
+          }
         }
-      } else {
-        float d2[4] = {0.f, 0.f, 0.f, 0.f}, d3[4] = {0.f, 0.f, 0.f, 0.f};
+      }
+    }
+    if (!ok && lane == 0) {  // never leave copies in flight into this CTA's shared memory
+      const long long t0 = clock64();
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const uint4 hv = lds16(ha + j * 512), lv = lds16(ha + 2048 + j * 512);
-          uint32_t p0[4], p1[4];
-          w0.template pairs<false>(j, p0);
-          w1.template pairs<false>(j, p1);
-          mma_bf16(d0, p0[0], p1[0], p0[1], p1[1], hv.x, hv.y);
-          mma_bf16(d1, p0[2], p1[2], p0[3], p1[3], hv.z, hv.w);
-          mma_bf16(d2, p0[0], p1[0], p0[1], p1[1], lv.x, lv.y);
-          mma_bf16(d3, p0[2], p1[2], p0[3], p1[3], lv.z, lv.w);
+      for (int q = 0; q < GROUPS; ++q)
+        for (int i = max(0, issued[q] - depth); i < issued[q]; ++i)
+          while (!mbar_try_wait(&sm.full[q][i % depth], (i / depth) & 1) && clock64() - t0 < kTimeoutCycles) {
+          }
+    }
+  } else {
+    const int begin = bound(group), end = bound(group + 1);
+    const int r = Codes<BITS>::row_of(g), r0 = tile * 16 + r;  // this lane's rows of the panel: r0 and r0 + 8
+    const int n0 = min(panel * PANEL + r0, a.H - 1), n1 = min(panel * PANEL + r0 + 8, a.H - 1);
+    bool ok = true;
+    int st = 0;
+    uint32_t phase = 0;
+    for (int at = begin; at < end && ok;) {
+      const int si = at / slots, za = at - si * slots, zb = min(slots, za + end - at);
+      const Segment sg = sm.seg[si];
+      const bool packed = sg.n <= 4;
+      const float* f0 = a.s2 + (static_cast<int64_t>(sg.expert) * a.H + n0) * a.groups2;
+      const float* f1 = a.s2 + (static_cast<int64_t>(sg.expert) * a.H + n1) * a.groups2;
+      float acc[4] = {0.f, 0.f, 0.f, 0.f};
+      float sc = TS ? 0.f : load_scale(f0, f1, za * SS, steps, a.gsteps2, t);
+      for (int z = za; z < zb; ++z, ++at) {
+        ok = mbar_wait(&sm.full[group][st], phase, abort_flag, 0x610 + group);
+        if (!ok) break;
+        const uint32_t stage = smem_u32(base + (group * depth + st) * S::BYTES);
+#pragma unroll
+        for (int h = 0; h < SS; ++h) {
+          const int s = z * SS + h;
+          if (s < steps) {
+            const uint32_t ha = stage + S::W + h * 4096 + lane * 16;
+            Codes<BITS> w0, w1;
+            w0.load128(stage + r0 * 128, r, h, t);
+            w1.load128(stage + (r0 + 8) * 128, r, h, t);
+            float f, v;
+            if (TS) {
+              const uint32_t fa = stage + S::W + S::H + r0 * 16 + (scale_index(s, a.gsteps2) & 3) * 4;
+              f = lds4(fa);
+              v = lds4(fa + 128);
+            } else {
+              quad_scales(sc, f, v);
+              sc = load_scale(f0, f1, s + 1, steps, a.gsteps2, t);
+            }
+            float d0[4] = {0.f, 0.f, 0.f, 0.f}, d1[4] = {0.f, 0.f, 0.f, 0.f};  // chains of MMAs
+            if (packed) {
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                const uint4 hv = lds16(ha + j * 512);
+                uint32_t p0[4], p1[4];
+                w0.template pairs<false>(j, p0);
+                w1.template pairs<false>(j, p1);
+                mma_bf16(d0, p0[0], p1[0], p0[1], p1[1], hv.x, hv.y);
+                mma_bf16(d1, p0[2], p1[2], p0[3], p1[3], hv.z, hv.w);
+              }
+            } else {
+              float d2[4] = {0.f, 0.f, 0.f, 0.f}, d3[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                const uint4 hv = lds16(ha + j * 512), lv = lds16(ha + 2048 + j * 512);
+                uint32_t p0[4], p1[4];
+                w0.template pairs<false>(j, p0);
+                w1.template pairs<false>(j, p1);
+                mma_bf16(d0, p0[0], p1[0], p0[1], p1[1], hv.x, hv.y);
+                mma_bf16(d1, p0[2], p1[2], p0[3], p1[3], hv.z, hv.w);
+                mma_bf16(d2, p0[0], p1[0], p0[1], p1[1], lv.x, lv.y);
+                mma_bf16(d3, p0[2], p1[2], p0[3], p1[3], lv.z, lv.w);
+              }
+#pragma unroll
+              for (int i = 0; i < 4; ++i) d0[i] = __fadd_rn(d0[i], __fadd_rn(d2[i], d3[i]));
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[i] = __fmaf_rn(i < 2 ? f : v, __fadd_rn(d0[i], d1[i]), acc[i]);
+          }
         }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) d0[i] = __fadd_rn(d0[i], __fadd_rn(d2[i], d3[i]));
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // our reads of the stage before its refill
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sm.empty[group][st]);
+        if (++st == depth) {
+          st = 0;
+          phase ^= 1;
+        }
       }
+      if (packed) {  // columns 4 to 7 are the lo parts of 0 to 3
 #pragma unroll
-      for (int i = 0; i < 4; ++i) acc[i] = __fmaf_rn(i < 2 ? f : v, __fadd_rn(d0[i], d1[i]), acc[i]);
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // our reads of the stage before its refill
+        for (int i = 0; i < 4; ++i) acc[i] = __fadd_rn(acc[i], __shfl_xor_sync(0xffffffffu, acc[i], 2));
+      }
+      // rows belong to this warp alone, and the tokens of a segment are distinct
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int col = 2 * t + i;
+        if (col < sg.n) {
+          float* p = parts + (group * PANEL + r0) * pitch + sg.token(col);
+          p[0] += acc[i];
+          p[8 * pitch] += acc[2 + i];
+        }
+      }
       __syncwarp();
-      if (lane == 0) mbar_arrive(&sm.empty[group][st]);
-      prev = st;
-      pphase = phase;
-      if (++st == depth) {
-        st = 0;
-        phase ^= 1;
-      }
-    }
-    if (packed) {  // columns 4 to 7 are the lo parts of 0 to 3
-#pragma unroll
-      for (int i = 0; i < 4; ++i) acc[i] = __fadd_rn(acc[i], __shfl_xor_sync(0xffffffffu, acc[i], 2));
-    }
-    // rows belong to this warp alone, and the tokens of a segment are distinct
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int col = 2 * t + i;
-      if (col < ntok) {
-        float* p = parts + (group * PANEL + r0) * pitch + nth_bit(mask, col);
-        p[0] += acc[i];
-        p[8 * pitch] += acc[2 + i];
-      }
-    }
-    __syncwarp();
-  }
-  if (!ok && tile == 0 && lane == 0) {  // never leave copies in flight into this CTA's shared memory
-    const long long t0 = clock64();
-    for (int i = 0; i < depth; ++i) {
-      const int q = (st + i) % depth;
-      while (!mbar_try_wait(&sm.full[group][q], q < st ? phase ^ 1 : phase) && clock64() - t0 < kTimeoutCycles) {
-      }
     }
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < PANEL * pitch; i += THREADS) {  // the groups' parts in the order of their steps
-    float v = parts[i];
+  // the groups' parts in the order of their steps; with one CTA a panel that is all
+  float* mine = a.partial + (static_cast<int64_t>(panel) * a.split + rank) * (PANEL * a.T);
+  auto store = [&](int i, float v) {  // i = token * PANEL + row
+    const int n = panel * PANEL + i % PANEL;
+    if (n < a.H) a.out[static_cast<int64_t>(i / PANEL) * a.H + n] = __float2bfloat16_rn(v);
+  };
+  for (int i = threadIdx.x; i < PANEL * a.T; i += THREADS2) {
+    const float* p = parts + i % PANEL * pitch + i / PANEL;
+    float v = p[0];
 #pragma unroll
-    for (int q = 1; q < GROUPS; ++q) v = __fadd_rn(v, parts[q * PANEL * pitch + i]);
-    parts[i] = v;
+    for (int q = 1; q < GROUPS; ++q) v = __fadd_rn(v, p[q * PANEL * pitch]);
+    if (a.split == 1) store(i, v);
+    else __stcg(mine + i, v);
   }
-  cluster.sync();
-  // then the CTAs', a share of the panel's rows in each
-  constexpr int ROWS = PANEL / CL2;
-  for (int i = threadIdx.x; i < ROWS * a.T; i += THREADS) {
-    const int row = rank * ROWS + i % ROWS, tok = i / ROWS;
-    float v[CL2];
+  if (a.split == 1) return;
+  __threadfence();
+  __syncthreads();
+  if (threadIdx.x == 0) sm.last = atomicAdd(&a.plan->done[panel], 1) == a.split - 1;
+  __syncthreads();
+  if (!sm.last) return;
+  __threadfence();
+  // the CTA that finishes last adds the CTAs' parts, again in the order of their steps
+  const float* all = a.partial + static_cast<int64_t>(panel) * a.split * (PANEL * a.T);
+  for (int i = threadIdx.x; i < PANEL * a.T; i += THREADS2) {
+    float v[MAX_SPLIT];
 #pragma unroll
-    for (int c = 0; c < CL2; ++c) v[c] = cluster.map_shared_rank(parts, c)[row * pitch + tok];
+    for (int c = 0; c < MAX_SPLIT; ++c) v[c] = c < a.split ? __ldcg(all + static_cast<int64_t>(c) * (PANEL * a.T) + i) : 0.f;
 #pragma unroll
-    for (int c = 1; c < CL2; ++c) v[0] = __fadd_rn(v[0], v[c]);
-    if (panel * PANEL + row < a.H)
-      a.out[static_cast<int64_t>(tok) * a.H + panel * PANEL + row] = __float2bfloat16_rn(v[0]);
+    for (int c = 1; c < MAX_SPLIT; ++c) v[0] = __fadd_rn(v[0], v[c]);
+    store(i, v[0]);
   }
-  cluster.sync();  // the others may still read this CTA's part
 }
 
 template <typename K>
-int launch_cluster(K kernel, int grid, int cluster, int smem, cudaStream_t st, const CUtensorMap& tw, const CUtensorMap& ts,
-                   const FewArgs& a, const char* what) {
+int launch_few_kernel(K kernel, int grid, int cluster, int threads, int smem, cudaStream_t st, const CUtensorMap& tw,
+                      const CUtensorMap& ts, const FewArgs& a, const char* what) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(grid);
-  cfg.blockDim = dim3(THREADS);
+  cfg.blockDim = dim3(threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cudaLaunchAttribute attr[2];
@@ -978,7 +1029,7 @@ int launch_cluster(K kernel, int grid, int cluster, int smem, cudaStream_t st, c
   attr[1].val.clusterDim.x = cluster;
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 2;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, tw, ts, a);
   if (e != cudaSuccess) {
     cudaGetLastError();
@@ -988,6 +1039,11 @@ int launch_cluster(K kernel, int grid, int cluster, int smem, cudaStream_t st, c
 }
 
 constexpr int kSmemMost = 232448;  // 227 KB
+
+inline int panels_of(int H) { return (H + PANEL - 1) / PANEL; }
+
+// CTAs of a panel: as many as fill the SMs once
+inline int split_of(int H) { return std::max(1, std::min(MAX_SPLIT, num_sms() / panels_of(H))); }
 
 template <typename K>
 int allow_smem(K kernel, std::atomic<uint64_t>& ready) {
@@ -1024,15 +1080,14 @@ int launch_gemm1(FewArgs& a, const int8_t* q1, cudaStream_t st) {
     if (smem <= kSmemMost) break;
   }
   if (smem > kSmemMost) return fail(LLQ_EUNSUPPORTED, "the few-token layer has no room for rows of %d", a.H);
-  return launch_cluster(few_gemm1_kernel<BITS, TS>, num_sms() / CL1 * CL1, CL1, smem, st, tw, ts, a, "few_gemm1_kernel");
+  return launch_few_kernel(few_gemm1_kernel<BITS, TS>, num_sms() / CL1 * CL1, CL1, THREADS, smem, st, tw, ts, a, "few_gemm1_kernel");
 }
 
 template <int BITS, bool TS>
 int launch_gemm2(FewArgs& a, cudaStream_t st) {
   const uint64_t kb = static_cast<uint64_t>(a.I) * BITS / 8, rows = static_cast<uint64_t>(a.E) * a.H;
   CUtensorMap tw, ts;
-  int rc = make_map(&tw, a.q2, CU_TENSOR_MAP_DATA_TYPE_UINT8, kb, rows, kb, KG * BITS / 8, PANEL,
-                    BITS == 4 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B);
+  int rc = make_map(&tw, a.q2, CU_TENSOR_MAP_DATA_TYPE_UINT8, kb, rows, kb, 128, PANEL, CU_TENSOR_MAP_SWIZZLE_128B);
   if (rc) return rc;
   ts = tw;
   if (TS) {
@@ -1046,8 +1101,8 @@ int launch_gemm2(FewArgs& a, cudaStream_t st) {
   // as deep as the partial outputs leave room for
   const int fixed = 1024 + static_cast<int>(sizeof(Smem2)) + GROUPS * PANEL * (a.T | 1) * 4;
   a.depth2 = std::min(MAX_DEPTH2, (kSmemMost - fixed) / (GROUPS * Stage2<BITS>::BYTES));
-  return launch_cluster(few_gemm2_kernel<BITS, TS>, (a.H + PANEL - 1) / PANEL * CL2, CL2,
-                        fixed + GROUPS * a.depth2 * Stage2<BITS>::BYTES, st, tw, ts, a, "few_gemm2_kernel");
+  return launch_few_kernel(few_gemm2_kernel<BITS, TS>, panels_of(a.H) * a.split, 1, THREADS2,
+                           fixed + GROUPS * a.depth2 * Stage2<BITS>::BYTES, st, tw, ts, a, "few_gemm2_kernel");
 }
 
 template <int BITS>
@@ -1065,11 +1120,24 @@ inline bool few_group_ok(int K, int group) { return group <= 0 || K % group != 0
 // most segments of a call: every chosen expert has one with fewer than 8 tokens at most, the others are full
 inline int64_t few_segments(int64_t T, int k, int E) { return std::min<int64_t>(T * k, E + T * k / 8); }
 
+struct FewWorkspace {
+  size_t h, partial, total;
+};
+
+// (sized for the most CTAs a panel can have, so that it does not hang on the device)
+FewWorkspace few_workspace(int64_t T, int k, int E, int H, int I) {
+  FewWorkspace w;
+  w.h = up256(sizeof(FewPlan));
+  w.partial = w.h + static_cast<size_t>(few_segments(T, k, E)) * ((I + KG - 1) / KG) * 4096;
+  w.total = w.partial + static_cast<size_t>(panels_of(H)) * MAX_SPLIT * PANEL * T * 4;
+  return w;
+}
+
 }  // namespace
 
-size_t moe_few_workspace(int64_t T, int k, int E, int I) {
-  if (T < 1 || k < 1 || E < 1 || I < 1 || T > MAX_T || k > MAX_K || E > MAX_EXP) return 0;
-  return up256(sizeof(FewPlan)) + static_cast<size_t>(few_segments(T, k, E)) * ((I + KG - 1) / KG) * 4096;
+size_t moe_few_workspace(int64_t T, int k, int E, int H, int I) {
+  if (T < 1 || k < 1 || E < 1 || H < 1 || I < 1 || T > MAX_T || k > MAX_K || E > MAX_EXP) return 0;
+  return few_workspace(T, k, E, H, I).total;
 }
 
 int moe_few(const llq_few_layer& L, const void* x, int64_t T, float* logits, float* topk_w, int32_t* topk_ids,
@@ -1091,7 +1159,7 @@ int moe_few(const llq_few_layer& L, const void* x, int64_t T, float* logits, flo
                        reinterpret_cast<uintptr_t>(L.qw1) | reinterpret_cast<uintptr_t>(L.qw2) |
                        reinterpret_cast<uintptr_t>(workspace);
   if (al & 15) return fail(LLQ_EINVAL, "x, gate_w, the packed weights and the workspace need 16-byte alignment");
-  const size_t need = moe_few_workspace(T, L.k, L.E, L.I);
+  const size_t need = moe_few_workspace(T, L.k, L.E, L.H, L.I);
   if (workspace == nullptr || bytes < need)
     return fail(LLQ_ENOSPACE, "workspace needs %zu bytes, got %zu", need, bytes);
   FewArgs a{};
@@ -1117,7 +1185,10 @@ int moe_few(const llq_few_layer& L, const void* x, int64_t T, float* logits, flo
   a.topk_ids = topk_ids;
   char* ws = static_cast<char*>(workspace);
   a.plan = reinterpret_cast<FewPlan*>(ws);
-  a.h = reinterpret_cast<uint4*>(ws + up256(sizeof(FewPlan)));
+  const FewWorkspace w = few_workspace(T, L.k, L.E, L.H, L.I);
+  a.h = reinterpret_cast<uint4*>(ws + w.h);
+  a.partial = reinterpret_cast<float*>(ws + w.partial);
+  a.split = split_of(L.H);
   a.out = static_cast<__nv_bfloat16*>(out);
   return L.bits == 4 ? launch_few<4>(a, L.qw1, st) : launch_few<8>(a, L.qw1, st);
 }

@@ -594,7 +594,7 @@ def few_call(layer: _lib.FewLayer, x: torch.Tensor, topk_w: torch.Tensor, topk_i
     T = x.shape[0]
     out = torch.empty_like(x)
     # scratch of this call alone: the caching allocator orders its reuse by stream and by graph
-    nbytes = lib.llq_moe_few_workspace_size(T, layer.k, layer.E, layer.I)
+    nbytes = lib.llq_moe_few_workspace_size(T, layer.k, layer.E, layer.H, layer.I)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
     rc = lib.llq_moe_few(_lib.byref(layer), x.data_ptr(), T, _ptr(logits), topk_w.data_ptr(), topk_ids.data_ptr(),
                          out.data_ptr(), ws.data_ptr(), nbytes, _raw_stream(x))

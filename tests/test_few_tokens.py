@@ -341,8 +341,8 @@ def test_c_edges_need_no_gpu():
     lib = _lib.load()
     assert lib.llq_moe_few(None, 16, 1, None, 16, 16, 16, 16, 1, None) == _lib.LLQ_EINVAL
     assert lib.llq_moe_few(ctypes.byref(_c_layer()), None, 0, None, None, None, None, None, 0, None) == _lib.LLQ_OK
-    assert lib.llq_moe_few_workspace_size(0, 8, 64, 1024) == 0
-    assert lib.llq_moe_few_workspace_size(32, 8, 64, 1024) >= 32 * 8 * 1024 * 4
+    assert lib.llq_moe_few_workspace_size(0, 8, 64, 2048, 1024) == 0
+    assert lib.llq_moe_few_workspace_size(32, 8, 64, 2048, 1024) >= 32 * 8 * 1024 * 4
 
 
 def test_python_refusals_need_no_gpu(monkeypatch):
