@@ -16,8 +16,8 @@
 //
 // Kernel 1 (router, GEMM1): each cluster of 2 CTAs computes the whole router (half of K per CTA,
 // exchanged through distributed shared memory), so no grid-wide wait stands between router and
-// experts.  The work is a list of segments (expert, up to 8 of its tokens), each of I / 8 jobs: 8
-// gate and the 8 up rows, so that SiLU(a) * b is local to a thread.  The CTAs take equal runs of jobs.
+// experts.  The work is a list of segments (expert, up to 8 of its tokens), each of I / 16 jobs: 16
+// gate and the 16 up rows, so that SiLU(a) * b is local to a thread.  The CTAs take equal runs of jobs.
 // Kernel 2 (GEMM2, combine): the CTAs of a panel of 128 output features split the list of (segment,
 // 128-group) steps evenly; each stores its partial outputs, and the one that finishes last adds them
 // in the order of the steps: no waits, and a fixed order of sums.
@@ -33,8 +33,8 @@
 // enough for HBM's latency; the tokens lie in shared memory in MMA order.  Measured on the way
 // (32 tokens, INT4, both kernels): lanes loading their own bytes with cp.async and their tokens from L1,
 // 132 us, bound by the L1 wavefronts that eight scattered rows per instruction cost; a register ring
-// unrolled over its slots, 527 us, its code larger than the instruction cache; TMA rings whose refill one
-// lane computed while its warp waited, 94 us.
+// unrolled over its slots, 527 us, its code larger than the instruction cache; TMA rings whose refill the
+// computing warps issued themselves, 87 us (a copy holds its warp up for hundreds of cycles).
 #include <algorithm>
 
 #include <cooperative_groups.h>
@@ -54,8 +54,8 @@ constexpr int MAX_K = 32;
 constexpr int MAX_SEG = MAX_EXP + MAX_T * MAX_K / 8;
 constexpr int CL1 = 2;        // CTAs of a cluster of kernel 1: all 148 SMs hold one (of 8, with this much
                               // shared memory, only 120 CTAs fit at once)
-constexpr int WARPS = 16;
-constexpr int THREADS = WARPS * 32;
+constexpr int WARPS = 12;     // of kernel 1 that compute, and one that issues the copies
+constexpr int THREADS = (WARPS + 1) * 32;
 constexpr int KG = 128;       // K elements of a step: 32 for each of a quad's four lanes
 
 constexpr int MAX_SPLIT = 16;  // CTAs of a panel in kernel 2
@@ -189,16 +189,16 @@ template <int BITS>
 struct Codes {
   static constexpr int STEPS = BITS == 4 ? 2 : 1;  // steps in 128 bytes
   uint4 v[BITS == 4 ? 1 : 2];
-  // `row` is the address of row r (mod 8), `step` the step in it.  With row_of(g) as lane g's row
-  // the eight lanes that a shared-memory access serves at a time (two rows) meet eight different 16-byte columns.
+  // With row_of(g) as lane g's row the eight lanes that a shared-memory access serves at a time (two rows) meet eight
+  // different 16-byte columns; offset(g, t) is where lane (g, t)'s first 16 bytes lie in its row.
   static __device__ __forceinline__ int row_of(int g) { return BITS == 4 ? ((g & 1) << 2) | (g >> 1) : g; }
-  __device__ __forceinline__ void load128(uint32_t row, int r, int step, int t) {
-    if (BITS == 4) {
-      v[0] = lds16(row + (((step * 4 + t) ^ r) << 4));
-    } else {
-      v[0] = lds16(row + (((2 * t) ^ r) << 4));
-      v[1] = lds16(row + (((2 * t + 1) ^ r) << 4));
-    }
+  static __device__ __forceinline__ uint32_t offset(int g, int t) {
+    return static_cast<uint32_t>(((BITS == 4 ? t : 2 * t) ^ row_of(g)) << 4);
+  }
+  // `at`: the lane's first 16 bytes in its row, at INT4 of the step (the second step's lie 64 bytes, xor, further)
+  __device__ __forceinline__ void load(uint32_t at) {
+    v[0] = lds16(at);
+    if (BITS == 8) v[1] = lds16(at ^ 16);
   }
   // codes 8j .. 8j + 7
   template <bool F16>
@@ -232,20 +232,54 @@ __device__ __forceinline__ int pair_place(int n) {
   return BITS == 4 ? (j < 4 ? 2 * j : 2 * j - 7) : (j & 4) + 2 * (j & 1) + ((j >> 1) & 1);
 }
 
-// The scale of step s of a row: where a row has a multiple of 4 of them, a copy brings the aligned four that hold it
-// (a slot never straddles them: they cover a multiple of 4 steps), else lanes load it (those of a quad share a row
-// pair: even lanes its first row, odd lanes its second).
-__device__ __forceinline__ int scale_index(int s, int gsteps) { return gsteps == 0 ? 0 : gsteps == 1 ? s : s / gsteps; }
-
-__device__ __forceinline__ float load_scale(const float* a, const float* b, int s, int steps, int gsteps, int t) {
-  return s < steps ? __ldg(((t & 1) ? b : a) + scale_index(s, gsteps)) : 0.f;
-}
-
-__device__ __forceinline__ void quad_scales(float v, float& a, float& b) {
-  const int src = threadIdx.x & 28;
-  a = __shfl_sync(0xffffffffu, v, src);
-  b = __shfl_sync(0xffffffffu, v, src + 1);
-}
+// The scales of a warp's 32 rows.  Lane t of a quad loads those of one of the quad's four rows (t = 2 q + i: the row
+// that is i of MMA q), and shuffles hand them to the quad.  V4: a row has a multiple of four scales, one per step: the
+// lane holds those of four steps and asks for the next four in time for HBM.  Else one is loaded per step, or one for
+// the whole row.
+template <int STEPS, bool V4>
+struct RowScales {
+  const float* p;
+  int gsteps, steps;
+  float4 cur, nxt;
+  __device__ __forceinline__ float4 four(int s) const {
+    return s < steps ? __ldg(reinterpret_cast<const float4*>(p + s)) : make_float4(0.f, 0.f, 0.f, 0.f);
+  }
+  __device__ __forceinline__ float one(int s) const { return s < steps ? __ldg(p + (gsteps == 1 ? s : s / gsteps)) : 0.f; }
+  // for steps from s on
+  __device__ __forceinline__ void start(const float* row, int s, int nsteps, int gs) {
+    p = row;
+    steps = nsteps;
+    gsteps = gs;
+    if (V4) {
+      cur = four(s & ~3);
+      nxt = four((s & ~3) + 4);
+    } else {
+      cur.x = gs == 0 ? __ldg(p) : one(s);
+    }
+  }
+  // of step s, for all four rows
+  __device__ __forceinline__ void get(int s, float (&f)[2][2]) {
+    float v;
+    if (V4) {
+      v = (s & 2) ? ((s & 1) ? cur.w : cur.z) : ((s & 1) ? cur.y : cur.x);
+    } else {
+      v = cur.x;
+      if (gsteps != 0) cur.x = one(s + 1);
+    }
+    const int src = threadIdx.x & 28;
+#pragma unroll
+    for (int q = 0; q < 2; ++q)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) f[q][i] = __shfl_sync(0xffffffffu, v, src + 2 * q + i);
+  }
+  // behind the slot whose first step was `first`
+  __device__ __forceinline__ void next(int first) {
+    if (V4 && ((first + STEPS) & 3) == 0) {
+      cur = nxt;
+      nxt = four(first + STEPS + 4);
+    }
+  }
+};
 
 // key > 0 that orders floats as their values; NaN lowest
 __device__ __forceinline__ uint32_t order_key(float z) {
@@ -255,10 +289,8 @@ __device__ __forceinline__ uint32_t order_key(float z) {
 }
 
 constexpr int MAX_DEPTH1 = 2;
-constexpr int TILE1 = 2048;      // 8 gate and 8 up rows of 128 bytes: one copy
-constexpr int SLOT1 = 2 * TILE1;
-constexpr int SCALE1 = 256;      // the same 16 rows' four scales
-constexpr int RED_SLICES = 8;
+constexpr int SLOT1 = 4096;      // 16 gate and 16 up rows of 128 bytes (two steps at INT4, one at INT8): one copy
+constexpr int RED_SLICES = WARPS / 2;
 constexpr int RED_PITCH = MAX_T + 1;
 constexpr int RED_BYTES = RED_SLICES * 64 * RED_PITCH * 4;
 constexpr int ROUTER_BYTES = RED_BYTES + CL1 * MAX_EXP * MAX_T * 4;  // over the rings and tokens, before they are used
@@ -270,67 +302,72 @@ struct Smem1 {
   Segment seg[MAX_SEG];
   float col_w[2][8];             // the columns' weights of the segments at hand
   float col_scale[2][64][8];     // what undoes the scaling of a step of a column's token
-  float4 head[WARPS][32];        // a warp's part of a job that an earlier warp began
-  uint64_t full[WARPS][MAX_DEPTH1];  // a slot of a warp's ring has landed
+  float4 head[WARPS][2][32];     // a warp's part of a job that an earlier warp began
+  uint64_t full[WARPS][MAX_DEPTH1];   // a slot of a warp's ring has landed
+  uint64_t empty[WARPS][MAX_DEPTH1];  // and was read
   int32_t nseg;
   int abort_flag;
 };
 
 using LogitPart = float[MAX_T][MAX_EXP];
 
-// The router: K is split over the CTAs of the cluster and eight slices of warps in each; half of the warps take 32 of
+// The router: K is split over the CTAs of the cluster and six slices of warps in each; half of the warps take 32 of
 // 64 experts at a time, the others the next 32.  A slice's sums meet in `red`, a CTA's in parts[rank] of both CTAs.
+template <int NT>  // tiles of 8 tokens
 __device__ void router_logits(const FewArgs& a, float (*red)[64][RED_PITCH], LogitPart* parts, cg::cluster_group& cluster) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int ntiles = (a.T + 7) / 8;
   const int rank = static_cast<int>(cluster.block_rank());
   const int slice = warp % RED_SLICES, half = warp / RED_SLICES;
   const int pairs = (a.H + 63) / 64;  // 128 bytes of a row: two chunks of 32
   const int p0 = pairs * rank / CL1, p1 = pairs * (rank + 1) / CL1;
+#pragma unroll 1
   for (int eg = 0; eg < a.E; eg += 64) {
-    float d[2][MAX_T / 8][4] = {};
-    const __nv_bfloat16* w[4];
+    if (warp < WARPS) {
+      float d[2][NT][4] = {};
+      const __nv_bfloat16* w[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)  // experts beyond the last read it and are not kept
-      w[i] = a.gate + static_cast<int64_t>(min(eg + half * 32 + i * 8 + g, a.E - 1)) * a.H + 8 * t;
-    for (int p = p0 + slice; p < p1; p += RED_SLICES) {
-      uint4 u[2][4], x[2][MAX_T / 8];
+      for (int i = 0; i < 4; ++i)  // experts beyond the last read it and are not kept
+        w[i] = a.gate + static_cast<int64_t>(min(eg + half * 32 + i * 8 + g, a.E - 1)) * a.H + 8 * t;
+#pragma unroll 1
+      for (int p = p0 + slice; p < p1; p += RED_SLICES) {
+        uint4 u[2][4], x[2][NT];
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        const int at = p * 64 + c * 32;
-        const bool in = at < a.H;
+        for (int c = 0; c < 2; ++c) {
+          const int at = p * 64 + c * 32;
+          const bool in = at < a.H;
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          u[c][i] = in ? __ldg(reinterpret_cast<const uint4*>(w[i] + at)) : make_uint4(0, 0, 0, 0);
+          for (int i = 0; i < 4; ++i)
+            u[c][i] = in ? __ldg(reinterpret_cast<const uint4*>(w[i] + at)) : make_uint4(0, 0, 0, 0);
 #pragma unroll
-        for (int n = 0; n < MAX_T / 8; ++n)
-          x[c][n] = in && n < ntiles ? __ldg(reinterpret_cast<const uint4*>(
-                                           a.x + static_cast<int64_t>(min(n * 8 + g, a.T - 1)) * a.H + 8 * t + at))
-                                     : make_uint4(0, 0, 0, 0);
+          for (int n = 0; n < NT; ++n)
+            x[c][n] = in ? __ldg(reinterpret_cast<const uint4*>(
+                                             a.x + static_cast<int64_t>(min(n * 8 + g, a.T - 1)) * a.H + 8 * t + at))
+                                       : make_uint4(0, 0, 0, 0);
+        }
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+            {
+#pragma unroll
+              for (int m = 0; m < 2; ++m) {
+                mma_bf16(d[m][n], u[c][2 * m].x, u[c][2 * m + 1].x, u[c][2 * m].y, u[c][2 * m + 1].y, x[c][n].x, x[c][n].y);
+                mma_bf16(d[m][n], u[c][2 * m].z, u[c][2 * m + 1].z, u[c][2 * m].w, u[c][2 * m + 1].w, x[c][n].z, x[c][n].w);
+              }
+            }
       }
 #pragma unroll
-      for (int c = 0; c < 2; ++c)
+      for (int m = 0; m < 2; ++m)
 #pragma unroll
-        for (int n = 0; n < MAX_T / 8; ++n)
-          if (n < ntiles) {
-#pragma unroll
-            for (int m = 0; m < 2; ++m) {
-              mma_bf16(d[m][n], u[c][2 * m].x, u[c][2 * m + 1].x, u[c][2 * m].y, u[c][2 * m + 1].y, x[c][n].x, x[c][n].y);
-              mma_bf16(d[m][n], u[c][2 * m].z, u[c][2 * m + 1].z, u[c][2 * m].w, u[c][2 * m + 1].w, x[c][n].z, x[c][n].w);
-            }
+        for (int n = 0; n < NT; ++n)
+          {
+            float* r = &red[slice][half * 32 + m * 16 + g][n * 8 + 2 * t];
+            r[0] = d[m][n][0];
+            r[1] = d[m][n][1];
+            r[8 * RED_PITCH] = d[m][n][2];
+            r[8 * RED_PITCH + 1] = d[m][n][3];
           }
     }
-#pragma unroll
-    for (int m = 0; m < 2; ++m)
-#pragma unroll
-      for (int n = 0; n < MAX_T / 8; ++n)
-        if (n < ntiles) {
-          float* r = &red[slice][half * 32 + m * 16 + g][n * 8 + 2 * t];
-          r[0] = d[m][n][0];
-          r[1] = d[m][n][1];
-          r[8 * RED_PITCH] = d[m][n][2];
-          r[8 * RED_PITCH + 1] = d[m][n][3];
-        }
     __syncthreads();
     for (int i = threadIdx.x; i < 64 * a.T; i += THREADS) {
       const int r = i & 63, tok = i >> 6;
@@ -352,80 +389,71 @@ __device__ __forceinline__ float logit_of(const FewArgs& a, const LogitPart* par
   return z;
 }
 
-// softmax and top-k of N tokens (WARPS apart) by one warp, 32 PER experts at most, into sm.ids, sm.w and sm.mask; the
-// tokens' chains of dependent steps overlap
-template <int PER, int N>
-__device__ void choose(const FewArgs& a, Smem1& sm, const LogitPart* parts, int tok0) {
+// softmax and top-k of one token by one warp, 32 PER experts at most, into sm.ids, sm.w and sm.mask.  (Here and in all
+// that a call runs once the code is kept short: it comes from L2 or HBM, 128 bytes at a time, and unrolling this for
+// three tokens made it 3 times slower.)
+template <int PER>
+__device__ void choose(const FewArgs& a, Smem1& sm, const LogitPart* parts, int tok) {
   const int lane = threadIdx.x & 31;
-  float p[N][PER], s[N], wt[N];
-  uint32_t key[N][PER];  // 0: no expert, or one that is taken
-  int id[N];             // lane i: choice i
+  float p[PER];
+  uint32_t key[PER];  // 0: no expert, or one that is taken
+  float m = -INFINITY;
+  bool bad = false;
 #pragma unroll
-  for (int n = 0; n < N; ++n) {
-    const int tok = min(tok0 + n * WARPS, a.T - 1);
-    float m = -INFINITY;
-    bool bad = false;
-#pragma unroll
-    for (int j = 0; j < PER; ++j) {
-      const int e = lane + 32 * j;
-      p[n][j] = e < a.E ? __fadd_rn(logit_of(a, parts, e, tok), 0.f) : -INFINITY;  // -0 ranks as +0
-      key[n][j] = e < a.E ? order_key(p[n][j]) : 0;
-      bad |= !(p[n][j] == p[n][j]);
-      m = fmaxf(m, p[n][j]);
-    }
-    m = warp_max(m);
-    s[n] = 0.f;
-#pragma unroll
-    for (int j = 0; j < PER; ++j) {
-      p[n][j] = lane + 32 * j < a.E ? expf(p[n][j] - m) : 0.f;
-      s[n] = __fadd_rn(s[n], p[n][j]);
-    }
-    s[n] = warp_sum(s[n]);
-    if (__any_sync(0xffffffffu, bad)) s[n] = NAN;  // as softmax over a row with a NaN
-    wt[n] = 0.f;
-    id[n] = 0;
+  for (int j = 0; j < PER; ++j) {
+    const int e = lane + 32 * j;
+    p[j] = e < a.E ? __fadd_rn(logit_of(a, parts, e, tok), 0.f) : -INFINITY;  // -0 ranks as +0
+    key[j] = e < a.E ? order_key(p[j]) : 0;
+    bad |= !(p[j] == p[j]);
+    m = fmaxf(m, p[j]);
   }
+  m = warp_max(m);
+  float s = 0.f;
+#pragma unroll
+  for (int j = 0; j < PER; ++j) {
+    p[j] = lane + 32 * j < a.E ? expf(p[j] - m) : 0.f;
+    s = __fadd_rn(s, p[j]);
+  }
+  s = warp_sum(s);
+  if (__any_sync(0xffffffffu, bad)) s = NAN;  // as softmax over a row with a NaN
+  float wt = 0.f;
+  int id = 0;  // lane i: choice i
+#pragma unroll 1
   for (int i = 0; i < a.k; ++i) {
+    uint32_t best = key[0];
+    float q = p[0];
+    int bj = 0;
 #pragma unroll
-    for (int n = 0; n < N; ++n) {
-      uint32_t best = key[n][0];
-      float q = p[n][0];
-      int bj = 0;
-#pragma unroll
-      for (int j = 1; j < PER; ++j) {
-        if (key[n][j] > best) {
-          best = key[n][j];
-          q = p[n][j];
-          bj = j;
-        }
+    for (int j = 1; j < PER; ++j) {
+      if (key[j] > best) {
+        best = key[j];
+        q = p[j];
+        bj = j;
       }
-      const uint32_t top = __reduce_max_sync(0xffffffffu, best);
-      const uint32_t mine = best == top ? static_cast<uint32_t>(lane + 32 * bj) : 0xffffffffu;
-      const uint32_t e = __reduce_min_sync(0xffffffffu, mine);
+    }
+    const uint32_t top = __reduce_max_sync(0xffffffffu, best);
+    const uint32_t mine = best == top ? static_cast<uint32_t>(lane + 32 * bj) : 0xffffffffu;
+    const uint32_t e = __reduce_min_sync(0xffffffffu, mine);
 #pragma unroll
-      for (int j = 0; j < PER; ++j)
-        if (mine == e && j == bj) key[n][j] = 0;
-      q = __shfl_sync(0xffffffffu, q, e & 31);
-      if (lane == i) {
-        id[n] = static_cast<int>(e);
-        wt[n] = q;
-      }
+    for (int j = 0; j < PER; ++j)
+      if (mine == e && j == bj) key[j] = 0;
+    q = __shfl_sync(0xffffffffu, q, e & 31);
+    if (lane == i) {
+      id = static_cast<int>(e);
+      wt = q;
     }
   }
-#pragma unroll
-  for (int n = 0; n < N; ++n) {
-    const int tok = tok0 + n * WARPS;
-    if (lane < a.k) wt[n] = __fdiv_rn(wt[n], s[n]);
-    if (a.renormalize) {
-      float total = 0.f;
-      for (int i = 0; i < a.k; ++i) total = __fadd_rn(total, __shfl_sync(0xffffffffu, wt[n], i));
-      wt[n] = __fdiv_rn(wt[n], total);
-    }
-    if (lane < a.k && tok < a.T) {
-      sm.ids[tok][lane] = static_cast<int16_t>(id[n]);
-      sm.w[tok][lane] = wt[n];
-      atomicOr(&sm.mask[id[n]], 1u << tok);
-    }
+  if (lane < a.k) wt = __fdiv_rn(wt, s);
+  if (a.renormalize) {
+    float total = 0.f;
+#pragma unroll 1
+    for (int i = 0; i < a.k; ++i) total = __fadd_rn(total, __shfl_sync(0xffffffffu, wt, i));
+    wt = __fdiv_rn(wt, total);
+  }
+  if (lane < a.k) {
+    sm.ids[tok][lane] = static_cast<int16_t>(id);
+    sm.w[tok][lane] = wt;
+    atomicOr(&sm.mask[id], 1u << tok);
   }
 }
 
@@ -441,28 +469,62 @@ __device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
 }
 
-// TS: scales by copies
-template <int BITS, bool TS>
+// h of a finished job: features 16 rb and on of segment seg (a function of its own: it is called from two places)
+template <int BITS>
+__device__ __noinline__ void emit(const FewArgs& a, const Segment& sg, const float* col_w, int seg, int rb,
+                                  const float (&acc)[2][4]) {
+  const int lane = threadIdx.x & 31, t = lane & 3, r = Codes<BITS>::row_of(lane >> 2);
+  const int hsteps = (a.I + KG - 1) / KG, ntok = sg.n;
+  const int lo = (ntok <= 4 ? 16 : 128);  // pieces from the hi to the lo parts: four columns, or a plane, further
+#pragma unroll
+  for (int q = 0; q < 2; ++q) {
+    // feature n of columns 2t and 2t + 1: its place in the 16 bytes of the 8 features from n - r on
+    const int n = rb * 16 + q * 8 + r, s = n / KG, pt = (n % KG) / 32, pj = (n % 32) / 8;
+    uint4* step = a.h + (static_cast<int64_t>(seg) * hsteps + s) * 256 + pj * 32 + pt;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int col = 2 * t + i;
+      if (col < ntok) {
+        const float ga = acc[q][i], up = acc[q][2 + i];
+        const float h = __fdiv_rn(ga, 1.f + expf(-ga)) * up * col_w[col];
+        const __nv_bfloat16 hi = __float2bfloat16_rn(h);
+        __nv_bfloat16* at = reinterpret_cast<__nv_bfloat16*>(step + col * 4) + pair_place<BITS>(n);
+        at[0] = hi;
+        at[lo * 8] = __float2bfloat16_rn(h - __bfloat162float(hi));
+      }
+    }
+  }
+  if (rb == a.I / 16 - 1) {  // zeros behind the last feature of the last step
+    for (int p = a.I / 8; p < hsteps * 16; ++p) {
+      uint4* piece = a.h + (static_cast<int64_t>(seg) * hsteps + p / 16) * 256 + p % 4 * 32 + p % 16 / 4;
+      if (lane < 2 * ntok) piece[(lane & 1) * lo + (lane >> 1) * 4] = make_uint4(0, 0, 0, 0);
+    }
+  }
+}
+
+template <int BITS, bool V4>
 __global__ void __launch_bounds__(THREADS, 1)
-    few_gemm1_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_s, const FewArgs a) {
+    few_gemm1_kernel(const __grid_constant__ CUtensorMap tm_w, const FewArgs a) {
   extern __shared__ __align__(1024) uint8_t raw[];
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
-  constexpr int SS = Codes<BITS>::STEPS;  // steps of a tile
-  const int steps = (a.H + KG - 1) / KG, slots = (steps + 2 * SS - 1) / (2 * SS);
-  // [rings of codes][rings of scales][tokens in MMA order, nbuf segments][Smem1]; the router's sums before all but the last
-  const int ring_bytes = WARPS * a.depth1 * (SLOT1 + SCALE1);
-  const int xf_pieces = slots * 2 * SS * 128;  // of a segment: 2 KB a step
+  constexpr int SS = Codes<BITS>::STEPS;  // steps of a slot
+  const int steps = (a.H + KG - 1) / KG, slots = (steps + SS - 1) / SS;
+  // [rings of codes][tokens in MMA order, nbuf segments][Smem1]; the router's sums before all but the last
+  const int ring_bytes = WARPS * a.depth1 * SLOT1;
+  const int xf_pieces = slots * SS * 128;  // of a segment: 2 KB a step
   uint4* xf = reinterpret_cast<uint4*>(base + ring_bytes);
   Smem1& sm = *reinterpret_cast<Smem1*>(base + max(ring_bytes + a.nbuf * xf_pieces * 16, ROUTER_BYTES));
   cg::cluster_group cluster = cg::this_cluster();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int grid = static_cast<int>(gridDim.x), cta = static_cast<int>(blockIdx.x);
-  if (threadIdx.x < WARPS * MAX_DEPTH1) mbar_init(&sm.full[threadIdx.x / MAX_DEPTH1][threadIdx.x % MAX_DEPTH1], 1);
+  if (threadIdx.x < WARPS * MAX_DEPTH1) {
+    mbar_init(&sm.full[threadIdx.x / MAX_DEPTH1][threadIdx.x % MAX_DEPTH1], 1);
+    mbar_init(&sm.empty[threadIdx.x / MAX_DEPTH1][threadIdx.x % MAX_DEPTH1], 1);
+  }
+  asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   if (threadIdx.x == 0) {
     sm.abort_flag = 0;
     prefetch_map(&tm_w);
-    if (TS) prefetch_map(&tm_s);
-    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   for (int i = threadIdx.x; i < a.E; i += THREADS) sm.mask[i] = 0;
   asm volatile("barrier.cluster.arrive.aligned;" ::: "memory");
@@ -471,14 +533,16 @@ __global__ void __launch_bounds__(THREADS, 1)
 
   if (a.gate != nullptr) {
     LogitPart* parts = reinterpret_cast<LogitPart*>(base + RED_BYTES);
-    router_logits(a, reinterpret_cast<float (*)[64][RED_PITCH]>(base), parts, cluster);
+    float (*red)[64][RED_PITCH] = reinterpret_cast<float (*)[64][RED_PITCH]>(base);
+    if (a.T <= 8) router_logits<1>(a, red, parts, cluster);
+    else router_logits<4>(a, red, parts, cluster);
     cluster.sync();  // every CTA's sums are in every CTA
-    if (a.E > 64) {
-      for (int tok = warp; tok < a.T; tok += WARPS) choose<MAX_EXP / 32, 1>(a, sm, parts, tok);
-    } else if (warp + WARPS < a.T) {
-      choose<2, 2>(a, sm, parts, warp);
-    } else if (warp < a.T) {
-      choose<2, 1>(a, sm, parts, warp);
+    if (warp < WARPS) {
+#pragma unroll 1
+      for (int tok = warp; tok < a.T; tok += WARPS) {
+        if (a.E <= 64) choose<2>(a, sm, parts, tok);
+        else choose<MAX_EXP / 32>(a, sm, parts, tok);
+      }
     }
     if (a.logits != nullptr && cta == grid - 1)
       for (int i = threadIdx.x; i < a.T * a.E; i += THREADS) a.logits[i] = logit_of(a, parts, i % a.E, i / a.E);
@@ -525,7 +589,7 @@ __global__ void __launch_bounds__(THREADS, 1)
   pdl_trigger();
 
   // ---- GEMM1: this CTA's run [begin, end) of the jobs, with few segments inside one of them
-  const int tiles = a.I / 8, nseg = sm.nseg;
+  const int tiles = a.I / 16, nseg = sm.nseg;
   int begin, end;
   if (nseg > 0 && grid / nseg >= 8) {
     const int per = grid / nseg, s = cta / per, c = cta - s * per;  // CTAs of a segment
@@ -538,56 +602,56 @@ __global__ void __launch_bounds__(THREADS, 1)
   }
   // The run goes in windows of nbuf segments; the slots of a window's jobs are split evenly over the warps, so that a
   // job may begin in one warp and end in another.
-  const int kb = a.H * BITS / 8;  // bytes of a row of w1
-  uint8_t* ring = base + warp * a.depth1 * SLOT1;
-  uint8_t* sring = base + WARPS * a.depth1 * SLOT1 + warp * a.depth1 * SCALE1;
   volatile int* abort_flag = &sm.abort_flag;
   auto window_end = [&](int wb) { return min(end, (wb / tiles + a.nbuf) * tiles); };
   // the units (slots of jobs, in order) of window [wb, we) that warp w begins at
   auto unit = [&](int wb, int we, int w) { return static_cast<int>(static_cast<int64_t>(we - wb) * slots * w / WARPS); };
 
-  // what is copied next: slot lz of row block lrow of expert half lhalf; lleft units are left in the window at lwb
-  int lwb = begin, lleft = 0, lz = 0, lseg = 0, lrow = 0, lhalf = 0, lslot = 0;
-  auto open = [&]() {  // the first window from lwb on in which this warp has units
+  // Copies: lane w of the last warp follows warp w's jobs, slot lz of row block lrow of expert half lhalf next, `left`
+  // units left in the window at lwb.
+  int lwb = begin, left = 0, lz = 0, lseg = 0, lrow = 0, lhalf = 0, lslot = 0, issued = 0;
+  uint32_t lphase = 1;
+  auto open = [&]() {  // the first window from lwb on in which the warp has units
     for (; lwb < end; lwb = window_end(lwb)) {
-      const int we = window_end(lwb), u = unit(lwb, we, warp);
-      lleft = unit(lwb, we, warp + 1) - u;
-      if (lleft > 0) {
+      const int we = window_end(lwb), u = unit(lwb, we, lane);
+      left = unit(lwb, we, lane + 1) - u;
+      if (left > 0) {
         const int job = lwb + u / slots;
         lz = u % slots;
         lseg = job / tiles;
-        lrow = (job - lseg * tiles) * 8;
+        lrow = (job - lseg * tiles) * 16;
         lhalf = sm.seg[lseg].expert * 2;
         return;
       }
     }
   };
-  // The whole warp follows the cursor and three lanes issue a copy each (two tiles, the scales): one lane doing it all
-  // held the warp up for 950 cycles a slot.
-  const CUtensorMap* lmap = lane == 2 ? &tm_s : &tm_w;
-  auto fetch = [&]() {
-    uint64_t* bar = &sm.full[warp][lslot];
-    const bool two = lz * 256 + 128 < kb;
-    if (lane == 0) mbar_expect_tx(bar, SLOT1 - (two ? 0 : TILE1) + (TS ? SCALE1 : 0));
-    __syncwarp();
-    uint8_t* dst = lane == 2 ? sring + lslot * SCALE1 : ring + lslot * SLOT1 + lane * TILE1;
-    const int x = lane == 2 ? scale_index(lz * 2 * SS, a.gsteps1) & ~3 : lz * 256 + lane * 128;
-    if (lane == 0 || (lane == 1 && two) || (lane == 2 && TS)) tma_load_3d(dst, lmap, x, lrow, lhalf, bar);
-    if (++lslot == a.depth1) lslot = 0;
-    if (--lleft == 0) {
+  auto copy = [&]() {
+    uint64_t* bar = &sm.full[lane][lslot];
+    mbar_expect_tx(bar, SLOT1);
+    tma_load_3d(base + (lane * a.depth1 + lslot) * SLOT1, &tm_w, lz * 128, lrow, lhalf, bar);
+    ++issued;
+    if (++lslot == a.depth1) {
+      lslot = 0;
+      lphase ^= 1;
+    }
+    if (--left == 0) {
       lwb = window_end(lwb);
       open();
     } else if (++lz == slots) {
       lz = 0;
-      lrow += 8;
+      lrow += 16;
       if (lrow == a.I) {
         lrow = 0;
         lhalf = sm.seg[++lseg].expert * 2;
       }
     }
   };
-  open();
-  for (int i = 0; i < a.depth1 && lwb < end; ++i) fetch();
+  if (warp == WARPS) {
+    if (lane < WARPS) open();
+    else lwb = end;
+    for (int i = 0; i < a.depth1; ++i)
+      if (lwb < end) copy();
+  }
   if (cta == 0) {
     for (int i = threadIdx.x; i < nseg; i += THREADS) a.plan->seg[i] = sm.seg[i];
     if (threadIdx.x < MAX_PANELS) a.plan->done[threadIdx.x] = 0;
@@ -595,54 +659,63 @@ __global__ void __launch_bounds__(THREADS, 1)
   }
 
   const int r = Codes<BITS>::row_of(g);
-  const int hsteps = (a.I + KG - 1) / KG;
+  const uint32_t ring = smem_u32(base + warp * a.depth1 * SLOT1) + r * 128 + Codes<BITS>::offset(g, t);
   int slot = 0;
   uint32_t phase = 0;
   bool ok = true;
   for (int wb = begin; wb < end; wb = window_end(wb)) {
     const int we = window_end(wb), seg0 = wb / tiles, nsegs = (we - 1) / tiles - seg0 + 1;
     if (wb > begin) __syncthreads();  // the tokens of the window before are done with
-    // the segments' tokens to fp16 in MMA order, eight 16-byte pieces in flight per thread
+    // the segments' tokens in MMA order: every thread copies its 16-byte pieces, then makes them fp16 where they lie
     const int row = xf_pieces / 8;  // pieces of a token with the zeros behind it, a multiple of 16
     const int n0 = sm.seg[seg0].n, cols = n0 + (nsegs > 1 ? sm.seg[seg0 + 1].n : 0);
-    for (int i0 = 0; i0 < row * cols; i0 += 8 * THREADS) {
-      uint4 v[8];
+    auto piece = [&](int i, int& b, int& c, int& p) {
+      const int cc = i / row;
+      p = i - cc * row;
+      b = cc >= n0;
+      c = cc - b * n0;
+      // step p / 16, lane p / 4 % 4 of the quad, piece p % 4 of the lane
+      return xf + b * xf_pieces + ((p >> 4) * 4 + (p & 3)) * 32 + c * 4 + ((p >> 2) & 3);
+    };
+#pragma unroll 1
+    for (int i = threadIdx.x; i < row * cols; i += THREADS) {
+      int b, c, p;
+      const uint32_t dst = smem_u32(piece(i, b, c, p));
+      const bool in = p * 8 < a.H;
+      const uint4* src = reinterpret_cast<const uint4*>(a.x + static_cast<int64_t>(sm.seg[seg0 + b].token(c)) * a.H) + (in ? p : 0);
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(in ? 16 : 0) : "memory");
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+#pragma unroll 1
+    for (int i0 = 0; i0 < row * cols; i0 += THREADS) {
+      const int i = i0 + static_cast<int>(threadIdx.x);
+      const bool in = i < row * cols;  // (16 threads in a row share a step)
+      int b, c, p;
+      uint4* at = piece(in ? i : 0, b, c, p);
+      uint4 v = make_uint4(0, 0, 0, 0);
+      if (in) v = *at;
+      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+      float f[8];
+      uint32_t m = 0;
 #pragma unroll
-      for (int q = 0; q < 8; ++q) {
-        const int i = i0 + q * THREADS + static_cast<int>(threadIdx.x), cc = i / row, p = i - cc * row;
-        const int b = cc >= n0;
-        v[q] = make_uint4(0, 0, 0, 0);
-        if (cc < cols && p * 8 < a.H)
-          v[q] = __ldg(reinterpret_cast<const uint4*>(a.x + static_cast<int64_t>(sm.seg[seg0 + b].token(cc - b * n0)) * a.H) + p);
+      for (int k = 0; k < 4; ++k) {
+        f[2 * k] = __uint_as_float(w[k] << 16);
+        f[2 * k + 1] = __uint_as_float(w[k] & 0xffff0000u);
+        m = max(m, max(w[k] & 0x7fff0000u, (w[k] << 16) & 0x7fffffffu));
       }
 #pragma unroll
-      for (int q = 0; q < 8; ++q) {
-        const int i = i0 + q * THREADS + static_cast<int>(threadIdx.x), cc = i / row, p = i - cc * row;
-        const int b = cc >= n0, c = cc - b * n0;
-        const int s = p >> 4, pt = (p >> 2) & 3, pj = p & 3;  // step, lane of the quad, piece of the lane
-        const uint32_t w[4] = {v[q].x, v[q].y, v[q].z, v[q].w};
-        float f[8];
-        uint32_t m = 0;
+      for (int o = 8; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));  // the step's 16 pieces
+      const uint32_t e = min(max(m >> 23, 15u), 254u);  // largest magnitude in [2^(e-127), 2^(e-126))
+      const float up = __uint_as_float((268u - e) << 23);
+      uint32_t h[4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          f[2 * k] = __uint_as_float(w[k] << 16);
-          f[2 * k + 1] = __uint_as_float(w[k] & 0xffff0000u);
-          m = max(m, max(w[k] & 0x7fff0000u, (w[k] << 16) & 0x7fffffffu));
-        }
-#pragma unroll
-        for (int o = 8; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));  // the step's 16 pieces
-        const uint32_t e = min(max(m >> 23, 15u), 254u);  // largest magnitude in [2^(e-127), 2^(e-126))
-        const float up = __uint_as_float((268u - e) << 23);
-        uint32_t h[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const __half2 pr = __floats2half2_rn(f[pair_element<BITS>(2 * k)] * up, f[pair_element<BITS>(2 * k + 1)] * up);
-          h[k] = *reinterpret_cast<const uint32_t*>(&pr);
-        }
-        if (cc < cols) {
-          xf[b * xf_pieces + (s * 4 + pj) * 32 + c * 4 + pt] = make_uint4(h[0], h[1], h[2], h[3]);
-          if ((p & 15) == 0) sm.col_scale[b][s][c] = __uint_as_float((e - 14u) << 23);
-        }
+      for (int k = 0; k < 4; ++k) {
+        const __half2 pr = __floats2half2_rn(f[pair_element<BITS>(2 * k)] * up, f[pair_element<BITS>(2 * k + 1)] * up);
+        h[k] = *reinterpret_cast<const uint32_t*>(&pr);
+      }
+      if (in) {
+        *at = make_uint4(h[0], h[1], h[2], h[3]);
+        if ((p & 15) == 0) sm.col_scale[b][p >> 4][c] = __uint_as_float((e - 14u) << 23);
       }
     }
     if (threadIdx.x < cols) {
@@ -656,93 +729,93 @@ __global__ void __launch_bounds__(THREADS, 1)
     }
     __syncthreads();
 
-    // h of a finished job
-    auto emit = [&](int job, const float (&acc)[4]) {
-      const int seg = job / tiles, rb = job - seg * tiles, ntok = sm.seg[seg].n;
-      const bool packed = ntok <= 4;
-      // feature n = 8 rb + r of columns 2t and 2t + 1: its place in the 16 bytes of 8 features that rb is
-      const int n = rb * 8 + r, s = n / KG, pt = (n % KG) / 32, pj = (n % 32) / 8;
-      uint4* step = a.h + (static_cast<int64_t>(seg) * hsteps + s) * 256 + pj * 32 + pt;
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int col = 2 * t + i;
-        if (col < ntok) {
-          const float ga = acc[i], up = acc[2 + i];
-          const float h = __fdiv_rn(ga, 1.f + expf(-ga)) * up * sm.col_w[seg - seg0][col];
-          const __nv_bfloat16 hi = __float2bfloat16_rn(h);
-          __nv_bfloat16* at = reinterpret_cast<__nv_bfloat16*>(step + col * 4) + pair_place<BITS>(n);
-          at[0] = hi;
-          at[(packed ? 16 : 128) * 8] = __float2bfloat16_rn(h - __bfloat162float(hi));  // four columns, or a plane, further
+    if (warp == WARPS) {  // the copies of this window, as the warps give slots back
+      long long t0 = clock64();
+      bool more = lwb < we && ok;
+      while (__any_sync(0xffffffffu, more)) {
+        const bool can = more && mbar_test(&sm.empty[lane][lslot], lphase);
+        if (can) {
+          copy();
+          more = lwb < we;
+        }
+        if (__any_sync(0xffffffffu, can)) {
+          t0 = clock64();
+        } else if (*abort_flag || clock64() - t0 > kTimeoutCycles) {
+          if (lane == 0 && !*abort_flag) atomicExch(&g_device_error, 0x620);
+          *abort_flag = 1;
+          ok = false;
+          break;
+        } else {
+          __nanosleep(40);
         }
       }
-      if (rb == tiles - 1) {  // zeros behind the last feature of the last step
-        for (int p = tiles; p < hsteps * 16; ++p) {
-          uint4* piece = a.h + (static_cast<int64_t>(seg) * hsteps + p / 16) * 256 + p % 4 * 32 + p % 16 / 4;
-          if (lane < 2 * ntok) piece[(lane & 1) * (packed ? 16 : 128) + (lane >> 1) * 4] = make_uint4(0, 0, 0, 0);
-        }
-      }
-    };
-    int left = unit(wb, we, warp + 1) - unit(wb, we, warp);
+      __syncthreads();
+      continue;
+    }
+    int units = unit(wb, we, warp + 1) - unit(wb, we, warp);
     int job = wb + unit(wb, we, warp) / slots, za = unit(wb, we, warp) % slots;
-    float acc[4] = {0.f, 0.f, 0.f, 0.f};
+    float acc[2][4] = {};
     int open_job = -1;  // a job that this warp began and a later one ends
-    while (left > 0 && ok) {
-      const int zb = min(slots, za + left), seg = job / tiles, b = seg - seg0;
-      left -= zb - za;
-      const int64_t wrow = static_cast<int64_t>(sm.seg[seg].expert) * 2 * a.I + (job - seg * tiles) * 8 + r;
-      const float* fg = a.s1 + wrow * a.groups1;
-      const float* fu = fg + static_cast<int64_t>(a.I) * a.groups1;
-      float sc = TS ? 0.f : load_scale(fg, fu, za * 2 * SS, steps, a.gsteps1, t);
-      acc[0] = acc[1] = acc[2] = acc[3] = 0.f;
-      uint32_t xb = smem_u32(xf + b * xf_pieces + lane) + za * (2 * SS * 2048);
-      uint32_t cb = smem_u32(&sm.col_scale[b][za * 2 * SS][2 * t]);
-      for (int z = za; z < zb && ok; ++z) {
-        ok = mbar_wait(&sm.full[warp][slot], phase, abort_flag, 0x600 + warp);
-        const uint32_t tile = smem_u32(ring + slot * SLOT1) + r * 128, sa = smem_u32(sring + slot * SCALE1) + r * 16;
+    while (units > 0 && ok) {
+      const int zb = min(slots, za + units), seg = job / tiles, b = seg - seg0;
+      units -= zb - za;
+      // of the quad's rows lane t has the scales of gate (t even) or up row t / 2 * 8 + r of the job
+      const int64_t wrow = static_cast<int64_t>(sm.seg[seg].expert) * 2 * a.I + (t & 1) * a.I + (job - seg * tiles) * 16 + (t >> 1) * 8 + r;
+      RowScales<SS, V4> scales;
+      scales.start(a.s1 + wrow * a.groups1, za * SS, steps, a.gsteps1);
 #pragma unroll
-        for (int h = 0; h < 2 * SS; ++h) {  // behind the last step codes and tokens are zero
-          float f, v;
-          if (TS) {
-            const uint32_t at = sa + (scale_index(z * 2 * SS + h, a.gsteps1) & 3) * 4;
-            f = lds4(at);
-            v = lds4(at + SCALE1 / 2);
-          } else {
-            quad_scales(sc, f, v);
-            sc = load_scale(fg, fu, z * 2 * SS + h + 1, steps, a.gsteps1, t);
+      for (int i = 0; i < 4; ++i) acc[0][i] = acc[1][i] = 0.f;
+      uint32_t xb = smem_u32(xf + b * xf_pieces + lane) + za * (SS * 2048);
+      uint32_t cb = smem_u32(&sm.col_scale[b][za * SS][2 * t]);
+      for (int z = za; z < zb; ++z) {
+        ok = mbar_wait(&sm.full[warp][slot], phase, abort_flag, 0x600 + warp);
+        if (!ok) break;
+        uint32_t rows = ring + slot * SLOT1;
+#pragma unroll 1
+        for (int h = 0; h < SS; ++h, rows ^= 64) {  // behind the last step codes and tokens are zero
+          Codes<BITS> w[2][2];
+#pragma unroll
+          for (int q = 0; q < 2; ++q) {
+            w[q][0].load(rows + q * 1024);
+            w[q][1].load(rows + SLOT1 / 2 + q * 1024);
           }
-          const float c0 = lds4(cb + h * 32), c1 = lds4(cb + h * 32 + 4);
-          Codes<BITS> wg, wu;
-          wg.load128(tile + h / SS * TILE1, r, h % SS, t);
-          wu.load128(tile + h / SS * TILE1 + TILE1 / 2, r, h % SS, t);
-          float d0[4] = {0.f, 0.f, 0.f, 0.f}, d1[4] = {0.f, 0.f, 0.f, 0.f};  // two chains of MMAs
+          float f[2][2], d0[2][4] = {}, d1[2][4] = {};  // two chains of MMAs for each of the two row tiles
+          scales.get(z * SS + h, f);
+          const float c0 = lds4(cb), c1 = lds4(cb + 4);
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            const uint4 x = lds16(xb + h * 2048 + j * 512);
-            uint32_t ag[4], au[4];
-            wg.template pairs<true>(j, ag);
-            wu.template pairs<true>(j, au);
-            mma_f16(d0, ag[0], au[0], ag[1], au[1], x.x, x.y);
-            mma_f16(d1, ag[2], au[2], ag[3], au[3], x.z, x.w);
+            const uint4 x = lds16(xb + j * 512);
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+              uint32_t ag[4], au[4];
+              w[q][0].template pairs<true>(j, ag);
+              w[q][1].template pairs<true>(j, au);
+              mma_f16(d0[q], ag[0], au[0], ag[1], au[1], x.x, x.y);
+              mma_f16(d1[q], ag[2], au[2], ag[3], au[3], x.z, x.w);
+            }
           }
-          acc[0] = __fmaf_rn(f * c0, __fadd_rn(d0[0], d1[0]), acc[0]);
-          acc[1] = __fmaf_rn(f * c1, __fadd_rn(d0[1], d1[1]), acc[1]);
-          acc[2] = __fmaf_rn(v * c0, __fadd_rn(d0[2], d1[2]), acc[2]);
-          acc[3] = __fmaf_rn(v * c1, __fadd_rn(d0[3], d1[3]), acc[3]);
+#pragma unroll
+          for (int q = 0; q < 2; ++q)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              acc[q][i] = __fmaf_rn(f[q][i >> 1] * ((i & 1) ? c1 : c0), __fadd_rn(d0[q][i], d1[q][i]), acc[q][i]);
+          xb += 2048;
+          cb += 32;
         }
-        xb += 2 * SS * 2048;
-        cb += 2 * SS * 32;
+        scales.next(z * SS);
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // our reads of the slot before its refill
         __syncwarp();
-        if (lwb < end && ok) fetch();
+        if (lane == 0) mbar_arrive(&sm.empty[warp][slot]);
         if (++slot == a.depth1) {
           slot = 0;
           phase ^= 1;
         }
       }
       if (za == 0 && zb == slots) {
-        emit(job, acc);
+        emit<BITS>(a, sm.seg[seg], sm.col_w[b], seg, job - seg * tiles, acc);
       } else if (za > 0) {
-        sm.head[warp][lane] = make_float4(acc[0], acc[1], acc[2], acc[3]);
+#pragma unroll
+        for (int q = 0; q < 2; ++q) sm.head[warp][q][lane] = make_float4(acc[q][0], acc[q][1], acc[q][2], acc[q][3]);
       } else {
         open_job = job;
       }
@@ -754,39 +827,41 @@ __global__ void __launch_bounds__(THREADS, 1)
       const int stop = (open_job - wb + 1) * slots;
       for (int w = warp + 1; w < WARPS && unit(wb, we, w) < stop; ++w) {
         if (unit(wb, we, w) == unit(wb, we, w + 1)) continue;
-        const float4 v = sm.head[w][lane];
-        acc[0] = __fadd_rn(acc[0], v.x);
-        acc[1] = __fadd_rn(acc[1], v.y);
-        acc[2] = __fadd_rn(acc[2], v.z);
-        acc[3] = __fadd_rn(acc[3], v.w);
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          const float4 v = sm.head[w][q][lane];
+          acc[q][0] = __fadd_rn(acc[q][0], v.x);
+          acc[q][1] = __fadd_rn(acc[q][1], v.y);
+          acc[q][2] = __fadd_rn(acc[q][2], v.z);
+          acc[q][3] = __fadd_rn(acc[q][3], v.w);
+        }
       }
-      emit(open_job, acc);
+      const int seg = open_job / tiles;
+      emit<BITS>(a, sm.seg[seg], sm.col_w[seg - seg0], seg, open_job - seg * tiles, acc);
     }
   }
   // never leave copies in flight into this CTA's shared memory
-  if (!ok && lane == 0) {
+  if (warp == WARPS && lane < WARPS && *abort_flag) {
     const long long t0 = clock64();
-    for (int i = 0; i < a.depth1; ++i) {
-      const int q = (slot + i) % a.depth1;
-      while (!mbar_try_wait(&sm.full[warp][q], q < slot ? phase ^ 1 : phase) && clock64() - t0 < kTimeoutCycles) {
+    for (int i = max(0, issued - a.depth1); i < issued; ++i)
+      while (!mbar_try_wait(&sm.full[lane][i % a.depth1], (i / a.depth1) & 1) && clock64() - t0 < kTimeoutCycles) {
       }
-    }
   }
 }
 
-constexpr int MT = 8;                  // 16-row tiles of a panel, one warp of a group each
-constexpr int PANEL = MT * 16;         // output features of a CTA of kernel 2
-constexpr int GROUPS = WARPS / MT;     // groups of a CTA, each with a part of the steps
+constexpr int MT = 4;                  // warps of a group, 32 rows each
+constexpr int PANEL = MT * 32;         // output features of a CTA of kernel 2
+constexpr int GROUPS = 2;              // groups of a CTA, each with a part of the steps
+constexpr int WARPS2 = MT * GROUPS;
+constexpr int THREADS2 = (WARPS2 + 1) * 32;  // and a warp that issues the copies
 constexpr int MAX_DEPTH2 = 4;
-constexpr int THREADS2 = THREADS + 32;  // and a warp that issues the copies
 
 template <int BITS>
-struct Stage2 {  // 128 bytes of the panel's packed rows (two steps at INT4, one at INT8), h, four scales of the rows
+struct Stage2 {  // 128 bytes of the panel's packed rows (two steps at INT4, one at INT8), and h
   static constexpr int STEPS = Codes<BITS>::STEPS;
   static constexpr int W = PANEL * 128;
   static constexpr int H = STEPS * 4096;
-  static constexpr int S = PANEL * 16;
-  static constexpr int BYTES = W + H + S;
+  static constexpr int BYTES = W + H;
 };
 
 struct Smem2 {
@@ -797,9 +872,9 @@ struct Smem2 {
   int last;
 };
 
-template <int BITS, bool TS>
+template <int BITS, bool V4>
 __global__ void __launch_bounds__(THREADS2, 1)
-    few_gemm2_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_s, const FewArgs a) {
+    few_gemm2_kernel(const __grid_constant__ CUtensorMap tm_w, const FewArgs a) {
   extern __shared__ __align__(1024) uint8_t raw[];
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
   using S = Stage2<BITS>;
@@ -817,14 +892,13 @@ __global__ void __launch_bounds__(THREADS2, 1)
   if (threadIdx.x == 0) {
     sm.abort_flag = 0;
     prefetch_map(&tm_w);
-    if (TS) prefetch_map(&tm_s);
   }
   for (int i = threadIdx.x; i < GROUPS * PANEL * pitch; i += THREADS2) parts[i] = 0.f;
   asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   pdl_wait();
   asm volatile("fence.proxy.async.global;" ::: "memory");  // kernel 1's stores of h before the copies read them
   const int nseg = a.plan->n;
-  if (threadIdx.x < MAX_SEG) sm.seg[threadIdx.x] = a.plan->seg[threadIdx.x];  // (those behind the last are not looked at)
+  for (int i = threadIdx.x; i < MAX_SEG; i += THREADS2) sm.seg[i] = a.plan->seg[i];  // (those behind the last are not looked at)
   __syncthreads();
 
   // the slots (a stage each) of all segments in a row; a group has [begin, end) of them
@@ -833,7 +907,7 @@ __global__ void __launch_bounds__(THREADS2, 1)
   auto bound = [&](int grp) { return static_cast<int>(total * (rank * GROUPS + grp) / (a.split * GROUPS)); };
   volatile int* abort_flag = &sm.abort_flag;
 
-  if (warp == WARPS) {
+  if (warp == WARPS2) {
     // ---- copies: the groups' next slots in turn
     int at[GROUPS], seg[GROUPS], z[GROUPS], st[GROUPS], issued[GROUPS];
     uint32_t ph[GROUPS];
@@ -858,11 +932,10 @@ __global__ void __launch_bounds__(THREADS2, 1)
           const int n = min(SS, steps - z[q] * SS);
           const int hb = sg.n <= 4 ? 2048 : 4096;  // of a step
           const int y = sg.expert * a.H + panel * PANEL;
-          if (lane == 0) mbar_expect_tx(bar, S::W + n * hb + (TS ? S::S : 0));
+          if (lane == 0) mbar_expect_tx(bar, S::W + n * hb);
           __syncwarp();
           if (lane == 0) {
             tma_load_2d(dst, &tm_w, z[q] * 128, y, bar);
-            if (TS) tma_load_2d(dst + S::W + S::H, &tm_s, scale_index(z[q] * SS, a.gsteps2) & ~3, y, bar);
           } else if (lane <= n) {
             bulk_load(dst + S::W + (lane - 1) * 4096, a.h + (static_cast<int64_t>(seg[q]) * steps + z[q] * SS + lane - 1) * 256,
                       hb, bar);
@@ -890,8 +963,9 @@ __global__ void __launch_bounds__(THREADS2, 1)
     }
   } else {
     const int begin = bound(group), end = bound(group + 1);
-    const int r = Codes<BITS>::row_of(g), r0 = tile * 16 + r;  // this lane's rows of the panel: r0 and r0 + 8
-    const int n0 = min(panel * PANEL + r0, a.H - 1), n1 = min(panel * PANEL + r0 + 8, a.H - 1);
+    const int r0 = tile * 32 + Codes<BITS>::row_of(g);  // this lane's rows of the panel: r0, and 8, 16 and 24 further
+    const int ns = min(panel * PANEL + r0 + 8 * t, a.H - 1);  // the one that it has the scales of
+    const uint32_t lane_row = r0 * 128 + Codes<BITS>::offset(g, t);
     bool ok = true;
     int st = 0;
     uint32_t phase = 0;
@@ -899,62 +973,51 @@ __global__ void __launch_bounds__(THREADS2, 1)
       const int si = at / slots, za = at - si * slots, zb = min(slots, za + end - at);
       const Segment sg = sm.seg[si];
       const bool packed = sg.n <= 4;
-      const float* f0 = a.s2 + (static_cast<int64_t>(sg.expert) * a.H + n0) * a.groups2;
-      const float* f1 = a.s2 + (static_cast<int64_t>(sg.expert) * a.H + n1) * a.groups2;
-      float acc[4] = {0.f, 0.f, 0.f, 0.f};
-      float sc = TS ? 0.f : load_scale(f0, f1, za * SS, steps, a.gsteps2, t);
+      RowScales<SS, V4> scales;
+      scales.start(a.s2 + (static_cast<int64_t>(sg.expert) * a.H + ns) * a.groups2, za * SS, steps, a.gsteps2);
+      float acc[2][4] = {};
       for (int z = za; z < zb; ++z, ++at) {
         ok = mbar_wait(&sm.full[group][st], phase, abort_flag, 0x610 + group);
         if (!ok) break;
         const uint32_t stage = smem_u32(base + (group * depth + st) * S::BYTES);
+        uint32_t rows = stage + lane_row, ha = stage + S::W + lane * 16;
+#pragma unroll 1
+        for (int h = 0; h < SS; ++h, rows ^= 64, ha += 4096) {
+          if (z * SS + h < steps) {
+            Codes<BITS> w[2][2];
 #pragma unroll
-        for (int h = 0; h < SS; ++h) {
-          const int s = z * SS + h;
-          if (s < steps) {
-            const uint32_t ha = stage + S::W + h * 4096 + lane * 16;
-            Codes<BITS> w0, w1;
-            w0.load128(stage + r0 * 128, r, h, t);
-            w1.load128(stage + (r0 + 8) * 128, r, h, t);
-            float f, v;
-            if (TS) {
-              const uint32_t fa = stage + S::W + S::H + r0 * 16 + (scale_index(s, a.gsteps2) & 3) * 4;
-              f = lds4(fa);
-              v = lds4(fa + 128);
-            } else {
-              quad_scales(sc, f, v);
-              sc = load_scale(f0, f1, s + 1, steps, a.gsteps2, t);
-            }
-            float d0[4] = {0.f, 0.f, 0.f, 0.f}, d1[4] = {0.f, 0.f, 0.f, 0.f};  // chains of MMAs
-            if (packed) {
+            for (int q = 0; q < 2; ++q)
 #pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                const uint4 hv = lds16(ha + j * 512);
-                uint32_t p0[4], p1[4];
-                w0.template pairs<false>(j, p0);
-                w1.template pairs<false>(j, p1);
-                mma_bf16(d0, p0[0], p1[0], p0[1], p1[1], hv.x, hv.y);
-                mma_bf16(d1, p0[2], p1[2], p0[3], p1[3], hv.z, hv.w);
+              for (int i = 0; i < 2; ++i) w[q][i].load(rows + (2 * q + i) * 1024);
+            float f[2][2], d0[2][4] = {}, d1[2][4] = {};  // chains of MMAs
+            scales.get(z * SS + h, f);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const uint4 hv = lds16(ha + j * 512);
+              uint32_t p[2][2][4];
+#pragma unroll
+              for (int q = 0; q < 2; ++q) {
+#pragma unroll
+                for (int i = 0; i < 2; ++i) w[q][i].template pairs<false>(j, p[q][i]);
+                mma_bf16(d0[q], p[q][0][0], p[q][1][0], p[q][0][1], p[q][1][1], hv.x, hv.y);
+                mma_bf16(d1[q], p[q][0][2], p[q][1][2], p[q][0][3], p[q][1][3], hv.z, hv.w);
               }
-            } else {
-              float d2[4] = {0.f, 0.f, 0.f, 0.f}, d3[4] = {0.f, 0.f, 0.f, 0.f};
+              if (!packed) {
+                const uint4 lv = lds16(ha + 2048 + j * 512);
 #pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                const uint4 hv = lds16(ha + j * 512), lv = lds16(ha + 2048 + j * 512);
-                uint32_t p0[4], p1[4];
-                w0.template pairs<false>(j, p0);
-                w1.template pairs<false>(j, p1);
-                mma_bf16(d0, p0[0], p1[0], p0[1], p1[1], hv.x, hv.y);
-                mma_bf16(d1, p0[2], p1[2], p0[3], p1[3], hv.z, hv.w);
-                mma_bf16(d2, p0[0], p1[0], p0[1], p1[1], lv.x, lv.y);
-                mma_bf16(d3, p0[2], p1[2], p0[3], p1[3], lv.z, lv.w);
+                for (int q = 0; q < 2; ++q) {
+                  mma_bf16(d0[q], p[q][0][0], p[q][1][0], p[q][0][1], p[q][1][1], lv.x, lv.y);
+                  mma_bf16(d1[q], p[q][0][2], p[q][1][2], p[q][0][3], p[q][1][3], lv.z, lv.w);
+                }
               }
-#pragma unroll
-              for (int i = 0; i < 4; ++i) d0[i] = __fadd_rn(d0[i], __fadd_rn(d2[i], d3[i]));
             }
 #pragma unroll
-            for (int i = 0; i < 4; ++i) acc[i] = __fmaf_rn(i < 2 ? f : v, __fadd_rn(d0[i], d1[i]), acc[i]);
+            for (int q = 0; q < 2; ++q)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) acc[q][i] = __fmaf_rn(f[q][i >> 1], __fadd_rn(d0[q][i], d1[q][i]), acc[q][i]);
           }
         }
+        scales.next(z * SS);
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // our reads of the stage before its refill
         __syncwarp();
         if (lane == 0) mbar_arrive(&sm.empty[group][st]);
@@ -965,7 +1028,9 @@ __global__ void __launch_bounds__(THREADS2, 1)
       }
       if (packed) {  // columns 4 to 7 are the lo parts of 0 to 3
 #pragma unroll
-        for (int i = 0; i < 4; ++i) acc[i] = __fadd_rn(acc[i], __shfl_xor_sync(0xffffffffu, acc[i], 2));
+        for (int q = 0; q < 2; ++q)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) acc[q][i] = __fadd_rn(acc[q][i], __shfl_xor_sync(0xffffffffu, acc[q][i], 2));
       }
       // rows belong to this warp alone, and the tokens of a segment are distinct
 #pragma unroll
@@ -973,8 +1038,8 @@ __global__ void __launch_bounds__(THREADS2, 1)
         const int col = 2 * t + i;
         if (col < sg.n) {
           float* p = parts + (group * PANEL + r0) * pitch + sg.token(col);
-          p[0] += acc[i];
-          p[8 * pitch] += acc[2 + i];
+#pragma unroll
+          for (int q = 0; q < 4; ++q) p[8 * q * pitch] += acc[q >> 1][2 * (q & 1) + i];
         }
       }
       __syncwarp();
@@ -1003,20 +1068,29 @@ __global__ void __launch_bounds__(THREADS2, 1)
   if (!sm.last) return;
   __threadfence();
   // the CTA that finishes last adds the CTAs' parts, again in the order of their steps
-  const float* all = a.partial + static_cast<int64_t>(panel) * a.split * (PANEL * a.T);
-  for (int i = threadIdx.x; i < PANEL * a.T; i += THREADS2) {
-    float v[MAX_SPLIT];
+  const float4* all = reinterpret_cast<const float4*>(a.partial + static_cast<int64_t>(panel) * a.split * (PANEL * a.T));
+  const int vecs = PANEL * a.T / 4;
+  for (int i = threadIdx.x; i < vecs; i += THREADS2) {
+    float4 v[MAX_SPLIT];
 #pragma unroll
-    for (int c = 0; c < MAX_SPLIT; ++c) v[c] = c < a.split ? __ldcg(all + static_cast<int64_t>(c) * (PANEL * a.T) + i) : 0.f;
+    for (int c = 0; c < MAX_SPLIT; ++c) v[c] = c < a.split ? __ldcg(all + c * vecs + i) : make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-    for (int c = 1; c < MAX_SPLIT; ++c) v[0] = __fadd_rn(v[0], v[c]);
-    store(i, v[0]);
+    for (int c = 1; c < MAX_SPLIT; ++c) {
+      v[0].x = __fadd_rn(v[0].x, v[c].x);
+      v[0].y = __fadd_rn(v[0].y, v[c].y);
+      v[0].z = __fadd_rn(v[0].z, v[c].z);
+      v[0].w = __fadd_rn(v[0].w, v[c].w);
+    }
+    store(4 * i, v[0].x);
+    store(4 * i + 1, v[0].y);
+    store(4 * i + 2, v[0].z);
+    store(4 * i + 3, v[0].w);
   }
 }
 
 template <typename K>
 int launch_few_kernel(K kernel, int grid, int cluster, int threads, int smem, cudaStream_t st, const CUtensorMap& tw,
-                      const CUtensorMap& ts, const FewArgs& a, const char* what) {
+                      const FewArgs& a, const char* what) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(grid);
   cfg.blockDim = dim3(threads);
@@ -1030,7 +1104,7 @@ int launch_few_kernel(K kernel, int grid, int cluster, int threads, int smem, cu
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = cluster > 1 ? 2 : 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, tw, ts, a);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, tw, a);
   if (e != cudaSuccess) {
     cudaGetLastError();
     return fail(LLQ_ECUDA, "%s: %s", what, cudaGetErrorString(e));
@@ -1052,26 +1126,20 @@ int allow_smem(K kernel, std::atomic<uint64_t>& ready) {
   return e == cudaSuccess ? LLQ_OK : fail(LLQ_ECUDA, "few-token layer: %s", cudaGetErrorString(e));
 }
 
-template <int BITS, bool TS>
+template <int BITS, bool V4>
 int launch_gemm1(FewArgs& a, const int8_t* q1, cudaStream_t st) {
-  // w1 as [2 E halves][I rows][bytes]: a copy takes 8 gate rows and the same up rows
-  const uint64_t kb = static_cast<uint64_t>(a.H) * BITS / 8, gb = static_cast<uint64_t>(a.groups1) * 4;
-  CUtensorMap tw, ts;
-  int rc = make_map_3d(&tw, q1, CU_TENSOR_MAP_DATA_TYPE_UINT8, kb, a.I, 2 * static_cast<uint64_t>(a.E), kb, kb * a.I, 128, 8,
+  // w1 as [2 E halves][I rows][bytes]: a copy takes 16 gate rows and the same up rows
+  const uint64_t kb = static_cast<uint64_t>(a.H) * BITS / 8;
+  CUtensorMap tw;
+  int rc = make_map_3d(&tw, q1, CU_TENSOR_MAP_DATA_TYPE_UINT8, kb, a.I, 2 * static_cast<uint64_t>(a.E), kb, kb * a.I, 128, 16,
                        2, CU_TENSOR_MAP_SWIZZLE_128B);
   if (rc) return rc;
-  ts = tw;
-  if (TS) {
-    rc = make_map_3d(&ts, a.s1, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, a.groups1, a.I, 2 * static_cast<uint64_t>(a.E), gb, gb * a.I,
-                     4, 8, 2, CU_TENSOR_MAP_SWIZZLE_NONE);
-    if (rc) return rc;
-  }
   static std::atomic<uint64_t> ready{0};
-  rc = allow_smem(few_gemm1_kernel<BITS, TS>, ready);
+  rc = allow_smem(few_gemm1_kernel<BITS, V4>, ready);
   if (rc) return rc;
-  // two segments' tokens and two slots of every ring where they fit (H up to 2048), then one segment's, then one slot
+  // two segments' tokens and two slots of every ring where they fit, then one segment's, then one slot
   constexpr int SS = Codes<BITS>::STEPS;
-  const int seg = ((a.H + KG - 1) / KG + 2 * SS - 1) / (2 * SS) * (2 * SS) * 2048, slot = WARPS * (SLOT1 + SCALE1);
+  const int seg = ((a.H + KG - 1) / KG + SS - 1) / SS * SS * 2048, slot = WARPS * SLOT1;
   int smem = 0;
   for (int i = 0; i < 3; ++i) {
     a.nbuf = i == 0 ? 2 : 1;
@@ -1080,37 +1148,34 @@ int launch_gemm1(FewArgs& a, const int8_t* q1, cudaStream_t st) {
     if (smem <= kSmemMost) break;
   }
   if (smem > kSmemMost) return fail(LLQ_EUNSUPPORTED, "the few-token layer has no room for rows of %d", a.H);
-  return launch_few_kernel(few_gemm1_kernel<BITS, TS>, num_sms() / CL1 * CL1, CL1, THREADS, smem, st, tw, ts, a, "few_gemm1_kernel");
+  return launch_few_kernel(few_gemm1_kernel<BITS, V4>, num_sms() / CL1 * CL1, CL1, THREADS, smem, st, tw, a, "few_gemm1_kernel");
 }
 
-template <int BITS, bool TS>
+template <int BITS, bool V4>
 int launch_gemm2(FewArgs& a, cudaStream_t st) {
-  const uint64_t kb = static_cast<uint64_t>(a.I) * BITS / 8, rows = static_cast<uint64_t>(a.E) * a.H;
-  CUtensorMap tw, ts;
-  int rc = make_map(&tw, a.q2, CU_TENSOR_MAP_DATA_TYPE_UINT8, kb, rows, kb, 128, PANEL, CU_TENSOR_MAP_SWIZZLE_128B);
+  const uint64_t kb = static_cast<uint64_t>(a.I) * BITS / 8;
+  CUtensorMap tw;
+  int rc = make_map(&tw, a.q2, CU_TENSOR_MAP_DATA_TYPE_UINT8, kb, static_cast<uint64_t>(a.E) * a.H, kb, 128, PANEL,
+                    CU_TENSOR_MAP_SWIZZLE_128B);
   if (rc) return rc;
-  ts = tw;
-  if (TS) {
-    rc = make_map(&ts, a.s2, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, a.groups2, rows, static_cast<uint64_t>(a.groups2) * 4, 4, PANEL,
-                  CU_TENSOR_MAP_SWIZZLE_NONE);
-    if (rc) return rc;
-  }
   static std::atomic<uint64_t> ready{0};
-  rc = allow_smem(few_gemm2_kernel<BITS, TS>, ready);
+  rc = allow_smem(few_gemm2_kernel<BITS, V4>, ready);
   if (rc) return rc;
   // as deep as the partial outputs leave room for
   const int fixed = 1024 + static_cast<int>(sizeof(Smem2)) + GROUPS * PANEL * (a.T | 1) * 4;
   a.depth2 = std::min(MAX_DEPTH2, (kSmemMost - fixed) / (GROUPS * Stage2<BITS>::BYTES));
-  return launch_few_kernel(few_gemm2_kernel<BITS, TS>, panels_of(a.H) * a.split, 1, THREADS2,
-                           fixed + GROUPS * a.depth2 * Stage2<BITS>::BYTES, st, tw, ts, a, "few_gemm2_kernel");
+  return launch_few_kernel(few_gemm2_kernel<BITS, V4>, panels_of(a.H) * a.split, 1, THREADS2,
+                           fixed + GROUPS * a.depth2 * Stage2<BITS>::BYTES, st, tw, a, "few_gemm2_kernel");
 }
 
 template <int BITS>
 int launch_few(FewArgs& a, const int8_t* q1, cudaStream_t st) {
-  auto aligned = [](const float* s, int groups) { return groups % 4 == 0 && (reinterpret_cast<uintptr_t>(s) & 15) == 0; };
-  const int rc = aligned(a.s1, a.groups1) ? launch_gemm1<BITS, true>(a, q1, st) : launch_gemm1<BITS, false>(a, q1, st);
+  auto v4 = [](const float* s, int groups, int gsteps) {
+    return gsteps == 1 && groups % 4 == 0 && (reinterpret_cast<uintptr_t>(s) & 15) == 0;
+  };
+  const int rc = v4(a.s1, a.groups1, a.gsteps1) ? launch_gemm1<BITS, true>(a, q1, st) : launch_gemm1<BITS, false>(a, q1, st);
   if (rc) return rc;
-  return aligned(a.s2, a.groups2) ? launch_gemm2<BITS, true>(a, st) : launch_gemm2<BITS, false>(a, st);
+  return v4(a.s2, a.groups2, a.gsteps2) ? launch_gemm2<BITS, true>(a, st) : launch_gemm2<BITS, false>(a, st);
 }
 
 inline size_t up256(size_t v) { return (v + 255) / 256 * 256; }
