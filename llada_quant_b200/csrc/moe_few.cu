@@ -54,7 +54,7 @@ constexpr int MAX_K = 32;
 constexpr int MAX_SEG = MAX_EXP + MAX_T * MAX_K / 8;
 constexpr int CL1 = 2;        // CTAs of a cluster of kernel 1: all 148 SMs hold one (of 8, with this much
                               // shared memory, only 120 CTAs fit at once)
-constexpr int WARPS = 12;     // of kernel 1 that compute, and one that issues the copies
+constexpr int WARPS = 15;     // of kernel 1 that compute, and one that issues the copies
 constexpr int THREADS = (WARPS + 1) * 32;
 constexpr int KG = 128;       // K elements of a step: 32 for each of a quad's four lanes
 
@@ -311,7 +311,7 @@ struct Smem1 {
 
 using LogitPart = float[MAX_T][MAX_EXP];
 
-// The router: K is split over the CTAs of the cluster and six slices of warps in each; half of the warps take 32 of
+// The router: K is split over the CTAs of the cluster and seven slices of warps in each; half of the warps take 32 of
 // 64 experts at a time, the others the next 32.  A slice's sums meet in `red`, a CTA's in parts[rank] of both CTAs.
 template <int NT>  // tiles of 8 tokens
 __device__ void router_logits(const FewArgs& a, float (*red)[64][RED_PITCH], LogitPart* parts, cg::cluster_group& cluster) {
@@ -322,7 +322,7 @@ __device__ void router_logits(const FewArgs& a, float (*red)[64][RED_PITCH], Log
   const int p0 = pairs * rank / CL1, p1 = pairs * (rank + 1) / CL1;
 #pragma unroll 1
   for (int eg = 0; eg < a.E; eg += 64) {
-    if (warp < WARPS) {
+    if (warp < 2 * RED_SLICES) {
       float d[2][NT][4] = {};
       const __nv_bfloat16* w[4];
 #pragma unroll
@@ -851,7 +851,7 @@ __global__ void __launch_bounds__(THREADS, 1)
 
 constexpr int MT = 4;                  // warps of a group, 32 rows each
 constexpr int PANEL = MT * 32;         // output features of a CTA of kernel 2
-constexpr int GROUPS = 2;              // groups of a CTA, each with a part of the steps
+constexpr int GROUPS = 3;              // groups of a CTA, each with a part of the steps
 constexpr int WARPS2 = MT * GROUPS;
 constexpr int THREADS2 = (WARPS2 + 1) * 32;  // and a warp that issues the copies
 constexpr int MAX_DEPTH2 = 4;
@@ -920,10 +920,12 @@ __global__ void __launch_bounds__(THREADS2, 1)
       ph[q] = 1;
     }
     bool ok = true;
-    while (ok && (at[0] < bound(1) || at[GROUPS - 1] < bound(GROUPS))) {
+    for (bool more = true; more && ok;) {
+      more = false;
 #pragma unroll
       for (int q = 0; q < GROUPS; ++q) {
         if (ok && at[q] < bound(q + 1)) {
+          more = true;
           ok = mbar_wait(&sm.empty[q][st[q]], ph[q], abort_flag, 0x620 + q);
           if (!ok) break;
           const Segment sg = sm.seg[seg[q]];
