@@ -31,11 +31,49 @@ __device__ __forceinline__ float ratio(float v, float amax) {
   return __fdiv_rn(__fmul_rn(v, 0.4375f), __fmul_rn(amax, 0x1p-10f));
 }
 
+// v * 448 / amax by the reciprocal and one correction with the exact remainder (Markstein, 1990): within a rounding of
+// the quotient, and the quotient itself where it fits in fp32.  Of bf16 or fp16 values it is either a border between two
+// codes exactly or at least 2^-22 of itself away from one (the numerator has 14 bits at most, a border times the
+// denominator 16, both in units that differ by powers of two), so the code is that of ratio().  fp32 values may come
+// closer: quantize_values looks.
+struct Divider {
+  float a, r;
+  __device__ __forceinline__ explicit Divider(float amax) {
+    a = __fmul_rn(amax, 0x1p-10f);
+    r = __fdiv_rn(1.f, a);
+    a = fminf(a, 3e38f);  // amax infinite: r = 0, and every finite value gives 0
+  }
+  __device__ __forceinline__ float operator()(float v) const {
+    const float n = __fmul_rn(v, 0.4375f), q = __fmul_rn(n, r);
+    return copysignf(__fmaf_rn(__fmaf_rn(-q, a, n), r, q), v);  // (the correction makes +0 of -0)
+  }
+};
+
 // two values to e4m3 (nearest even; NaN stays NaN), lo in the low byte
 __device__ __forceinline__ uint16_t to_e4m3x2(float lo, float hi) {
   uint16_t r;
   asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
   return r;
+}
+
+// The codes of N values of type T of a group: e4m3 of ratio(v).  (A division for each value took 42 us at 8192 x 4096
+// bf16, and a test for borders with the division behind it 50: a quarter of all groups of bf16 values has some on one.)
+template <typename T, int N>
+__device__ __forceinline__ void quantize_values(const float (&v)[N], float amax, const Divider& div, uint16_t (&q)[N / 2]) {
+  uint32_t differ = 0;
+#pragma unroll
+  for (int i = 0; i < N / 2; ++i) {
+    const float x = div(v[2 * i]), y = div(v[2 * i + 1]);
+    q[i] = to_e4m3x2(x, y);
+    if (sizeof(T) == 4) {  // next to a border?
+      const float lo = 1.f - 0x1p-22f, hi = 1.f + 0x1p-22f;
+      differ |= to_e4m3x2(x * lo, y * lo) ^ to_e4m3x2(x * hi, y * hi);
+    }
+  }
+  if (sizeof(T) == 4 && differ) {
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) q[i] = to_e4m3x2(ratio(v[2 * i], amax), ratio(v[2 * i + 1], amax));
+  }
 }
 
 // two e4m3 codes as an fp16 pair, exactly
@@ -99,33 +137,40 @@ __device__ __forceinline__ void store_part(uint8_t* row, int64_t c, int64_t K, c
   }
 }
 
-// one scale per 128 values of a row: 16 lanes hold a group, 8 values each
-template <typename T>
-__global__ void __launch_bounds__(256) fp8_rows_kernel(const T* __restrict__ x, int64_t M, int64_t K, int64_t ldx, int vec,
+// One scale per 128 values of a row: 16 lanes hold a group, 8 values each, and two groups at a time, both asked for
+// before either is used.  I: 32-bit indices of groups where they fit (a 64-bit division per group took as long as all
+// the rest).
+template <typename T, typename I>
+__global__ void __launch_bounds__(256) fp8_rows_kernel(const T* __restrict__ x, I n, I G, int64_t K, int64_t ldx, int vec,
                                                        uint8_t* __restrict__ codes, int64_t ldc, float* __restrict__ scale) {
   pdl_wait();
-  const int64_t G = (K + BLK - 1) / BLK;
-  const int64_t n = M * G;
   const int l = threadIdx.x & 15;
-  for (int64_t i = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) >> 4; i - (threadIdx.x >> 4 & 1) < n;
-       i += static_cast<int64_t>(gridDim.x) * (blockDim.x >> 4)) {
-    const bool in = i < n;  // a warp's two groups leave the loop together
-    const int64_t m = in ? i / G : 0, g = in ? i - m * G : 0;
-    const int64_t c = g * BLK + 8 * l;
-    float v[8];
-    load_part(x + m * ldx, in ? c : K, K, vec != 0, v);
-    uint32_t b = 0;
+  const I stride = static_cast<I>(gridDim.x) * (blockDim.x >> 4);
+  const I first = static_cast<I>(blockIdx.x) * (blockDim.x >> 4) + (threadIdx.x >> 4);
+#pragma unroll 1
+  for (I i0 = first; i0 - (threadIdx.x >> 4 & 1) < n; i0 += 2 * stride) {  // a warp's lanes leave the loop together
+    float v[2][8];
+    I m[2];
+    int64_t c[2];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) b = max(b, mag(v[j]));
+    for (int q = 0; q < 2; ++q) {
+      const I i = i0 + q * stride;
+      m[q] = i < n ? i / G : 0;
+      c[q] = i < n ? static_cast<int64_t>(i - m[q] * G) * BLK + 8 * l : K;
+      load_part(x + static_cast<int64_t>(m[q]) * ldx, c[q], K, vec != 0, v[q]);
+    }
 #pragma unroll
-    for (int o = 8; o > 0; o >>= 1) b = max(b, __shfl_xor_sync(0xffffffffu, b, o));
-    const float amax = group_amax(b);
-    uint16_t q[4];
+    for (int q = 0; q < 2; ++q) {
+      uint32_t b = 0;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) q[j] = to_e4m3x2(ratio(v[2 * j], amax), ratio(v[2 * j + 1], amax));
-    if (in) {
-      store_part(codes + m * ldc, c, K, q);
-      if (l == 0) scale[i] = group_scale(amax);
+      for (int j = 0; j < 8; ++j) b = max(b, mag(v[q][j]));
+#pragma unroll
+      for (int o = 8; o > 0; o >>= 1) b = max(b, __shfl_xor_sync(0xffffffffu, b, o));
+      const float amax = group_amax(b);
+      uint16_t w[4];
+      quantize_values<T>(v[q], amax, Divider(amax), w);
+      store_part(codes + static_cast<int64_t>(m[q]) * ldc, c[q], K, w);
+      if (l == 0 && i0 + q * stride < n) scale[i0 + q * stride] = group_scale(amax);
     }
   }
 }
@@ -154,12 +199,12 @@ __global__ void __launch_bounds__(256) fp8_blocks_kernel(const T* __restrict__ x
 #pragma unroll
   for (int j = 0; j < 8; ++j) b = max(b, red[j]);
   const float amax = group_amax(b);
+  const Divider div(amax);
 #pragma unroll
   for (int p = 0; p < 8; ++p) {
     const int64_t m = mb * BLK + p * 16 + (threadIdx.x >> 4);
     uint16_t q[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) q[j] = to_e4m3x2(ratio(v[p][2 * j], amax), ratio(v[p][2 * j + 1], amax));
+    quantize_values<T>(v[p], amax, div, q);
     if (m < M) store_part(codes + m * ldc, c, K, q);
   }
   if (threadIdx.x == 0) scale[blockIdx.x] = group_scale(amax);
@@ -234,12 +279,14 @@ __device__ __forceinline__ void row_codes(const LinArgs& a, int64_t m, bool in, 
   b = max(b, __shfl_xor_sync(0xffffffffu, b, 2));
   const float amax = group_amax(b);
   scale = group_scale(amax);
+  const Divider div(amax);
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
+  for (int i = 0; i < 4; ++i) {
+    uint16_t c[4];
+    quantize_values<T>(v[i], amax, div, c);
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
-      q[2 * i + j] = to_e4m3x2(ratio(v[i][4 * j], amax), ratio(v[i][4 * j + 1], amax)) |
-                     (static_cast<uint32_t>(to_e4m3x2(ratio(v[i][4 * j + 2], amax), ratio(v[i][4 * j + 3], amax))) << 16);
+    for (int j = 0; j < 2; ++j) q[2 * i + j] = c[2 * j] | (static_cast<uint32_t>(c[2 * j + 1]) << 16);
+  }
 }
 template <>
 __device__ __forceinline__ void row_codes<Raw>(const LinArgs& a, int64_t m, bool in, int s, int t, uint32_t (&q)[8], float& scale) {
@@ -257,11 +304,15 @@ __device__ __forceinline__ void row_codes<Raw>(const LinArgs& a, int64_t m, bool
   scale = in ? a.xs[m * a.G + s] : 0.f;
 }
 
-// 16 weight rows per CTA as the rows of mma.sync m16n8k16, 8 rows of x as its columns; the warps
-// split K by 128-groups.  e4m3 is exact in fp16, so the products are exact and sums are fp32.
+// 16 weight rows per CTA as the rows of mma.sync m16n8k16, 8 rows of x as its columns; 16 warps split K by
+// 128-groups and hold the next group's codes while they work on one.  e4m3 is exact in fp16, so the products are exact
+// and sums are fp32.  Rows of x that come as values are quantized by every CTA for itself: 4 KB of them against the 32
+// KB of weights that the CTA reads, and one launch less.
+constexpr int FEW_WARPS = 16;
+
 template <typename T>
-__global__ void __launch_bounds__(256) fp8_few_rows_kernel(const LinArgs a) {
-  __shared__ float red[8][16][9];
+__global__ void __launch_bounds__(FEW_WARPS * 32) fp8_few_rows_kernel(const LinArgs a) {
+  __shared__ float red[FEW_WARPS][16][9];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   pdl_wait();
   const int n0 = blockIdx.x * 16;
@@ -271,14 +322,20 @@ __global__ void __launch_bounds__(256) fp8_few_rows_kernel(const LinArgs a) {
   const uint8_t* pb = a.w + rb * a.ldw + 32 * t;
   const float* ws = a.ws + static_cast<int64_t>(n0 / BLK) * a.G;
   float acc[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int s = warp; s < a.G; s += 8) {
-    uint4 wa[2], wb[2];
+  uint4 wa[2], wb[2];
+  float wsc = 0.f;
+  auto load = [&](int s) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const bool in = s * BLK + 32 * t + 16 * i < a.K;
       wa[i] = in ? load_once(pa + s * BLK + 16 * i) : make_uint4(0, 0, 0, 0);
       wb[i] = in ? load_once(pb + s * BLK + 16 * i) : make_uint4(0, 0, 0, 0);
     }
+    wsc = s < a.G ? __ldg(ws + s) : 0.f;
+  };
+  load(warp);
+#pragma unroll 1
+  for (int s = warp; s < a.G; s += FEW_WARPS) {
     uint32_t q[8];
     float sc;
     row_codes<T>(a, m0 + g < a.M ? m0 + g : 0, m0 + g < a.M, s, t, q, sc);
@@ -296,9 +353,9 @@ __global__ void __launch_bounds__(256) fp8_few_rows_kernel(const LinArgs a) {
       }
     }
     // columns 2t and 2t + 1: rows of x whose scales lanes 8t and 8t + 4 hold
-    const float w = ws[s];
-    const float s0 = __fmul_rn(__shfl_sync(0xffffffffu, sc, 8 * t), w);
-    const float s1 = __fmul_rn(__shfl_sync(0xffffffffu, sc, 8 * t + 4), w);
+    const float s0 = __fmul_rn(__shfl_sync(0xffffffffu, sc, 8 * t), wsc);
+    const float s1 = __fmul_rn(__shfl_sync(0xffffffffu, sc, 8 * t + 4), wsc);
+    load(s + FEW_WARPS);
     acc[0] = __fmaf_rn(s0, d[0], acc[0]);
     acc[1] = __fmaf_rn(s1, d[1], acc[1]);
     acc[2] = __fmaf_rn(s0, d[2], acc[2]);
@@ -313,7 +370,7 @@ __global__ void __launch_bounds__(256) fp8_few_rows_kernel(const LinArgs a) {
     const int r = threadIdx.x & 15, col = threadIdx.x >> 4;
     float v = 0.f;
 #pragma unroll
-    for (int w = 0; w < 8; ++w) v = __fadd_rn(v, red[w][r][col]);
+    for (int w = 0; w < FEW_WARPS; ++w) v = __fadd_rn(v, red[w][r][col]);
     const int n = n0 + r;
     const int64_t m = m0 + col;
     if (n < a.N && m < a.M) {
@@ -329,11 +386,17 @@ int launch_rows(const void* x, int64_t M, int64_t K, int64_t ldx, int block_rows
   const int vec = (reinterpret_cast<uintptr_t>(x) & 15) == 0 && (ldx * sizeof(T)) % 16 == 0;
   const int64_t G = (K + BLK - 1) / BLK;
   if (block_rows == 1) {
-    int64_t blocks = (M * G + 15) / 16;
+    const int64_t n = M * G;
+    int64_t blocks = (n + 31) / 32;
     const int64_t most = static_cast<int64_t>(num_sms()) * 8;
     if (blocks > most) blocks = most;
-    launch_pdl(fp8_rows_kernel<T>, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, st, static_cast<const T*>(x), M, K, ldx,
-               vec, codes, ldc, scale);
+    const dim3 grid(static_cast<unsigned>(blocks));
+    if (n < (1 << 30))
+      launch_pdl(fp8_rows_kernel<T, uint32_t>, grid, dim3(256), 0, st, static_cast<const T*>(x), static_cast<uint32_t>(n),
+                 static_cast<uint32_t>(G), K, ldx, vec, codes, ldc, scale);
+    else
+      launch_pdl(fp8_rows_kernel<T, int64_t>, grid, dim3(256), 0, st, static_cast<const T*>(x), n, G, K, ldx, vec, codes, ldc,
+                 scale);
     return check_launch("fp8_rows_kernel");
   }
   launch_pdl(fp8_blocks_kernel<T>, dim3(static_cast<unsigned>((M + BLK - 1) / BLK * G)), dim3(256), 0, st,
@@ -431,10 +494,10 @@ int fp8_linear(const void* x, int x_dtype, const float* x_scale, int64_t M, int 
   a.G = G;
   const dim3 grid((N + 15) / 16, static_cast<unsigned>((M + 7) / 8));
   switch (x_dtype) {
-    case LLQ_E4M3: launch_pdl(fp8_few_rows_kernel<Raw>, grid, dim3(256), 0, st, a); break;
-    case LLQ_F32: launch_pdl(fp8_few_rows_kernel<float>, grid, dim3(256), 0, st, a); break;
-    case LLQ_F16: launch_pdl(fp8_few_rows_kernel<__half>, grid, dim3(256), 0, st, a); break;
-    default: launch_pdl(fp8_few_rows_kernel<__nv_bfloat16>, grid, dim3(256), 0, st, a); break;
+    case LLQ_E4M3: launch_pdl(fp8_few_rows_kernel<Raw>, grid, dim3(FEW_WARPS * 32), 0, st, a); break;
+    case LLQ_F32: launch_pdl(fp8_few_rows_kernel<float>, grid, dim3(FEW_WARPS * 32), 0, st, a); break;
+    case LLQ_F16: launch_pdl(fp8_few_rows_kernel<__half>, grid, dim3(FEW_WARPS * 32), 0, st, a); break;
+    default: launch_pdl(fp8_few_rows_kernel<__nv_bfloat16>, grid, dim3(FEW_WARPS * 32), 0, st, a); break;
   }
   return check_launch("fp8_few_rows_kernel");
 }

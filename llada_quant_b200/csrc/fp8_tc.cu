@@ -11,7 +11,11 @@
 // A tile is 128 rows (TMEM lanes, so a row's scale is one number per thread) by BN weight rows.
 //   warp 0      TMA producer: per block the 128 x 128 and BN x 128 byte boxes (128-byte swizzle)
 //   warp 1      TMEM allocator and MMA issuer (one elected lane)
-//   warps 2-9   epilogue: one TMEM lane quarter each, half of the columns; BN / 2 sums per thread
+//   warps 2, 3  idle: they fill the warpgroup whose registers the epilogue takes over
+//   warps 4-11  epilogue: one TMEM lane quarter each, half of the columns; BN / 2 sums per thread
+// What bounds a large product is this epilogue: 128 x BN sums per 128 of K leave TMEM and pass the FMA pipe (as
+// pairs, fma.rn.f32x2) while the tensor core needs 512 cycles for 128 x 256 x 128.  So a thread asks for its next 32
+// columns before it adds the last, which takes 216 registers at BN = 256.
 // Persistent over tiles when K is not split.  When the tiles do not cover the SMs, a cluster of `split`
 // CTAs shares one tile, each takes a part of K, and the parts meet in distributed shared memory and are
 // added in rank order.
@@ -38,7 +42,8 @@ struct F8Cfg {
   static constexpr int TMEM_COLS = ACC_BUFS * BN;
   static constexpr int EPI_WARPS = 8;
   static constexpr int COLS = BN / 2;  // columns of an epilogue thread
-  static constexpr int THREADS = (2 + EPI_WARPS) * 32;
+  static constexpr int FIRST_EPI = 4;
+  static constexpr int THREADS = (FIRST_EPI + EPI_WARPS) * 32;
   static constexpr int OUT_BYTES = EPI_WARPS * 4096;  // per warp 32 rows of 128 bytes
   static constexpr size_t SMEM_BYTES = 1024 + static_cast<size_t>(STAGES) * STAGE_BYTES + OUT_BYTES + 512;
   static_assert(128 * BN * 4 <= STAGES * STAGE_BYTES, "the parts of a split tile reuse the stages");
@@ -84,6 +89,18 @@ __device__ __forceinline__ void tc_ld32(uint32_t taddr, uint32_t (&r)[32]) {
         "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
       : "r"(taddr)
       : "memory");
+}
+
+// the loads into v are complete (v is an operand, so that nothing that uses it moves up)
+__device__ __forceinline__ void tc_wait_ld32(uint32_t (&r)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]),
+                 "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]),
+                 "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]),
+                 "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29])
+               :
+               : "memory");
+  asm volatile("" : "+r"(r[30]), "+r"(r[31]));
 }
 
 // two sums at once: acc = v * s + acc
@@ -164,6 +181,12 @@ __global__ void __launch_bounds__(F8Cfg<BN>::THREADS, 1)
   // the codes may come from generic stores of the kernel before
   asm volatile("fence.proxy.async.global;" ::: "memory");
 
+  // the epilogue's threads take over the others' registers: 128 x 64 + 256 x 216 of the block's 384 x 168
+  if (BN == 256) {
+    if (warp < C::FIRST_EPI) asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+    else asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+  }
+
   const int rank = blockIdx.x % a.split;
   const int stride = gridDim.x / a.split;
   const int g0 = static_cast<int>(static_cast<int64_t>(a.G) * rank / a.split);
@@ -224,11 +247,11 @@ __global__ void __launch_bounds__(F8Cfg<BN>::THREADS, 1)
         }
       }
     }
-  } else {
-    const int half = (warp - 2) >> 2;
+  } else if (warp >= C::FIRST_EPI) {
+    const int half = (warp - C::FIRST_EPI) >> 2;
     const int q = warp & 3;  // the TMEM lanes a warp may read
     const uint32_t lane_addr = tmem + (static_cast<uint32_t>(q * 32) << 16) + half * C::COLS;
-    uint8_t* stage = so + (warp - 2) * 4096;
+    uint8_t* stage = so + (warp - C::FIRST_EPI) * 4096;
     int ab = 0;
     uint32_t aph = 0;
     bool ok = true;
@@ -252,17 +275,23 @@ __global__ void __launch_bounds__(F8Cfg<BN>::THREADS, 1)
         }
         if (!mbar_wait(&acc_full[ab], aph, abort_flag, 0x530 + ab)) { ok = false; break; }
         tc_fence_after();
+        constexpr int CH = C::COLS / 32;
+        const uint32_t at = lane_addr + ab * BN;
+        uint32_t v[CH > 1 ? 2 : 1][32];
+        tc_ld32(at, v[0]);
 #pragma unroll
-        for (int c = 0; c < C::COLS / 32; ++c) {
-          uint32_t v[32];
-          tc_ld32(lane_addr + ab * BN + c * 32, v);
-          tc_wait_ld();
+        for (int c = 0; c < CH; ++c) {
+          tc_wait_ld32(v[c & 1]);
+          if (c + 1 < CH) {
+            tc_ld32(at + (c + 1) * 32, v[(c + 1) & 1]);
+          } else {  // all is read: the buffer goes back before the last sums
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&acc_empty[ab]);
+          }
 #pragma unroll
-          for (int i = 0; i < 16; ++i) fma2(acc[c * 16 + i], v[2 * i], v[2 * i + 1], s2);
+          for (int i = 0; i < 16; ++i) fma2(acc[c * 16 + i], v[c & 1][2 * i], v[c & 1][2 * i + 1], s2);
         }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&acc_empty[ab]);
         if (++ab == C::ACC_BUFS) {
           ab = 0;
           aph ^= 1;
@@ -426,8 +455,24 @@ int fp8_gemm_tc(const Fp8Operands& p, cudaStream_t st) {
   const int64_t mt = (p.M + BM - 1) / BM;
   const int sms = num_sms();
   auto tiles = [&](int bn) { return mt * ((p.N + bn - 1) / bn); };
-  int bn = 256;
-  if (tiles(256) < sms) bn = tiles(128) < sms ? 64 : 128;
+  // Tile width and K split by the bytes that the busiest SM brings from L2: waves x blocks of K x (128 + BN) rows of 128
+  // bytes; a split costs about 1 us more, that is 1000 such rows, and its clusters must fit at once (148 SMs hold 132
+  // CTAs in clusters of four, 120 in clusters of eight).  Measured at 256 x 8192 x 2048: 128 wide in one wave 9.9 us,
+  // 64 wide in two 14.4.
+  int bn = 64, split = 1;
+  int64_t best = INT64_MAX;
+  for (int w : {256, 128, 64}) {
+    for (int sp : {1, 2, 4, 8}) {
+      const int room = sp == 8 ? sms * 120 / 148 : sp == 4 ? sms * 132 / 148 : sms;
+      if (sp > 1 && (tiles(w) * sp > room || sp * 2 > p.G || w == 256)) break;
+      const int64_t cost = (tiles(w) + sms - 1) / sms * ((p.G + sp - 1) / sp) * (BM + w) + (sp > 1 ? 1000 : 0);
+      if (cost < best) {
+        best = cost;
+        bn = w;
+        split = sp;
+      }
+    }
+  }
   F8Args a{};
   a.xs = p.xs;
   a.ws = p.ws;
@@ -439,9 +484,7 @@ int fp8_gemm_tc(const Fp8Operands& p, cudaStream_t st) {
   if (tiles(bn) > 0x7fffffff) return fail(LLQ_EINVAL, "too many tiles");
   a.mtiles = static_cast<int>(mt);
   a.tiles = static_cast<int>(tiles(bn));
-  a.split = 1;
-  if (bn == 64)
-    while (a.split < 8 && a.tiles * a.split * 2 <= sms && a.split * 4 <= a.G) a.split *= 2;
+  a.split = split;
   return bn == 256 ? launch_out<256>(p, a, st) : bn == 128 ? launch_out<128>(p, a, st) : launch_out<64>(p, a, st);
 }
 
