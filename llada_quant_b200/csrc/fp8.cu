@@ -1,5 +1,7 @@
 // 8-bit floating point (e4m3) with one fp32 scale per 128 values of a row, or per 128 x 128 block:
 // the quantizer and the product of e4m3 rows with an e4m3 weight.
+#include <type_traits>
+
 #include <cuda_fp8.h>
 
 #include "fp8.cuh"
@@ -137,41 +139,82 @@ __device__ __forceinline__ void store_part(uint8_t* row, int64_t c, int64_t K, c
   }
 }
 
-// One scale per 128 values of a row: 16 lanes hold a group, 8 values each, and two groups at a time, both asked for
-// before either is used.  I: 32-bit indices of groups where they fit (a 64-bit division per group took as long as all
-// the rest).
+// 16 values c .. c + 15 of a row of K (zero beyond), and the largest magnitude's bits among them as fp32
+template <typename T>
+__device__ __forceinline__ void load16(const T* row, int64_t c, int64_t K, bool vec, float (&v)[16], uint32_t& m) {
+  if (vec && c + 16 <= K) {
+    if (sizeof(T) == 2) {
+      const uint4 a = __ldg(reinterpret_cast<const uint4*>(row + c)), b = __ldg(reinterpret_cast<const uint4*>(row + c) + 1);
+      const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+      uint32_t top = 0;  // of both halves: their patterns order as magnitudes
+#pragma unroll
+      for (int i = 0; i < 8; ++i) top = __vmaxu2(top, w[i] & 0x7fff7fffu);
+      const uint16_t t16 = static_cast<uint16_t>(max(top >> 16, top & 0xffffu));
+      m = std::is_same<T, __half>::value ? __float_as_uint(__half2float(__ushort_as_half(t16)))
+                                         : static_cast<uint32_t>(t16) << 16;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if (std::is_same<T, __half>::value) {
+          const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+          v[2 * i] = f.x;
+          v[2 * i + 1] = f.y;
+        } else {
+          v[2 * i] = __uint_as_float(w[i] << 16);
+          v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+        }
+      }
+      return;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float4 a = __ldg(reinterpret_cast<const float4*>(row + c) + i);
+      v[4 * i] = a.x;
+      v[4 * i + 1] = a.y;
+      v[4 * i + 2] = a.z;
+      v[4 * i + 3] = a.w;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = c + i < K ? to_f32(row[c + i]) : 0.f;
+  }
+  m = 0;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) m = max(m, mag(v[i]));
+}
+
+// One scale per 128 values of a row: 8 lanes hold a group, 16 values each.  I: 32-bit indices of groups where they fit
+// (a 64-bit division per group took as long as all the rest).
 template <typename T, typename I>
 __global__ void __launch_bounds__(256) fp8_rows_kernel(const T* __restrict__ x, I n, I G, int64_t K, int64_t ldx, int vec,
                                                        uint8_t* __restrict__ codes, int64_t ldc, float* __restrict__ scale) {
   pdl_wait();
-  const int l = threadIdx.x & 15;
-  const I stride = static_cast<I>(gridDim.x) * (blockDim.x >> 4);
-  const I first = static_cast<I>(blockIdx.x) * (blockDim.x >> 4) + (threadIdx.x >> 4);
+  const int l = threadIdx.x & 7;
+  const I stride = static_cast<I>(gridDim.x) * (blockDim.x >> 3);
 #pragma unroll 1
-  for (I i0 = first; i0 - (threadIdx.x >> 4 & 1) < n; i0 += 2 * stride) {  // a warp's lanes leave the loop together
-    float v[2][8];
-    I m[2];
-    int64_t c[2];
+  for (I i = static_cast<I>(blockIdx.x) * (blockDim.x >> 3) + (threadIdx.x >> 3); i - (threadIdx.x >> 3 & 3) < n; i += stride) {
+    const bool in = i < n;  // a warp's four groups leave the loop together
+    const I m = in ? i / G : 0;
+    const int64_t c = in ? static_cast<int64_t>(i - m * G) * BLK + 16 * l : K;
+    float v[16];
+    uint32_t b;
+    load16(x + static_cast<int64_t>(m) * ldx, c, K, vec != 0, v, b);
 #pragma unroll
-    for (int q = 0; q < 2; ++q) {
-      const I i = i0 + q * stride;
-      m[q] = i < n ? i / G : 0;
-      c[q] = i < n ? static_cast<int64_t>(i - m[q] * G) * BLK + 8 * l : K;
-      load_part(x + static_cast<int64_t>(m[q]) * ldx, c[q], K, vec != 0, v[q]);
+    for (int o = 4; o > 0; o >>= 1) b = max(b, __shfl_xor_sync(0xffffffffu, b, o));
+    const float amax = group_amax(b);
+    uint16_t q[8];
+    quantize_values<T>(v, amax, Divider(amax), q);
+    uint8_t* to = codes + static_cast<int64_t>(m) * ldc;
+    if (c + 16 <= K) {
+      uint32_t w[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) w[j] = q[2 * j] | (static_cast<uint32_t>(q[2 * j + 1]) << 16);
+      *reinterpret_cast<uint4*>(to + c) = make_uint4(w[0], w[1], w[2], w[3]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 16; ++j)
+        if (c + j < K) to[c + j] = static_cast<uint8_t>(q[j >> 1] >> (8 * (j & 1)));
     }
-#pragma unroll
-    for (int q = 0; q < 2; ++q) {
-      uint32_t b = 0;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) b = max(b, mag(v[q][j]));
-#pragma unroll
-      for (int o = 8; o > 0; o >>= 1) b = max(b, __shfl_xor_sync(0xffffffffu, b, o));
-      const float amax = group_amax(b);
-      uint16_t w[4];
-      quantize_values<T>(v[q], amax, Divider(amax), w);
-      store_part(codes + static_cast<int64_t>(m[q]) * ldc, c[q], K, w);
-      if (l == 0 && i0 + q * stride < n) scale[i0 + q * stride] = group_scale(amax);
-    }
+    if (l == 0 && in) scale[i] = group_scale(amax);
   }
 }
 

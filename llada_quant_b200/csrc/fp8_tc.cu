@@ -13,9 +13,9 @@
 //   warp 1      TMEM allocator and MMA issuer (one elected lane)
 //   warps 2, 3  idle: they fill the warpgroup whose registers the epilogue takes over
 //   warps 4-11  epilogue: one TMEM lane quarter each, half of the columns; BN / 2 sums per thread
-// What bounds a large product is this epilogue: 128 x BN sums per 128 of K leave TMEM and pass the FMA pipe (as
-// pairs, fma.rn.f32x2) while the tensor core needs 512 cycles for 128 x 256 x 128.  So a thread asks for its next 32
-// columns before it adds the last, which takes 216 registers at BN = 256.
+// What bounds a large product is this epilogue: 128 x BN sums per 128 of K leave TMEM and pass the FMA pipe (256
+// cycles at BN = 256; as fma.rn.f32x2 it took three instructions a pair) while the tensor core needs 512 cycles for
+// 128 x 256 x 128.  So a thread asks for its next 32 columns before it adds the last, which takes 216 registers at BN = 256.
 // Persistent over tiles when K is not split.  When the tiles do not cover the SMs, a cluster of `split`
 // CTAs shares one tile, each takes a part of K, and the parts meet in distributed shared memory and are
 // added in rank order.
@@ -101,11 +101,6 @@ __device__ __forceinline__ void tc_wait_ld32(uint32_t (&r)[32]) {
                :
                : "memory");
   asm volatile("" : "+r"(r[30]), "+r"(r[31]));
-}
-
-// two sums at once: acc = v * s + acc
-__device__ __forceinline__ void fma2(uint64_t& acc, uint32_t lo, uint32_t hi, uint64_t s) {
-  asm("{\n\t.reg .b64 v;\n\tmov.b64 v, {%1, %2};\n\tfma.rn.f32x2 %0, v, %3, %0;\n\t}" : "+l"(acc) : "r"(lo), "r"(hi), "l"(s));
 }
 
 __device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, const void* src, int x, int y) {
@@ -261,14 +256,12 @@ __global__ void __launch_bounds__(F8Cfg<BN>::THREADS, 1)
       const bool in = row < a.M;
       const float* xs = a.xs + (in ? row : 0) * a.G;
       const float* ws = a.ws + static_cast<int64_t>(min(n0, a.N - 1) / 128) * a.G;
-      uint64_t acc[C::COLS / 2];
+      float acc[C::COLS];
 #pragma unroll
-      for (int i = 0; i < C::COLS / 2; ++i) acc[i] = 0;
+      for (int i = 0; i < C::COLS; ++i) acc[i] = 0.f;
       float sx = in && g0 < g1 ? __ldg(xs + g0) : 0.f, sw = g0 < g1 ? __ldg(ws + g0) : 0.f;
       for (int g = g0; g < g1; ++g) {
         const float s = __fmul_rn(sx, sw);
-        uint64_t s2;
-        asm("mov.b64 %0, {%1, %1};" : "=l"(s2) : "f"(s));
         if (g + 1 < g1) {  // the next block's scales ahead of the wait
           sx = in ? __ldg(xs + g + 1) : 0.f;
           sw = __ldg(ws + g + 1);
@@ -290,7 +283,7 @@ __global__ void __launch_bounds__(F8Cfg<BN>::THREADS, 1)
             if (lane == 0) mbar_arrive(&acc_empty[ab]);
           }
 #pragma unroll
-          for (int i = 0; i < 16; ++i) fma2(acc[c * 16 + i], v[c & 1][2 * i], v[c & 1][2 * i + 1], s2);
+          for (int i = 0; i < 32; ++i) acc[c * 32 + i] = __fmaf_rn(__uint_as_float(v[c & 1][i]), s, acc[c * 32 + i]);
         }
         if (++ab == C::ACC_BUFS) {
           ab = 0;
@@ -301,10 +294,7 @@ __global__ void __launch_bounds__(F8Cfg<BN>::THREADS, 1)
       if (a.split > 1) {  // this CTA's part of the tile, column by column, over the drained stages
         float* part = reinterpret_cast<float*>(smem) + (half * C::COLS) * BM + q * 32 + lane;
 #pragma unroll
-        for (int i = 0; i < C::COLS / 2; ++i) {
-          part[(2 * i) * BM] = __uint_as_float(static_cast<uint32_t>(acc[i]));
-          part[(2 * i + 1) * BM] = __uint_as_float(static_cast<uint32_t>(acc[i] >> 32));
-        }
+        for (int i = 0; i < C::COLS; ++i) part[i * BM] = acc[i];
         break;
       }
       // 128 bytes of every row at a time through this warp's shared memory
@@ -320,11 +310,7 @@ __global__ void __launch_bounds__(F8Cfg<BN>::THREADS, 1)
         for (int j = 0; j < CC / PER; ++j) {
           float v[PER];
 #pragma unroll
-          for (int i = 0; i < PER; i += 2) {
-            const uint64_t p = acc[(c * CC + j * PER + i) / 2];
-            v[i] = __uint_as_float(static_cast<uint32_t>(p));
-            v[i + 1] = __uint_as_float(static_cast<uint32_t>(p >> 32));
-          }
+          for (int i = 0; i < PER; ++i) v[i] = acc[c * CC + j * PER + i];
           if (a.bias != nullptr) {
 #pragma unroll
             for (int i = 0; i < PER; ++i)
