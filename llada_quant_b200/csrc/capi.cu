@@ -375,6 +375,7 @@ int llq_fp8_linear(const void* x, int x_dtype, const float* x_scale, int64_t M, 
 int llq_device_error(int32_t* code) {
   if (code == nullptr) return fail(LLQ_EINVAL, "null code pointer");
   cudaError_t e = cudaMemcpyFromSymbol(code, g_device_error, sizeof(int32_t));
+  if (e == cudaSuccess && *code == 0) e = fp8_tc_error(code);
   if (e != cudaSuccess) return fail(LLQ_ECUDA, "reading the device error word: %s", cudaGetErrorString(e));
   return LLQ_OK;
 }
@@ -382,6 +383,7 @@ int llq_device_error(int32_t* code) {
 int llq_clear_device_error(void) {
   const int32_t zero = 0;
   cudaError_t e = cudaMemcpyToSymbol(g_device_error, &zero, sizeof(int32_t));
+  if (e == cudaSuccess) e = fp8_tc_clear_error();
   if (e != cudaSuccess) return fail(LLQ_ECUDA, "clearing the device error word: %s", cudaGetErrorString(e));
   return LLQ_OK;
 }

@@ -19,6 +19,10 @@
 // Persistent over tiles when K is not split.  When the tiles do not cover the SMs, a cluster of `split`
 // CTAs shares one tile, each takes a part of K, and the parts meet in distributed shared memory and are
 // added in rank order.
+//
+// This file is compiled without relocatable device code (build.py), which setmaxnreg needs; so it has an error word of
+// its own.
+#define LLQ_OWN_ERROR_WORD
 #include <cooperative_groups.h>
 
 #include "fp8.cuh"
@@ -37,7 +41,6 @@ template <int BN>
 struct F8Cfg {
   static constexpr int A_BYTES = BM * BK;
   static constexpr int STAGE_BYTES = A_BYTES + BN * BK;
-  static constexpr int STAGES = 196608 / STAGE_BYTES;
   static constexpr int ACC_BUFS = BN == 256 ? 2 : 4;
   static constexpr int TMEM_COLS = ACC_BUFS * BN;
   static constexpr int EPI_WARPS = 8;
@@ -45,6 +48,7 @@ struct F8Cfg {
   static constexpr int FIRST_EPI = 4;
   static constexpr int THREADS = (FIRST_EPI + EPI_WARPS) * 32;
   static constexpr int OUT_BYTES = EPI_WARPS * 4096;  // per warp 32 rows of 128 bytes
+  static constexpr int STAGES = (232448 - 1024 - 512 - OUT_BYTES) / STAGE_BYTES;
   static constexpr size_t SMEM_BYTES = 1024 + static_cast<size_t>(STAGES) * STAGE_BYTES + OUT_BYTES + 512;
   static_assert(128 * BN * 4 <= STAGES * STAGE_BYTES, "the parts of a split tile reuse the stages");
   static_assert(SMEM_BYTES <= 232448, "shared memory");
@@ -176,17 +180,15 @@ __global__ void __launch_bounds__(F8Cfg<BN>::THREADS, 1)
   // the codes may come from generic stores of the kernel before
   asm volatile("fence.proxy.async.global;" ::: "memory");
 
-  // the epilogue's threads take over the others' registers: 128 x 64 + 256 x 216 of the block's 384 x 168
-  if (BN == 256) {
-    if (warp < C::FIRST_EPI) asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
-    else asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
-  }
-
   const int rank = blockIdx.x % a.split;
   const int stride = gridDim.x / a.split;
   const int g0 = static_cast<int>(static_cast<int64_t>(a.G) * rank / a.split);
   const int g1 = static_cast<int>(static_cast<int64_t>(a.G) * (rank + 1) / a.split);
 
+  // the epilogue's threads take over the others' registers: 128 x 64 + 256 x 216 of the block's 384 x 168
+  if (warp < C::FIRST_EPI) {
+    if (BN == 256) asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+  }
   if (warp == 0) {
     if (lane == 0) {
       int issued = 0, rs = 0;
@@ -243,15 +245,16 @@ __global__ void __launch_bounds__(F8Cfg<BN>::THREADS, 1)
       }
     }
   } else if (warp >= C::FIRST_EPI) {
-    const int half = (warp - C::FIRST_EPI) >> 2;
+    if (BN == 256) asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+    const int part_of = (warp - C::FIRST_EPI) >> 2;  // this warp's columns
     const int q = warp & 3;  // the TMEM lanes a warp may read
-    const uint32_t lane_addr = tmem + (static_cast<uint32_t>(q * 32) << 16) + half * C::COLS;
+    const uint32_t lane_addr = tmem + (static_cast<uint32_t>(q * 32) << 16) + part_of * C::COLS;
     uint8_t* stage = so + (warp - C::FIRST_EPI) * 4096;
     int ab = 0;
     uint32_t aph = 0;
     bool ok = true;
     for (int u = blockIdx.x / a.split; u < a.tiles && ok; u += stride) {
-      const int m0 = u % a.mtiles * BM, n0 = u / a.mtiles * BN + half * C::COLS;
+      const int m0 = u % a.mtiles * BM, n0 = u / a.mtiles * BN + part_of * C::COLS;
       const int64_t row = static_cast<int64_t>(m0) + q * 32 + lane;
       const bool in = row < a.M;
       const float* xs = a.xs + (in ? row : 0) * a.G;
@@ -292,7 +295,7 @@ __global__ void __launch_bounds__(F8Cfg<BN>::THREADS, 1)
       }
       if (!ok) break;
       if (a.split > 1) {  // this CTA's part of the tile, column by column, over the drained stages
-        float* part = reinterpret_cast<float*>(smem) + (half * C::COLS) * BM + q * 32 + lane;
+        float* part = reinterpret_cast<float*>(smem) + (part_of * C::COLS) * BM + q * 32 + lane;
 #pragma unroll
         for (int i = 0; i < C::COLS; ++i) part[i * BM] = acc[i];
         break;
@@ -436,6 +439,13 @@ int launch_out(const Fp8Operands& p, const F8Args& a, cudaStream_t st) {
 }
 
 }  // namespace
+
+cudaError_t fp8_tc_error(int32_t* code) { return cudaMemcpyFromSymbol(code, g_device_error, sizeof(int32_t)); }
+
+cudaError_t fp8_tc_clear_error() {
+  const int32_t zero = 0;
+  return cudaMemcpyToSymbol(g_device_error, &zero, sizeof(int32_t));
+}
 
 int fp8_gemm_tc(const Fp8Operands& p, cudaStream_t st) {
   const int64_t mt = (p.M + BM - 1) / BM;

@@ -105,8 +105,13 @@ cudaError_t launch_pdl(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t s
   return launch_pdl_ex(false, kernel, grid, block, smem, st, std::forward<Args>(args)...);
 }
 
-// device error word (bounded waits record where they gave up)
+// device error word (bounded waits record where they gave up); a source that is compiled
+// without relocatable device code keeps its own
+#ifdef LLQ_OWN_ERROR_WORD
+static __device__ int32_t g_device_error = 0;
+#else
 extern __device__ int32_t g_device_error;
+#endif
 
 // ---------------------------------------------------------------------------
 // element helpers

@@ -56,6 +56,9 @@ int moe_few(const llq_few_layer& L, const void* x, int64_t T, float* logits, flo
             void* out, void* workspace, size_t bytes, cudaStream_t st);
 int fp8_quantize(const void* x, int x_dtype, int64_t M, int64_t K, int64_t ldx, int block_rows, uint8_t* codes,
                  int64_t ldc, float* scale, cudaStream_t st);
+// the error word of the e4m3 product's tensor-core kernel
+cudaError_t fp8_tc_error(int32_t* code);
+cudaError_t fp8_tc_clear_error();
 size_t fp8_linear_workspace(int64_t M, int K, int N, int x_dtype);
 int fp8_linear(const void* x, int x_dtype, const float* x_scale, int64_t M, int K, int64_t ldx, const uint8_t* w,
                const float* w_scale, int N, int64_t ldw, const void* bias, void* out, int out_dtype, void* workspace,
