@@ -22,7 +22,7 @@ from . import ops
 BLOCK = ops.FP8_BLOCK
 
 
-@dataclass(frozen=True)
+@dataclass(slots=True)
 class Fp8Tensor:
     """e4m3 ``codes [M, K]`` and fp32 ``scale [ceil(M / block_rows), ceil(K / 128)]``: value = code * scale."""
 

@@ -749,7 +749,7 @@ def fp8_operand(codes: torch.Tensor, what: str) -> torch.Tensor:
 class Fp8Weight:
     """A checked e4m3 weight [N, K] with its scales and bias, ready to multiply."""
 
-    __slots__ = ("codes", "scale", "bias", "N", "K", "G", "ldw", "device", "dtype", "_out", "_w", "_s", "_b")
+    __slots__ = ("codes", "scale", "bias", "N", "K", "G", "ldw", "device", "dtype", "_out", "_w", "_s", "_b", "_need")
 
     def __init__(self, codes: torch.Tensor, scale: torch.Tensor, bias: Optional[torch.Tensor],
                  out_dtype: torch.dtype) -> None:
@@ -773,6 +773,7 @@ class Fp8Weight:
             raise ValueError("the product's operands lie on several devices")
         self.ldw = codes.stride(0) if self.N > 1 else fp8_pitch(self.K)
         self._w, self._s, self._b = codes.data_ptr(), self.scale.data_ptr(), _ptr(bias)
+        self._need = {}  # workspace bytes by (rows, kind)
 
     def multiply(self, x: torch.Tensor, x_scale: Optional[torch.Tensor] = None) -> torch.Tensor:
         """x fp32/fp16/bf16 values [M, K], or e4m3 codes with ``x_scale [M, G]`` -> [M, N]."""
@@ -806,7 +807,11 @@ class Fp8Weight:
         out = torch.empty(M, self.N, dtype=self.dtype, device=self.device)
         ws, need = None, 0
         if x_scale is None:
-            need = lib.llq_fp8_linear_workspace_size(M, self.K, self.N, kind)
+            need = self._need.get((M, kind))
+            if need is None:
+                if len(self._need) > 4096:
+                    self._need.clear()
+                need = self._need[M, kind] = lib.llq_fp8_linear_workspace_size(M, self.K, self.N, kind)
             if need:  # the quantized rows, of this call alone
                 ws = torch.empty(need, dtype=torch.uint8, device=self.device)
         rc = lib.llq_fp8_linear(x.data_ptr(), kind, None if x_scale is None else x_scale.data_ptr(), M, self.K,
