@@ -12,8 +12,7 @@ namespace llq {
 namespace {
 
 constexpr int BLK = 128;
-// up to this many rows the product runs on fp8_few_rows_kernel, above on fp8_tc_kernel
-constexpr int64_t kFewRows = 16;
+constexpr int64_t kOwnK = 16384;  // longest rows that fp8_few_rows_kernel quantizes (it holds 8 in shared memory)
 // groups whose largest magnitude lies below 448 * 2^-60 are scaled as if it were this, so that the
 // product of two scales stays a normal fp32 number
 constexpr float kAmaxFloor = 448.f * 0x1p-60f;
@@ -59,7 +58,8 @@ __device__ __forceinline__ uint16_t to_e4m3x2(float lo, float hi) {
 }
 
 // The codes of N values of type T of a group: e4m3 of ratio(v).  (A division for each value took 42 us at 8192 x 4096
-// bf16, and a test for borders with the division behind it 50: a quarter of all groups of bf16 values has some on one.)
+// bf16 where this took 28, and a test for borders with the division behind it 50: a quarter of all groups of bf16 values
+// has some on one.)
 template <typename T, int N>
 __device__ __forceinline__ void quantize_values(const float (&v)[N], float amax, const Divider& div, uint16_t (&q)[N / 2]) {
   uint32_t differ = 0;
@@ -85,157 +85,152 @@ __device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint16_t c) {
   return r;
 }
 
-// 8 consecutive values as fp32
-template <typename T>
-__device__ __forceinline__ void load8(const T* p, float (&v)[8]);
-template <>
-__device__ __forceinline__ void load8<float>(const float* p, float (&v)[8]) {
-  const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
-  v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-  v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-}
-template <>
-__device__ __forceinline__ void load8<__nv_bfloat16>(const __nv_bfloat16* p, float (&v)[8]) {
-  const uint4 a = __ldg(reinterpret_cast<const uint4*>(p));
-  const uint32_t w[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    v[2 * i] = __uint_as_float(w[i] << 16);
-    v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-  }
-}
-template <>
-__device__ __forceinline__ void load8<__half>(const __half* p, float (&v)[8]) {
-  const uint4 a = __ldg(reinterpret_cast<const uint4*>(p));
-  const uint32_t w[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-    v[2 * i] = f.x;
-    v[2 * i + 1] = f.y;
-  }
-}
-
-// values c .. c + 7 of a row of K, zero beyond; `vec`: the row may be read in 16-byte pieces
-template <typename T>
-__device__ __forceinline__ void load_part(const T* row, int64_t c, int64_t K, bool vec, float (&v)[8]) {
-  if (vec && c + 8 <= K) {
-    load8(row + c, v);
+// the codes of values c .. c + 15 into a row whose pitch is a multiple of 16 bytes; nothing beyond K is written
+__device__ __forceinline__ void store16(uint8_t* row, int64_t c, int64_t K, const uint32_t (&w)[4]) {
+  if (c + 16 <= K) {
+    *reinterpret_cast<uint4*>(row + c) = make_uint4(w[0], w[1], w[2], w[3]);
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = c + i < K ? to_f32(row[c + i]) : 0.f;
+    for (int j = 0; j < 16; ++j)
+      if (c + j < K) row[c + j] = static_cast<uint8_t>(w[j >> 2] >> (8 * (j & 3)));
   }
 }
 
-// the codes of values c .. c + 7 into a row whose pitch is a multiple of 16 bytes; nothing beyond K is written
-__device__ __forceinline__ void store_part(uint8_t* row, int64_t c, int64_t K, const uint16_t (&q)[4]) {
-  if (c + 8 <= K) {
-    *reinterpret_cast<uint2*>(row + c) = make_uint2(q[0] | (static_cast<uint32_t>(q[1]) << 16),
-                                                    q[2] | (static_cast<uint32_t>(q[3]) << 16));
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (c + i < K) row[c + i] = static_cast<uint8_t>(q[i >> 1] >> (8 * (i & 1)));
-  }
-}
-
-// 16 values c .. c + 15 of a row of K (zero beyond), and the largest magnitude's bits among them as fp32
+// 16 values of a row as they lie in memory: they stay so until their codes are made, which halves the registers
 template <typename T>
-__device__ __forceinline__ void load16(const T* row, int64_t c, int64_t K, bool vec, float (&v)[16], uint32_t& m) {
-  if (vec && c + 16 <= K) {
-    if (sizeof(T) == 2) {
-      const uint4 a = __ldg(reinterpret_cast<const uint4*>(row + c)), b = __ldg(reinterpret_cast<const uint4*>(row + c) + 1);
-      const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-      uint32_t top = 0;  // of both halves: their patterns order as magnitudes
+struct Raw16 {
+  uint32_t w[4 * sizeof(T)];
+
+  // values c .. c + 15 of a row of K, zero beyond
+  __device__ __forceinline__ void load(const T* row, int64_t c, int64_t K, bool vec) {
+    constexpr int N = sizeof(T);  // 16-byte pieces
+    if (vec && c + 16 <= K) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) top = __vmaxu2(top, w[i] & 0x7fff7fffu);
-      const uint16_t t16 = static_cast<uint16_t>(max(top >> 16, top & 0xffffu));
-      m = std::is_same<T, __half>::value ? __float_as_uint(__half2float(__ushort_as_half(t16)))
-                                         : static_cast<uint32_t>(t16) << 16;
+      for (int i = 0; i < N; ++i) {
+        const uint4 a = __ldg(reinterpret_cast<const uint4*>(row + c) + i);
+        w[4 * i] = a.x;
+        w[4 * i + 1] = a.y;
+        w[4 * i + 2] = a.z;
+        w[4 * i + 3] = a.w;
+      }
+    } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
+      for (int i = 0; i < 4 * N; ++i) {
+        if (sizeof(T) == 4) {
+          w[i] = c + i < K ? reinterpret_cast<const uint32_t*>(row)[c + i] : 0u;
+        } else {
+          const uint16_t* h = reinterpret_cast<const uint16_t*>(row);
+          w[i] = (c + 2 * i < K ? h[c + 2 * i] : 0u) | (c + 2 * i + 1 < K ? static_cast<uint32_t>(h[c + 2 * i + 1]) << 16 : 0u);
+        }
+      }
+    }
+  }
+
+  // the largest magnitude's bits as fp32
+  __device__ __forceinline__ uint32_t top() const {
+    uint32_t m = 0;
+    if (sizeof(T) == 4) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) m = max(m, w[i] & 0x7fffffffu);
+      return m;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = __vmaxu2(m, w[i] & 0x7fff7fffu);  // halves order as magnitudes too
+    const uint32_t t = max(m >> 16, m & 0xffffu);
+    return std::is_same<T, __half>::value ? __float_as_uint(__half2float(__ushort_as_half(static_cast<uint16_t>(t)))) : t << 16;
+  }
+
+  // the codes under a group's largest magnitude
+  __device__ __forceinline__ void codes(float amax, const Divider& div, uint32_t (&c)[4]) const {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      float v[4];
+      uint16_t q[2];
+      four(j, v);
+      quantize_values<T>(v, amax, div, q);
+      c[j] = q[0] | (static_cast<uint32_t>(q[1]) << 16);
+    }
+  }
+
+  // values 4 j .. 4 j + 3
+  __device__ __forceinline__ void four(int j, float (&v)[4]) const {
+    if (sizeof(T) == 4) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = __uint_as_float(w[(4 * j + i) % (4 * sizeof(T))]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const uint32_t u = w[2 * j + i];
         if (std::is_same<T, __half>::value) {
-          const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+          const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&u));
           v[2 * i] = f.x;
           v[2 * i + 1] = f.y;
         } else {
-          v[2 * i] = __uint_as_float(w[i] << 16);
-          v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+          v[2 * i] = __uint_as_float(u << 16);
+          v[2 * i + 1] = __uint_as_float(u & 0xffff0000u);
         }
       }
-      return;
     }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float4 a = __ldg(reinterpret_cast<const float4*>(row + c) + i);
-      v[4 * i] = a.x;
-      v[4 * i + 1] = a.y;
-      v[4 * i + 2] = a.z;
-      v[4 * i + 3] = a.w;
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 16; ++i) v[i] = c + i < K ? to_f32(row[c + i]) : 0.f;
   }
-  m = 0;
-#pragma unroll
-  for (int i = 0; i < 16; ++i) m = max(m, mag(v[i]));
-}
+};
 
 // One scale per 128 values of a row: 8 lanes hold a group, 16 values each.  I: 32-bit indices of groups where they fit
-// (a 64-bit division per group took as long as all the rest).
+// (a 64-bit division per group took as long as all the rest).  It has to read 2 (4) bytes a value and write 1; what holds
+// it below the memory's rate is that a warp computes while it has no load under way, so many warps are needed:
+// 8192 x 4096 bf16 takes 21.8 us at 6 CTAs per SM (4.7 TB/s), 23.6 at 4, 26.7 at 3 and 22.7 at 8, where registers spill;
+// asking for the next group ahead took 25.8.  fp32: 32.5 us at 4 CTAs (5.2 TB/s).
+template <typename T>
+constexpr int kRowsBlocks = sizeof(T) == 4 ? 4 : 6;
+// the same for blocks of 128 rows: 4096 x 8192 bf16 20.2 us at 4 CTAs per SM (5.0 TB/s), 23.9 at 5, 26.9 at 6, 21.3 at 3
+template <typename T>
+constexpr int kBlocksBlocks = sizeof(T) == 4 ? 2 : 4;
+
 template <typename T, typename I>
-__global__ void __launch_bounds__(256) fp8_rows_kernel(const T* __restrict__ x, I n, I G, int64_t K, int64_t ldx, int vec,
-                                                       uint8_t* __restrict__ codes, int64_t ldc, float* __restrict__ scale) {
+__global__ void __launch_bounds__(256, kRowsBlocks<T>) fp8_rows_kernel(const T* __restrict__ x, I n, I G, int64_t K, int64_t ldx,
+                                                                    int vec, uint8_t* __restrict__ codes, int64_t ldc,
+                                                                    float* __restrict__ scale) {
   pdl_wait();
   const int l = threadIdx.x & 7;
   const I stride = static_cast<I>(gridDim.x) * (blockDim.x >> 3);
+  const I i0 = static_cast<I>(blockIdx.x) * (blockDim.x >> 3) + (threadIdx.x >> 3);
 #pragma unroll 1
-  for (I i = static_cast<I>(blockIdx.x) * (blockDim.x >> 3) + (threadIdx.x >> 3); i - (threadIdx.x >> 3 & 3) < n; i += stride) {
-    const bool in = i < n;  // a warp's four groups leave the loop together
-    const I m = in ? i / G : 0;
-    const int64_t c = in ? static_cast<int64_t>(i - m * G) * BLK + 16 * l : K;
-    float v[16];
-    uint32_t b;
-    load16(x + static_cast<int64_t>(m) * ldx, c, K, vec != 0, v, b);
+  for (I i = i0; i - (threadIdx.x >> 3 & 3) < n; i += stride) {  // a warp's four groups leave the loop together
+    const I m = i < n ? i / G : 0;
+    const int64_t c = i < n ? static_cast<int64_t>(i - m * G) * BLK + 16 * l : K;
+    Raw16<T> raw;
+    raw.load(x + static_cast<int64_t>(m) * ldx, c, K, vec != 0);
+    uint32_t b = raw.top();
 #pragma unroll
     for (int o = 4; o > 0; o >>= 1) b = max(b, __shfl_xor_sync(0xffffffffu, b, o));
     const float amax = group_amax(b);
-    uint16_t q[8];
-    quantize_values<T>(v, amax, Divider(amax), q);
-    uint8_t* to = codes + static_cast<int64_t>(m) * ldc;
-    if (c + 16 <= K) {
-      uint32_t w[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) w[j] = q[2 * j] | (static_cast<uint32_t>(q[2 * j + 1]) << 16);
-      *reinterpret_cast<uint4*>(to + c) = make_uint4(w[0], w[1], w[2], w[3]);
-    } else {
-#pragma unroll
-      for (int j = 0; j < 16; ++j)
-        if (c + j < K) to[c + j] = static_cast<uint8_t>(q[j >> 1] >> (8 * (j & 1)));
-    }
-    if (l == 0 && in) scale[i] = group_scale(amax);
+    uint32_t w[4];
+    raw.codes(amax, Divider(amax), w);
+    store16(codes + static_cast<int64_t>(m) * ldc, c, K, w);
+    if (l == 0 && i < n) scale[i] = group_scale(amax);
   }
 }
 
-// one scale per 128 x 128 block: a CTA per block, 16 lanes a row, 8 rows of 16 passes
+// One scale per 128 x 128 block: a CTA per block, 8 lanes a row, 32 rows of 4 passes; the values wait in registers for
+// the block's maximum.
 template <typename T>
-__global__ void __launch_bounds__(256) fp8_blocks_kernel(const T* __restrict__ x, int64_t M, int64_t K, int64_t ldx, int vec,
-                                                         uint8_t* __restrict__ codes, int64_t ldc, float* __restrict__ scale) {
+__global__ void __launch_bounds__(256, kBlocksBlocks<T>) fp8_blocks_kernel(const T* __restrict__ x, int64_t M, int64_t K,
+                                                                          int64_t ldx, int vec, uint32_t G,
+                                                                          uint8_t* __restrict__ codes, int64_t ldc,
+                                                                          float* __restrict__ scale) {
   pdl_wait();
   __shared__ uint32_t red[8];
-  const int64_t G = (K + BLK - 1) / BLK;
-  const int64_t mb = blockIdx.x / G, g = blockIdx.x - mb * G;
-  const int64_t c = g * BLK + 8 * (threadIdx.x & 15);
-  float v[8][8];
+  const uint32_t mb = blockIdx.x / G, g = blockIdx.x - mb * G;
+  const int64_t c = static_cast<int64_t>(g) * BLK + 16 * (threadIdx.x & 7);
+  const int64_t m0 = static_cast<int64_t>(mb) * BLK + (threadIdx.x >> 3);
+  Raw16<T> raw[4];
   uint32_t b = 0;
 #pragma unroll
-  for (int p = 0; p < 8; ++p) {
-    const int64_t m = mb * BLK + p * 16 + (threadIdx.x >> 4);
-    load_part(x + (m < M ? m : 0) * ldx, m < M ? c : K, K, vec != 0, v[p]);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) b = max(b, mag(v[p][j]));
+  for (int p = 0; p < 4; ++p) {
+    const int64_t m = m0 + p * 32;
+    raw[p].load(x + (m < M ? m : 0) * ldx, m < M ? c : K, K, vec != 0);
   }
+#pragma unroll
+  for (int p = 0; p < 4; ++p) b = max(b, raw[p].top());
   b = __reduce_max_sync(0xffffffffu, b);
   if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = b;
   __syncthreads();
@@ -244,11 +239,11 @@ __global__ void __launch_bounds__(256) fp8_blocks_kernel(const T* __restrict__ x
   const float amax = group_amax(b);
   const Divider div(amax);
 #pragma unroll
-  for (int p = 0; p < 8; ++p) {
-    const int64_t m = mb * BLK + p * 16 + (threadIdx.x >> 4);
-    uint16_t q[4];
-    quantize_values<T>(v[p], amax, div, q);
-    if (m < M) store_part(codes + m * ldc, c, K, q);
+  for (int p = 0; p < 4; ++p) {
+    const int64_t m = m0 + p * 32;
+    uint32_t w[4];
+    raw[p].codes(amax, div, w);
+    store16(codes + m * ldc, m < M ? c : K, K, w);
   }
   if (threadIdx.x == 0) scale[blockIdx.x] = group_scale(amax);
 }
@@ -304,123 +299,146 @@ __device__ __forceinline__ void codes_to_f16(uint32_t c, uint32_t& lo, uint32_t&
   hi = e4m3x2_to_f16x2(static_cast<uint16_t>(c >> 16));
 }
 
-struct Raw {};  // tag: x holds e4m3 codes
+struct Codes {};  // tag: x holds e4m3 codes
 
-// this lane's 32 values 128 s + 32 t .. of a row of x, as 16 code pairs, and the group's scale
-template <typename T>
-__device__ __forceinline__ void row_codes(const LinArgs& a, int64_t m, bool in, int s, int t, uint32_t (&q)[8], float& scale) {
-  const int64_t c = static_cast<int64_t>(s) * BLK + 32 * t;
-  float v[4][8];
-  uint32_t b = 0;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    load_part(static_cast<const T*>(a.x) + m * a.ldx, in ? c + 8 * i : a.K, a.K, a.vec != 0, v[i]);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) b = max(b, mag(v[i][j]));
-  }
-  b = max(b, __shfl_xor_sync(0xffffffffu, b, 1));
-  b = max(b, __shfl_xor_sync(0xffffffffu, b, 2));
-  const float amax = group_amax(b);
-  scale = group_scale(amax);
-  const Divider div(amax);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    uint16_t c[4];
-    quantize_values<T>(v[i], amax, div, c);
-#pragma unroll
-    for (int j = 0; j < 2; ++j) q[2 * i + j] = c[2 * j] | (static_cast<uint32_t>(c[2 * j + 1]) << 16);
-  }
-}
-template <>
-__device__ __forceinline__ void row_codes<Raw>(const LinArgs& a, int64_t m, bool in, int s, int t, uint32_t (&q)[8], float& scale) {
-  const int64_t c = static_cast<int64_t>(s) * BLK + 32 * t;
-  const uint8_t* p = static_cast<const uint8_t*>(a.x) + m * a.ldx + c;
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    uint4 v = make_uint4(0, 0, 0, 0);
-    if (in && c + 16 * i < a.K) v = __ldg(reinterpret_cast<const uint4*>(p) + i);  // K is a multiple of 16
-    q[4 * i] = v.x;
-    q[4 * i + 1] = v.y;
-    q[4 * i + 2] = v.z;
-    q[4 * i + 3] = v.w;
-  }
-  scale = in ? a.xs[m * a.G + s] : 0.f;
-}
+// Rows of x as the columns of mma.sync m16n8k16 (NB blocks of 8), 16 weight rows per CTA as its rows; W warps split K
+// by 128-groups and hold the next group's codes while they work on one.  e4m3 is exact in fp16, so the products are
+// exact and sums are fp32.  The order of K within a group is free as long as both sides agree: lane t of a quad
+// has bytes 16 t and 64 + 16 t of a group's 128, so that a quad reads 64 bytes at once.
+// T other than Codes (NB = 1): every CTA quantizes the rows for itself into shared memory, which saves a launch.
+// The weight's bytes bound it: 8 x 8192 x 4096 takes 9.1 us (3.7 TB/s; 8 warps 8.5), 8 x 4096 x 14336 12.5 (4.7 TB/s; 8 warps
+// 16.2), 8 x 2048 x 2048 2.6 (8 warps 2.7), one token 2048 x 2048 with its quantization 2.8.
+template <int W, int NB>
+constexpr int kFewRed = W * 16 * (NB * 8 + 1) * 4;
 
-// 16 weight rows per CTA as the rows of mma.sync m16n8k16, 8 rows of x as its columns; 16 warps split K by
-// 128-groups and hold the next group's codes while they work on one.  e4m3 is exact in fp16, so the products are exact
-// and sums are fp32.  Rows of x that come as values are quantized by every CTA for itself: 4 KB of them against the 32
-// KB of weights that the CTA reads, and one launch less.
-constexpr int FEW_WARPS = 16;
+__host__ __device__ constexpr int few_pitch(int G) { return G * BLK + 64; }  // 8 rows' 64 bytes in different banks
 
-template <typename T>
-__global__ void __launch_bounds__(FEW_WARPS * 32) fp8_few_rows_kernel(const LinArgs a) {
-  __shared__ float red[FEW_WARPS][16][9];
+template <typename T, int W, int NB, int CTAS>
+__global__ void __launch_bounds__(W * 32, CTAS) fp8_few_rows_kernel(const LinArgs a) {
+  constexpr bool kCodes = std::is_same<T, Codes>::value;
+  extern __shared__ __align__(16) uint8_t few_smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   pdl_wait();
   const int n0 = blockIdx.x * 16;
-  const int64_t m0 = static_cast<int64_t>(blockIdx.y) * 8;
-  const int ra = min(n0 + g, a.N - 1), rb = min(n0 + g + 8, a.N - 1);
-  const uint8_t* pa = a.w + ra * a.ldw + 32 * t;
-  const uint8_t* pb = a.w + rb * a.ldw + 32 * t;
+  const uint8_t* pw[2] = {a.w + min(n0 + g, a.N - 1) * a.ldw + 16 * t, a.w + min(n0 + g + 8, a.N - 1) * a.ldw + 16 * t};
   const float* ws = a.ws + static_cast<int64_t>(n0 / BLK) * a.G;
-  float acc[4] = {0.f, 0.f, 0.f, 0.f};
-  uint4 wa[2], wb[2];
-  float wsc = 0.f;
+  const int pitch = few_pitch(a.G);
+  float* sscale = reinterpret_cast<float*>(few_smem + 8 * pitch);  // [8][G]
+  float acc[NB][4] = {};
+  uint4 wv[2][2], xv[NB][2];
+  float wsc = 0.f, xsc[NB][2];
   auto load = [&](int s) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const bool in = s * BLK + 32 * t + 16 * i < a.K;
-      wa[i] = in ? load_once(pa + s * BLK + 16 * i) : make_uint4(0, 0, 0, 0);
-      wb[i] = in ? load_once(pb + s * BLK + 16 * i) : make_uint4(0, 0, 0, 0);
+    for (int j = 0; j < 2; ++j) {
+      const int c = s * BLK + 64 * j;
+      const bool in = c + 16 * t < a.K;  // K is a multiple of 16
+#pragma unroll
+      for (int h = 0; h < 2; ++h) wv[h][j] = in ? load_once(pw[h] + c) : make_uint4(0, 0, 0, 0);
+      if (kCodes)
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+          xv[b][j] = in && 8 * b + g < a.M
+                         ? __ldg(reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(a.x) + (8 * b + g) * a.ldx + c + 16 * t))
+                         : make_uint4(0, 0, 0, 0);
     }
     wsc = s < a.G ? __ldg(ws + s) : 0.f;
+    if (kCodes)
+#pragma unroll
+      for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int m = 8 * b + 2 * t + i;
+          xsc[b][i] = s < a.G && m < a.M ? __ldg(a.xs + static_cast<int64_t>(m) * a.G + s) : 0.f;
+        }
   };
   load(warp);
+  if constexpr (!kCodes) {
+    const int l = threadIdx.x & 7, n = static_cast<int>(a.M) * a.G;
 #pragma unroll 1
-  for (int s = warp; s < a.G; s += FEW_WARPS) {
-    uint32_t q[8];
-    float sc;
-    row_codes<T>(a, m0 + g < a.M ? m0 + g : 0, m0 + g < a.M, s, t, q, sc);
-    float d[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int i = threadIdx.x >> 3; i - (threadIdx.x >> 3 & 3) < n; i += W * 4) {
+      const int m = i < n ? i / a.G : 0, s = i - m * a.G;
+      Raw16<T> raw;
+      raw.load(static_cast<const T*>(a.x) + m * a.ldx, i < n ? s * BLK + 16 * l : a.K, a.K, a.vec != 0);
+      uint32_t b = raw.top();
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const uint32_t ua[4] = {wa[i].x, wa[i].y, wa[i].z, wa[i].w}, ub[4] = {wb[i].x, wb[i].y, wb[i].z, wb[i].w};
+      for (int o = 4; o > 0; o >>= 1) b = max(b, __shfl_xor_sync(0xffffffffu, b, o));
+      const float amax = group_amax(b);
+      uint32_t w[4];
+      raw.codes(amax, Divider(amax), w);
+      if (i < n) *reinterpret_cast<uint4*>(few_smem + m * pitch + s * BLK + 16 * l) = make_uint4(w[0], w[1], w[2], w[3]);
+      if (l == 0 && i < n) sscale[i] = group_scale(amax);
+    }
+    __syncthreads();
+  }
+#pragma unroll 1
+  for (int s = warp; s < a.G; s += W) {
+    if (!kCodes) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        uint32_t a0, a1, a2, a3, b0, b1;
-        codes_to_f16(ua[j], a0, a2);
-        codes_to_f16(ub[j], a1, a3);
-        codes_to_f16(q[4 * i + j], b0, b1);
-        mma_f16(d, a0, a1, a2, a3, b0, b1);
+      for (int j = 0; j < 2; ++j)
+        xv[0][j] = g < a.M ? *reinterpret_cast<const uint4*>(few_smem + g * pitch + s * BLK + 64 * j + 16 * t)
+                           : make_uint4(0, 0, 0, 0);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) xsc[0][i] = 2 * t + i < a.M ? sscale[(2 * t + i) * a.G + s] : 0.f;
+    }
+    float d[NB][4] = {};
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        uint32_t a0, a1, a2, a3;
+        codes_to_f16(reinterpret_cast<const uint32_t*>(&wv[0][j])[k], a0, a2);
+        codes_to_f16(reinterpret_cast<const uint32_t*>(&wv[1][j])[k], a1, a3);
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+          uint32_t b0, b1;
+          codes_to_f16(reinterpret_cast<const uint32_t*>(&xv[b][j])[k], b0, b1);
+          mma_f16(d[b], a0, a1, a2, a3, b0, b1);
+        }
       }
     }
-    // columns 2t and 2t + 1: rows of x whose scales lanes 8t and 8t + 4 hold
-    const float s0 = __fmul_rn(__shfl_sync(0xffffffffu, sc, 8 * t), wsc);
-    const float s1 = __fmul_rn(__shfl_sync(0xffffffffu, sc, 8 * t + 4), wsc);
-    load(s + FEW_WARPS);
-    acc[0] = __fmaf_rn(s0, d[0], acc[0]);
-    acc[1] = __fmaf_rn(s1, d[1], acc[1]);
-    acc[2] = __fmaf_rn(s0, d[2], acc[2]);
-    acc[3] = __fmaf_rn(s1, d[3], acc[3]);
+    float f[NB][2];
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) f[b][i] = __fmul_rn(xsc[b][i], wsc);
+    load(s + W);
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[b][e] = __fmaf_rn(f[b][e & 1], d[b][e], acc[b][e]);
   }
-  red[warp][g][2 * t] = acc[0];
-  red[warp][g][2 * t + 1] = acc[1];
-  red[warp][g + 8][2 * t] = acc[2];
-  red[warp][g + 8][2 * t + 1] = acc[3];
+  if (!kCodes) __syncthreads();  // the parts go over the codes
+  float(*red)[16][NB * 8 + 1] = reinterpret_cast<float(*)[16][NB * 8 + 1]>(few_smem);
+#pragma unroll
+  for (int b = 0; b < NB; ++b)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) red[warp][g + 8 * (e >> 1)][8 * b + 2 * t + (e & 1)] = acc[b][e];
   __syncthreads();
-  if (threadIdx.x < 128) {
-    const int r = threadIdx.x & 15, col = threadIdx.x >> 4;
+  for (int i = threadIdx.x; i < 16 * NB * 8; i += W * 32) {
+    const int r = i % 16, m = i / 16, n = n0 + r;
+    if (n >= a.N || m >= a.M) continue;
     float v = 0.f;
 #pragma unroll
-    for (int w = 0; w < FEW_WARPS; ++w) v = __fadd_rn(v, red[w][r][col]);
-    const int n = n0 + r;
-    const int64_t m = m0 + col;
-    if (n < a.N && m < a.M) {
-      if (a.bias != nullptr) v = __fadd_rn(v, load_as_f32(a.bias, a.out_type, n));
-      store_from_f32(a.out, a.out_type, m * a.N + n, v);
-    }
+    for (int w = 0; w < W; ++w) v = __fadd_rn(v, red[w][r][m]);
+    if (a.bias != nullptr) v = __fadd_rn(v, load_as_f32(a.bias, a.out_type, n));
+    store_from_f32(a.out, a.out_type, static_cast<int64_t>(m) * a.N + n, v);
   }
+}
+
+template <typename T, int W, int NB, int CTAS>
+int launch_few(const LinArgs& a, cudaStream_t st) {
+  int smem = kFewRed<W, NB>;
+  if (!std::is_same<T, Codes>::value) smem = std::max(smem, 8 * few_pitch(a.G) + 32 * a.G);
+  if (smem > 48 * 1024) {
+    static std::atomic<uint64_t> ready{0};
+    const cudaError_t e = once_per_device(ready, [] {
+      return cudaFuncSetAttribute(fp8_few_rows_kernel<T, W, NB, CTAS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                  8 * few_pitch(kOwnK / BLK) + 32 * static_cast<int>(kOwnK / BLK));
+    });
+    if (e != cudaSuccess) return fail(LLQ_ECUDA, "fp8_few_rows_kernel: %s", cudaGetErrorString(e));
+  }
+  launch_pdl(fp8_few_rows_kernel<T, W, NB, CTAS>, dim3((a.N + 15) / 16), dim3(W * 32), smem, st, a);
+  return check_launch("fp8_few_rows_kernel");
 }
 
 template <typename T>
@@ -431,7 +449,7 @@ int launch_rows(const void* x, int64_t M, int64_t K, int64_t ldx, int block_rows
   if (block_rows == 1) {
     const int64_t n = M * G;
     int64_t blocks = (n + 31) / 32;
-    const int64_t most = static_cast<int64_t>(num_sms()) * 8;
+    const int64_t most = static_cast<int64_t>(num_sms()) * kRowsBlocks<T>;
     if (blocks > most) blocks = most;
     const dim3 grid(static_cast<unsigned>(blocks));
     if (n < (1 << 30))
@@ -443,7 +461,7 @@ int launch_rows(const void* x, int64_t M, int64_t K, int64_t ldx, int block_rows
     return check_launch("fp8_rows_kernel");
   }
   launch_pdl(fp8_blocks_kernel<T>, dim3(static_cast<unsigned>((M + BLK - 1) / BLK * G)), dim3(256), 0, st,
-             static_cast<const T*>(x), M, K, ldx, vec, codes, ldc, scale);
+             static_cast<const T*>(x), M, K, ldx, vec, static_cast<uint32_t>(G), codes, ldc, scale);
   return check_launch("fp8_blocks_kernel");
 }
 
@@ -469,6 +487,19 @@ int fp8_quantize(const void* x, int x_dtype, int64_t M, int64_t K, int64_t ldx, 
   return fail(LLQ_EUNSUPPORTED, "unknown dtype %d", x_dtype);
 }
 
+// Does the product run on fp8_few_rows_kernel (else on fp8_tc_kernel)?  Up to 16 rows it always won (16 x 2048 x 2048 3.1 us
+// against 7.9, 16 x 8192 x 4096 11.9 against 16.3); with 32, where every CTA reads
+// more of x than of the weight, only small weights are faster there (32 x 4096 x 2048 6.5 us against 10.5, 32 x 4096 x 4096
+// 10.6 against 11.9, 32 x 8192 x 4096 18.5 against 14.0).
+static bool few_rows(int64_t M, int64_t K, int64_t N) { return M <= 16 || (M <= 32 && N * K <= 1 << 24); }
+
+// Do its CTAs quantize the rows for themselves?  Each does all of them again, N / 16 times together, which beats a launch for
+// few values (1 x 1024 x 1024 2.2 us against 3.1, 8 x 2048 x 2048 4.0 against 4.2, 1 x 3000 x 7168 9.1 against 10.1) and not
+// for many (1 x 8192 x 4096 10.7 against 9.7, 8 x 8192 x 4096 20.0 against 10.0).
+static bool few_quantizes(int64_t M, int64_t K, int64_t N) {
+  return M <= 8 && K <= kOwnK && M * K * ((N + 15) / 16) <= 1 << 21;
+}
+
 int fp8_linear(const void* x, int x_dtype, const float* x_scale, int64_t M, int K, int64_t ldx, const uint8_t* w,
                const float* w_scale, int N, int64_t ldw, const void* bias, void* out, int out_dtype, void* workspace,
                size_t bytes, cudaStream_t st) {
@@ -480,6 +511,7 @@ int fp8_linear(const void* x, int x_dtype, const float* x_scale, int64_t M, int 
   if (ldw % 16 != 0 || (reinterpret_cast<uintptr_t>(w) & 15) != 0)
     return fail(LLQ_EINVAL, "the weight codes need a 16-byte aligned base and row pitch");
   if (M > 0x7fffffff - 256) return fail(LLQ_EINVAL, "too many rows");
+  if (K > 1 << 30) return fail(LLQ_EINVAL, "K too large");
   if (M == 0) return LLQ_OK;
   if (x == nullptr || w == nullptr || w_scale == nullptr || out == nullptr) return fail(LLQ_EINVAL, "null pointer");
   const int size = x_dtype == LLQ_E4M3 ? 1 : x_dtype == LLQ_F32 ? 4 : 2;
@@ -491,23 +523,25 @@ int fp8_linear(const void* x, int x_dtype, const float* x_scale, int64_t M, int 
     return fail(LLQ_EUNSUPPORTED, "unknown dtype %d", x_dtype);
   }
   const int G = (K + BLK - 1) / BLK;
-  if (M > kFewRows) {
+  const bool own = x_dtype != LLQ_E4M3 && few_quantizes(M, K, N);  // the product's own kernel quantizes the rows
+  const uint8_t* codes = static_cast<const uint8_t*>(x);
+  if (x_dtype != LLQ_E4M3 && !own) {  // quantized once into the workspace
+    const size_t need = fp8_linear_workspace(M, K, N, x_dtype);
+    if (workspace == nullptr || bytes < need) return fail(LLQ_ENOSPACE, "workspace needs %zu bytes, got %zu", need, bytes);
+    if (reinterpret_cast<uintptr_t>(workspace) & 15) return fail(LLQ_EINVAL, "the workspace needs 16-byte alignment");
+    uint8_t* to = static_cast<uint8_t*>(workspace);
+    float* scale = reinterpret_cast<float*>(to + static_cast<size_t>(M) * K);
+    const int rc = fp8_quantize(x, x_dtype, M, K, ldx, 1, to, K, scale, st);
+    if (rc) return rc;
+    codes = to;
+    x_scale = scale;
+    ldx = K;
+  }
+  if (!few_rows(M, K, N)) {
     Fp8Operands p{};
-    p.x = static_cast<const uint8_t*>(x);
+    p.x = codes;
     p.xs = x_scale;
     p.ldx = ldx;
-    if (x_dtype != LLQ_E4M3) {  // quantized once into the workspace
-      const size_t need = fp8_linear_workspace(M, K, N, x_dtype);
-      if (workspace == nullptr || bytes < need) return fail(LLQ_ENOSPACE, "workspace needs %zu bytes, got %zu", need, bytes);
-      if (reinterpret_cast<uintptr_t>(workspace) & 15) return fail(LLQ_EINVAL, "the workspace needs 16-byte alignment");
-      uint8_t* codes = static_cast<uint8_t*>(workspace);
-      float* scale = reinterpret_cast<float*>(codes + static_cast<size_t>(M) * K);
-      const int rc = fp8_quantize(x, x_dtype, M, K, ldx, 1, codes, K, scale, st);
-      if (rc) return rc;
-      p.x = codes;
-      p.xs = scale;
-      p.ldx = K;
-    }
     p.w = w;
     p.ws = w_scale;
     p.ldw = ldw;
@@ -521,7 +555,7 @@ int fp8_linear(const void* x, int x_dtype, const float* x_scale, int64_t M, int 
     return fp8_gemm_tc(p, st);
   }
   LinArgs a{};
-  a.x = x;
+  a.x = own ? x : codes;
   a.xs = x_scale;
   a.ldx = ldx;
   a.vec = vec;
@@ -535,19 +569,21 @@ int fp8_linear(const void* x, int x_dtype, const float* x_scale, int64_t M, int 
   a.N = N;
   a.K = K;
   a.G = G;
-  const dim3 grid((N + 15) / 16, static_cast<unsigned>((M + 7) / 8));
-  switch (x_dtype) {
-    case LLQ_E4M3: launch_pdl(fp8_few_rows_kernel<Raw>, grid, dim3(FEW_WARPS * 32), 0, st, a); break;
-    case LLQ_F32: launch_pdl(fp8_few_rows_kernel<float>, grid, dim3(FEW_WARPS * 32), 0, st, a); break;
-    case LLQ_F16: launch_pdl(fp8_few_rows_kernel<__half>, grid, dim3(FEW_WARPS * 32), 0, st, a); break;
-    default: launch_pdl(fp8_few_rows_kernel<__nv_bfloat16>, grid, dim3(FEW_WARPS * 32), 0, st, a); break;
+  if (!own) {
+    if (M > 16) return launch_few<Codes, 8, 4, 2>(a, st);
+    if (M > 8) return launch_few<Codes, 8, 2, 2>(a, st);
+    return launch_few<Codes, 16, 1, 2>(a, st);
   }
-  return check_launch("fp8_few_rows_kernel");
+  switch (x_dtype) {
+    case LLQ_F32: return launch_few<float, 16, 1, 2>(a, st);
+    case LLQ_F16: return launch_few<__half, 16, 1, 2>(a, st);
+    default: return launch_few<__nv_bfloat16, 16, 1, 2>(a, st);
+  }
 }
 
 // codes [M][K] (K is a multiple of 16) and scales [M][G] of rows that are quantized before the tensor-core product
 size_t fp8_linear_workspace(int64_t M, int K, int N, int x_dtype) {
-  if (M <= kFewRows || K < 1 || x_dtype == LLQ_E4M3) return 0;
+  if (M < 1 || K < 1 || x_dtype == LLQ_E4M3 || few_quantizes(M, K, N)) return 0;
   return static_cast<size_t>(M) * K + static_cast<size_t>(M) * ((K + BLK - 1) / BLK) * 4;
 }
 

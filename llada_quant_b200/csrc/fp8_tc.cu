@@ -452,16 +452,17 @@ int fp8_gemm_tc(const Fp8Operands& p, cudaStream_t st) {
   const int sms = num_sms();
   auto tiles = [&](int bn) { return mt * ((p.N + bn - 1) / bn); };
   // Tile width and K split by the bytes that the busiest SM brings from L2: waves x blocks of K x (128 + BN) rows of 128
-  // bytes; a split costs about 1 us more, that is 1000 such rows, and its clusters must fit at once (148 SMs hold 132
-  // CTAs in clusters of four, 120 in clusters of eight).  Measured at 256 x 8192 x 2048: 128 wide in one wave 9.9 us,
-  // 64 wide in two 14.4.
+  // bytes; a split costs about as much as 1500 such rows, and its clusters must fit at once (148 SMs hold 132 CTAs in
+  // clusters of four, 120 in clusters of eight).  Measured with each width forced (256 / 128 / 64, us): 256 x 8192 x 2048
+  // 13.1 / 9.8 / 16.3, 1024 x 4096 x 4096 24.2 / 26.3 / 46.1, 64 x 8192 x 2048 12.2 / 11.0 / 10.0; without a split
+  // 256 x 2048 x 8192 takes 22.4 instead of 14.6 and 512 x 1000 x 7168 20.6 instead of 13.5.
   int bn = 64, split = 1;
   int64_t best = INT64_MAX;
   for (int w : {256, 128, 64}) {
     for (int sp : {1, 2, 4, 8}) {
       const int room = sp == 8 ? sms * 120 / 148 : sp == 4 ? sms * 132 / 148 : sms;
       if (sp > 1 && (tiles(w) * sp > room || sp * 2 > p.G || w == 256)) break;
-      const int64_t cost = (tiles(w) + sms - 1) / sms * ((p.G + sp - 1) / sp) * (BM + w) + (sp > 1 ? 1000 : 0);
+      const int64_t cost = (tiles(w) + sms - 1) / sms * ((p.G + sp - 1) / sp) * (BM + w) + (sp > 1 ? 1500 : 0);
       if (cost < best) {
         best = cost;
         bn = w;
