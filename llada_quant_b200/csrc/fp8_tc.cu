@@ -11,7 +11,8 @@
 // A tile is 128 rows (TMEM lanes, so a row's scale is one number per thread) by BN weight rows.
 //   warp 0      TMA producer: per block the 128 x 128 and BN x 128 byte boxes (128-byte swizzle)
 //   warp 1      TMEM allocator and MMA issuer (one elected lane)
-//   warps 2, 3  idle: they fill the warpgroup whose registers the epilogue takes over
+//   warps 2, 3  bring the rows' scales to shared memory: as loads of the epilogue's threads, one line each, they held up
+//               its waits and took as many cycles as its sums
 //   warps 4-11  epilogue: one TMEM lane quarter each, half of the columns; BN / 2 sums per thread
 // What bounds a large product is this epilogue: 128 x BN sums per 128 of K leave TMEM and pass the FMA pipe (256
 // cycles at BN = 256; as fma.rn.f32x2 it took three instructions a pair) while the tensor core needs 512 cycles for
@@ -48,8 +49,10 @@ struct F8Cfg {
   static constexpr int FIRST_EPI = 4;
   static constexpr int THREADS = (FIRST_EPI + EPI_WARPS) * 32;
   static constexpr int OUT_BYTES = EPI_WARPS * 4096;  // per warp 32 rows of 128 bytes
-  static constexpr int STAGES = (232448 - 1024 - 512 - OUT_BYTES) / STAGE_BYTES;
-  static constexpr size_t SMEM_BYTES = 1024 + static_cast<size_t>(STAGES) * STAGE_BYTES + OUT_BYTES + 512;
+  static constexpr int HEAD_BYTES = 3072;  // barriers (1 KB) and the rows' scales, one vector per accumulator buffer
+  static constexpr int STAGES = (232448 - HEAD_BYTES - OUT_BYTES) / STAGE_BYTES;
+  static constexpr size_t SMEM_BYTES = HEAD_BYTES + static_cast<size_t>(STAGES) * STAGE_BYTES + OUT_BYTES;
+  static_assert(1024 + ACC_BUFS * BM * 4 <= HEAD_BYTES, "head");
   static_assert(128 * BN * 4 <= STAGES * STAGE_BYTES, "the parts of a split tile reuse the stages");
   static_assert(SMEM_BYTES <= 232448, "shared memory");
 };
@@ -115,6 +118,13 @@ __device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, const void*
   asm volatile("cp.async.bulk.commit_group;" ::: "memory");
 }
 
+// a load that stays where it is written: the compiler would move it down to its first use, behind the wait it is to overlap
+__device__ __forceinline__ float load_ahead(const float* p) {
+  float v;
+  asm volatile("ld.global.nc.f32 %0, [%1];" : "=f"(v) : "l"(p));
+  return v;
+}
+
 template <typename O>
 __device__ __forceinline__ float bias_at(const void* b, int n) {
   return to_f32(static_cast<const O*>(b)[n]);
@@ -142,10 +152,11 @@ __global__ void __launch_bounds__(F8Cfg<BN>::THREADS, 1)
     fp8_tc_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w,
                   const __grid_constant__ CUtensorMap tm_o, const F8Args a) {
   using C = F8Cfg<BN>;
-  extern __shared__ __align__(1024) uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  extern __shared__ __align__(1024) uint8_t smem_head[];  // 1024: what the 128-byte swizzle counts from
+  float* row_scale = reinterpret_cast<float*>(smem_head + 1024);  // [ACC_BUFS][BM]
+  uint8_t* smem = smem_head + C::HEAD_BYTES;
   uint8_t* so = smem + C::STAGES * C::STAGE_BYTES;
-  uint64_t* full = reinterpret_cast<uint64_t*>(so + C::OUT_BYTES);
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem_head);
   uint64_t* empty = full + C::STAGES;
   uint64_t* acc_full = empty + C::STAGES;
   uint64_t* acc_empty = acc_full + C::ACC_BUFS;
@@ -159,7 +170,7 @@ __global__ void __launch_bounds__(F8Cfg<BN>::THREADS, 1)
       mbar_init(&empty[i], 1);
     }
     for (int i = 0; i < C::ACC_BUFS; ++i) {
-      mbar_init(&acc_full[i], 1);
+      mbar_init(&acc_full[i], 1 + 2);  // the MMAs' commit and the scale warps
       mbar_init(&acc_empty[i], C::EPI_WARPS);
     }
     *abort_flag = 0;
@@ -224,8 +235,8 @@ __global__ void __launch_bounds__(F8Cfg<BN>::THREADS, 1)
     bool ok = true;
     for (int u = blockIdx.x / a.split; u < a.tiles && ok; u += stride) {
       for (int g = g0; g < g1; ++g) {
-        if (!mbar_wait(&acc_empty[ab], aph ^ 1, abort_flag, 0x510 + ab)) { ok = false; break; }
         if (!mbar_wait(&full[rs], ph, abort_flag, 0x520 + rs)) { ok = false; break; }
+        if (!mbar_wait(&acc_empty[ab], aph ^ 1, abort_flag, 0x510 + ab)) { ok = false; break; }
         tc_fence_after();
         const uint64_t ad = make_sdesc(smem_u32(smem + rs * C::STAGE_BYTES));
         const uint64_t bd = make_sdesc(smem_u32(smem + rs * C::STAGE_BYTES + C::A_BYTES));
@@ -244,7 +255,43 @@ __global__ void __launch_bounds__(F8Cfg<BN>::THREADS, 1)
         }
       }
     }
-  } else if (warp >= C::FIRST_EPI) {
+  } else if (warp < C::FIRST_EPI) {
+    // the scales of 64 rows, four blocks at a time, one block ahead of the accumulators
+    const int r0 = (warp - 2) * 64 + lane;
+    const bool vec = a.G % 4 == 0 && g0 % 4 == 0 && (reinterpret_cast<uintptr_t>(a.xs) & 15) == 0;
+    int ab = 0;
+    uint32_t aph = 0;
+    bool ok = true;
+    for (int u = blockIdx.x / a.split; u < a.tiles && ok; u += stride) {
+      const int64_t m = static_cast<int64_t>(u % a.mtiles) * BM + r0;
+      const float* p0 = a.xs + (m < a.M ? m : 0) * a.G;  // rows behind the last are zero, whatever scales them
+      const float* p1 = a.xs + (m + 32 < a.M ? m + 32 : 0) * a.G;
+      auto fetch = [&](const float* p, int g) {
+        if (vec && g < g1) return __ldg(reinterpret_cast<const float4*>(p + g));
+        return make_float4(g < g1 ? __ldg(p + g) : 0.f, g + 1 < g1 ? __ldg(p + g + 1) : 0.f, g + 2 < g1 ? __ldg(p + g + 2) : 0.f,
+                           g + 3 < g1 ? __ldg(p + g + 3) : 0.f);
+      };
+      float4 n0 = fetch(p0, g0), n1 = fetch(p1, g0);
+      for (int g = g0; g < g1 && ok; g += 4) {
+        const float v[2][4] = {{n0.x, n0.y, n0.z, n0.w}, {n1.x, n1.y, n1.z, n1.w}};
+        n0 = fetch(p0, g + 4);
+        n1 = fetch(p1, g + 4);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          if (g + k >= g1) break;
+          if (!mbar_wait(&acc_empty[ab], aph ^ 1, abort_flag, 0x540 + ab)) { ok = false; break; }
+          row_scale[ab * BM + r0] = v[0][k];
+          row_scale[ab * BM + r0 + 32] = v[1][k];
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&acc_full[ab]);
+          if (++ab == C::ACC_BUFS) {
+            ab = 0;
+            aph ^= 1;
+          }
+        }
+      }
+    }
+  } else {
     if (BN == 256) asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
     const int part_of = (warp - C::FIRST_EPI) >> 2;  // this warp's columns
     const int q = warp & 3;  // the TMEM lanes a warp may read
@@ -255,26 +302,21 @@ __global__ void __launch_bounds__(F8Cfg<BN>::THREADS, 1)
     bool ok = true;
     for (int u = blockIdx.x / a.split; u < a.tiles && ok; u += stride) {
       const int m0 = u % a.mtiles * BM, n0 = u / a.mtiles * BN + part_of * C::COLS;
-      const int64_t row = static_cast<int64_t>(m0) + q * 32 + lane;
-      const bool in = row < a.M;
-      const float* xs = a.xs + (in ? row : 0) * a.G;
       const float* ws = a.ws + static_cast<int64_t>(min(n0, a.N - 1) / 128) * a.G;
       float acc[C::COLS];
 #pragma unroll
       for (int i = 0; i < C::COLS; ++i) acc[i] = 0.f;
-      float sx = in && g0 < g1 ? __ldg(xs + g0) : 0.f, sw = g0 < g1 ? __ldg(ws + g0) : 0.f;
+      float next = g0 < g1 ? load_ahead(ws + g0) : 0.f;
       for (int g = g0; g < g1; ++g) {
-        const float s = __fmul_rn(sx, sw);
-        if (g + 1 < g1) {  // the next block's scales ahead of the wait
-          sx = in ? __ldg(xs + g + 1) : 0.f;
-          sw = __ldg(ws + g + 1);
-        }
+        const float sw = next;
+        if (g + 1 < g1) next = load_ahead(ws + g + 1);
         if (!mbar_wait(&acc_full[ab], aph, abort_flag, 0x530 + ab)) { ok = false; break; }
         tc_fence_after();
         constexpr int CH = C::COLS / 32;
         const uint32_t at = lane_addr + ab * BN;
         uint32_t v[CH > 1 ? 2 : 1][32];
         tc_ld32(at, v[0]);
+        const float s = __fmul_rn(row_scale[ab * BM + q * 32 + lane], sw);
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
           tc_wait_ld32(v[c & 1]);
