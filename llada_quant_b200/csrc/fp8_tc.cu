@@ -48,7 +48,7 @@ struct F8Cfg {
   static constexpr int COLS = BN / 2;  // columns of an epilogue thread
   static constexpr int FIRST_EPI = 4;
   static constexpr int THREADS = (FIRST_EPI + EPI_WARPS) * 32;
-  static constexpr int OUT_BYTES = EPI_WARPS * 4096;  // per warp 32 rows of 128 bytes
+  static constexpr int OUT_BYTES = EPI_WARPS * 4096;  // per warp twice 32 rows of 64 bytes
   static constexpr int HEAD_BYTES = 3072;  // barriers (1 KB) and the rows' scales, one vector per accumulator buffer
   static constexpr int STAGES = (232448 - HEAD_BYTES - OUT_BYTES) / STAGE_BYTES;
   static constexpr size_t SMEM_BYTES = HEAD_BYTES + static_cast<size_t>(STAGES) * STAGE_BYTES + OUT_BYTES;
@@ -115,7 +115,6 @@ __device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, const void*
                    reinterpret_cast<uint64_t>(map)),
                "r"(x), "r"(y), "r"(smem_u32(src))
                : "memory");
-  asm volatile("cp.async.bulk.commit_group;" ::: "memory");
 }
 
 // a load that stays where it is written: the compiler would move it down to its first use, behind the wait it is to overlap
@@ -296,7 +295,6 @@ __global__ void __launch_bounds__(F8Cfg<BN>::THREADS, 1)
     const int part_of = (warp - C::FIRST_EPI) >> 2;  // this warp's columns
     const int q = warp & 3;  // the TMEM lanes a warp may read
     const uint32_t lane_addr = tmem + (static_cast<uint32_t>(q * 32) << 16) + part_of * C::COLS;
-    uint8_t* stage = so + (warp - C::FIRST_EPI) * 4096;
     int ab = 0;
     uint32_t aph = 0;
     bool ok = true;
@@ -342,13 +340,17 @@ __global__ void __launch_bounds__(F8Cfg<BN>::THREADS, 1)
         for (int i = 0; i < C::COLS; ++i) part[i * BM] = acc[i];
         break;
       }
-      // 128 bytes of every row at a time through this warp's shared memory
-      constexpr int PER = 16 / sizeof(O);                                      // outputs of 16 bytes
-      constexpr int CC = C::COLS * sizeof(O) < 128 ? C::COLS : 128 / sizeof(O);  // columns of a round
+      // 64 bytes of every row at a time through one of this warp's two pieces of shared memory
+      constexpr int PER = 16 / sizeof(O);  // outputs of 16 bytes
+      constexpr int CC = 64 / sizeof(O);   // columns of a round
 #pragma unroll
       for (int c = 0; c < C::COLS / CC; ++c) {
+        uint8_t* stage = so + (warp - C::FIRST_EPI) * 4096 + (c & 1) * 2048;  // an even number of rounds, or one
         if (a.tma_out) {
-          if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+          if (lane == 0) {
+            if (C::COLS / CC > 1) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+            else asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+          }
         }
         __syncwarp();
 #pragma unroll
@@ -361,12 +363,15 @@ __global__ void __launch_bounds__(F8Cfg<BN>::THREADS, 1)
             for (int i = 0; i < PER; ++i)
               v[i] = __fadd_rn(v[i], bias_at<O>(a.bias, min(n0 + c * CC + j * PER + i, a.N - 1)));
           }
-          *reinterpret_cast<uint4*>(stage + lane * 128 + ((j ^ (lane & 7)) * 16)) = pack_out(v, O());
+          *reinterpret_cast<uint4*>(stage + lane * 64 + ((j ^ (lane >> 1 & 3)) * 16)) = pack_out(v, O());
         }
         if (a.tma_out) {
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
           __syncwarp();
-          if (lane == 0 && n0 + c * CC < a.N && m0 + q * 32 < a.M) tma_store_2d(&tm_o, stage, n0 + c * CC, m0 + q * 32);
+          if (lane == 0) {
+            if (n0 + c * CC < a.N && m0 + q * 32 < a.M) tma_store_2d(&tm_o, stage, n0 + c * CC, m0 + q * 32);
+            asm volatile("cp.async.bulk.commit_group;" ::: "memory");  // also an empty one: the waits count them
+          }
         } else {
           __syncwarp();
           for (int r = 0; r < 32 && m0 + q * 32 + r < a.M; ++r) {
@@ -374,7 +379,7 @@ __global__ void __launch_bounds__(F8Cfg<BN>::THREADS, 1)
             for (int i = lane; i < CC; i += 32) {
               const int n = n0 + c * CC + i;
               if (n < a.N)
-                dst[n] = *reinterpret_cast<const O*>(stage + r * 128 + (((i / PER) ^ (r & 7)) * 16) + i % PER * sizeof(O));
+                dst[n] = *reinterpret_cast<const O*>(stage + r * 64 + (((i / PER) ^ (r >> 1 & 3)) * 16) + i % PER * sizeof(O));
             }
           }
           __syncwarp();
@@ -438,10 +443,10 @@ int launch_tc(const Fp8Operands& p, const F8Args& in, CUtensorMapDataType ot, cu
   if (rc) return rc;
   to = tx;
   const bool aligned = (reinterpret_cast<uintptr_t>(p.out) & 15) == 0 && (static_cast<size_t>(p.N) * sizeof(O)) % 16 == 0;
-  a.tma_out = aligned && (a.split > 1 || C::COLS * sizeof(O) >= 128);
+  a.tma_out = aligned;
   if (a.tma_out && a.split == 1) {
-    rc = make_map(&to, p.out, ot, p.N, p.M, static_cast<uint64_t>(p.N) * sizeof(O), 128 / sizeof(O), 32,
-                  CU_TENSOR_MAP_SWIZZLE_128B);
+    rc = make_map(&to, p.out, ot, p.N, p.M, static_cast<uint64_t>(p.N) * sizeof(O), 64 / sizeof(O), 32,
+                  CU_TENSOR_MAP_SWIZZLE_64B);
     if (rc) return rc;
   }
   static std::atomic<uint64_t> ready{0};
