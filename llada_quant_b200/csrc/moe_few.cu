@@ -490,7 +490,7 @@ __device__ __noinline__ void emit(const FewArgs& a, const Segment& sg, const flo
         const __nv_bfloat16 hi = __float2bfloat16_rn(h);
         __nv_bfloat16* at = reinterpret_cast<__nv_bfloat16*>(step + col * 4) + pair_place<BITS>(n);
         at[0] = hi;
-        at[lo * 8] = __float2bfloat16_rn(h - __bfloat162float(hi));
+        at[lo * 8] = __float2bfloat16_rn(__hisinf(hi) ? 0.f : h - __bfloat162float(hi));  // (infinity minus itself is a NaN)
       }
     }
   }

@@ -219,6 +219,23 @@ def test_a_bad_token_spoils_its_own_row_alone(bad):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("T", [3, 7])  # h's two parts in one plane, or in two
+@pytest.mark.parametrize("bits", [4, 8])
+def test_an_infinite_h_stays_infinite(T, bits):
+    """h beyond fp32: with positive weights its sum is infinite, not a NaN."""
+    from llada_quant_b200.few_tokens import FewTokenMoE
+    q1 = torch.full((2, 64, 32 if bits == 8 else 16), 1 if bits == 8 else 0x11, dtype=torch.int8, device="cuda")
+    q2 = torch.full((2, 32, 32 if bits == 8 else 16), 1 if bits == 8 else 0x11, dtype=torch.int8, device="cuda")
+    layer = (q1, torch.ones(2, 64, 1, device="cuda"), q2, torch.ones(2, 32, 1, device="cuda"), bits)
+    moe = FewTokenMoE(packed_of(layer, -1), torch.zeros(2, 32, dtype=torch.bfloat16, device="cuda"), 1)
+    x = torch.full((T, 32), 1.0, dtype=torch.bfloat16, device="cuda")
+    x[1] = 1e30
+    ids = torch.zeros(T, 1, dtype=torch.int32, device="cuda")
+    out = moe.routed(x, torch.ones(T, 1, device="cuda"), ids)
+    assert bool((out[1] == float("inf")).all()) and bool((out[0] == out[2]).all()) and bool(out[0].isfinite().all())
+
+
+@pytest.mark.gpu
 def test_every_code_of_both_formats():
     """One-hot rows read single weights: every byte value through w1's up rows with a constant gate."""
     from llada_quant_b200.few_tokens import FewTokenMoE

@@ -84,6 +84,14 @@ def test_quantizer_equals_its_definition(M, K, rows, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_quantizer_with_many_groups_per_warp(dtype):
+    from llada_quant_b200.fp8 import quantize_fp8
+    x = values(1200, 4104, dtype, 9)  # 39600 groups, and a tail of 8 in every row
+    same_bits(quantize_fp8(x), *plain_quantize(x, 1))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("rows", [1, 128])
 def test_quantizer_at_the_ends_of_the_range(rows):
     """Zeros, the smallest and largest numbers, exact ties, NaN and infinities; each in rows of its own."""
@@ -176,6 +184,33 @@ def test_product_of_values(M, N, K, dtype):
     out = Fp8Linear.from_codes(w, bias, dtype)(x)
     q = quantize_fp8(x)
     check_product(out, q.codes, q.scale, w, bias)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M,N,K", [(1, 130, 16384), (2, 1000, 16400), (8, 4500, 1040), (16, 2050, 2048), (24, 4352, 4096)])
+def test_product_on_either_side_of_each_choice(M, N, K):
+    """Rows quantized by the product or before it; few rows with a large weight."""
+    from llada_quant_b200.fp8 import fp8_linear, quantize_fp8
+    x, w = values(M, K, torch.bfloat16, M), quantize_fp8(values(N, K, torch.float32, N + 1) * 0.05, 128)
+    q = quantize_fp8(x)
+    check_product(fp8_linear(x, w), q.codes, q.scale, w)
+    check_product(fp8_linear(q, w, out_dtype=torch.float32), q.codes, q.scale, w)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("N", [5000, 5003])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_product_with_many_tiles_per_sm(N, dtype):
+    """Three waves of the widest tile, the last of every row partly or wholly behind N; rows that are 16-byte aligned or not."""
+    from llada_quant_b200 import ops
+    from llada_quant_b200.fp8 import fp8_linear, quantize_fp8
+    w = quantize_fp8(values(N, 400, torch.float32, 2) * 0.05, 128)
+    q = quantize_fp8(values(2500, 400, torch.bfloat16, 1))
+    bias = values(1, N, dtype, 3)[0]
+    out = fp8_linear(q, w, bias, dtype)
+    check_product(out, q.codes, q.scale, w, bias)
+    assert torch.equal(fp8_linear(q, w, bias, dtype), out)
+    assert ops.device_error() == 0
 
 
 @pytest.mark.gpu
