@@ -14,9 +14,12 @@
 //   warps 2, 3  bring the rows' scales to shared memory: as loads of the epilogue's threads, one line each, they held up
 //               its waits and took as many cycles as its sums
 //   warps 4-11  epilogue: one TMEM lane quarter each, half of the columns; BN / 2 sums per thread
-// What bounds a large product is this epilogue: 128 x BN sums per 128 of K leave TMEM and pass the FMA pipe (256
-// cycles at BN = 256; as fma.rn.f32x2 it took three instructions a pair) while the tensor core needs 512 cycles for
-// 128 x 256 x 128.  So a thread asks for its next 32 columns before it adds the last, which takes 216 registers at BN = 256.
+// What bounds a large product is the chain of these hand-overs: of about 950 cycles that 128 x 256 x 128 takes, the tensor
+// core works 510 and the epilogue's threads 600 (its reads of TMEM and its 128 sums are 256 each), and they overlap
+// only as far as two accumulator buffers let them.  So a thread asks for its next 32 columns before it adds the last,
+// which takes 216 registers at BN = 256.  8192 x 8192 x 2048: 140 us, 1.96 PFLOP/s.  Tried and not better: fma.rn.f32x2
+// for the sums (three instructions a pair, 176 us against 170 then), three column parts of 64 at BN = 192 (147 against 136), a pair of
+// CTAs on 256 x 256 (cta_group::2, 130 against 136, and 21 against 19.9 at 1024 x 4096 x 4096).
 // Persistent over tiles when K is not split.  When the tiles do not cover the SMs, a cluster of `split`
 // CTAs shares one tile, each takes a part of K, and the parts meet in distributed shared memory and are
 // added in rank order.
@@ -146,6 +149,23 @@ __device__ __forceinline__ uint4 pack_out(const float* v, O o) {
   return make_uint4(pack2(v[0], v[1], o), pack2(v[2], v[3], o), pack2(v[4], v[5], o), pack2(v[6], v[7], o));
 }
 
+// A wait that polls: each 128 of K runs through a chain of commit, epilogue, release and issue, and waking from a long
+// suspension is part of it (256 x 8192 x 2048 9.9 us suspended, 9.0 polled; 8192 x 8192 x 2048 140 both).
+__device__ __forceinline__ bool poll(uint64_t* b, uint32_t parity, volatile int* abort_flag, int code) {
+  const long long t0 = clock64();
+  for (int n = 1; !mbar_try_wait(b, parity); ++n) {
+    if ((n & 255) == 0) {
+      if (*abort_flag) return false;
+      if (clock64() - t0 > kTimeoutCycles) {
+        *abort_flag = 1;
+        atomicExch(&g_device_error, code);
+        return false;
+      }
+    }
+  }
+  return true;
+}
+
 template <int BN, typename O>
 __global__ void __launch_bounds__(F8Cfg<BN>::THREADS, 1)
     fp8_tc_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w,
@@ -234,8 +254,8 @@ __global__ void __launch_bounds__(F8Cfg<BN>::THREADS, 1)
     bool ok = true;
     for (int u = blockIdx.x / a.split; u < a.tiles && ok; u += stride) {
       for (int g = g0; g < g1; ++g) {
-        if (!mbar_wait(&full[rs], ph, abort_flag, 0x520 + rs)) { ok = false; break; }
-        if (!mbar_wait(&acc_empty[ab], aph ^ 1, abort_flag, 0x510 + ab)) { ok = false; break; }
+        if (!poll(&full[rs], ph, abort_flag, 0x520 + rs)) { ok = false; break; }
+        if (!poll(&acc_empty[ab], aph ^ 1, abort_flag, 0x510 + ab)) { ok = false; break; }
         tc_fence_after();
         const uint64_t ad = make_sdesc(smem_u32(smem + rs * C::STAGE_BYTES));
         const uint64_t bd = make_sdesc(smem_u32(smem + rs * C::STAGE_BYTES + C::A_BYTES));
@@ -308,7 +328,7 @@ __global__ void __launch_bounds__(F8Cfg<BN>::THREADS, 1)
       for (int g = g0; g < g1; ++g) {
         const float sw = next;
         if (g + 1 < g1) next = load_ahead(ws + g + 1);
-        if (!mbar_wait(&acc_full[ab], aph, abort_flag, 0x530 + ab)) { ok = false; break; }
+        if (!poll(&acc_full[ab], aph, abort_flag, 0x530 + ab)) { ok = false; break; }
         tc_fence_after();
         constexpr int CH = C::COLS / 32;
         const uint32_t at = lane_addr + ab * BN;
