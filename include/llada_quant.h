@@ -375,7 +375,8 @@ int llq_fp8_quantize(const void* x, int x_dtype, int64_t M, int64_t K, int64_t l
  * block_rows == 1.  w e4m3 [N, K] with w_scale [ceil(N / 128), G] from
  * block_rows == 128; bias [N] of out_dtype or NULL.  Row strides ldx (elements)
  * and ldw; e4m3 operands need 16-byte aligned bases and pitches.  K a multiple
- * of 16.  The products of two scales and their sums must stay finite in fp32.
+ * of 16, at most 2^30.  The products of two scales and their sums must stay
+ * finite in fp32.
  * workspace: llq_fp8_linear_workspace_size bytes (may be 0 and NULL), of this
  * call alone until it is done on the stream.
  */

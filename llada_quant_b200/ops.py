@@ -635,8 +635,11 @@ def _moe_few_impl(x: torch.Tensor, gate_w: torch.Tensor, bias: Optional[torch.Te
                   bits: int) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
     """Router + routed experts on PACKED weights for at most 32 tokens, two launches ->
     (out bf16 [T,H], topk_w f32 [T,k], topk_ids i32 [T,k], logits f32 [T,E])."""
-    layer = few_layer(qw1, sw1, qw2, sw2, k, bits, gate_w.contiguous(),
-                      None if bias is None else bias.contiguous().to(torch.float32), renormalize)
+    _need_cuda(gate_w, bias)
+    _no_grad_through("the few-token layer", gate_w, bias)
+    gate_w = _aligned(gate_w)  # (held until the call: the layer has their addresses)
+    bias = None if bias is None else bias.contiguous().to(torch.float32)
+    layer = few_layer(qw1, sw1, qw2, sw2, k, bits, gate_w, bias, renormalize)
     x = few_rows(x, layer.H, qw1.device)
     T = x.shape[0]
     tw = torch.empty(T, k, dtype=torch.float32, device=x.device)

@@ -270,6 +270,26 @@ def test_moe_layer_and_fused_moe_reach_it():
 
 
 @pytest.mark.gpu
+def test_copied_router_operands_live_until_the_call():
+    """gate_w and bias that have to be copied: the copies' memory is not given to the call's own tensors."""
+    from llada_quant_b200.fused_moe import moe_layer
+    layer, x, gate, _, _ = make_layer(9, 16, 512, 256, 4, 4, 128)
+    p = packed_of(layer, 128)
+    bias = (torch.arange(16, device="cuda") / 8).to(torch.bfloat16)  # exact in bf16
+    wide = torch.zeros(16, 1031, dtype=torch.bfloat16, device="cuda")
+    wide[:, 3:515] = gate
+    flat = torch.zeros(16 * 512 + 3, dtype=torch.bfloat16, device="cuda")
+    flat[3:] = gate.reshape(-1)
+    want = moe_layer(x, gate, p, 4, bias.float(), impl="few")
+    torch.cuda.synchronize()
+    for g in (gate, gate.t().contiguous().t(), wide[:, 3:515], flat[3:].view(16, 512)):
+        for _ in range(3):
+            assert torch.equal(moe_layer(x, g, p, 4, bias, impl="few"), want)
+    with pytest.raises(RuntimeError, match="no backward pass"):
+        moe_layer(x, gate.clone().requires_grad_(), p, 4, impl="few")
+
+
+@pytest.mark.gpu
 def test_captured_replayed_and_on_two_streams_at_once():
     from llada_quant_b200.few_tokens import FewTokenMoE
     layer, x, gate, _, _ = make_layer(9, 16, 512, 256, 4, 4, 128)

@@ -352,6 +352,8 @@ def test_c_refusals_need_no_gpu():
                            (dict(K=120), _lib.LLQ_EUNSUPPORTED, b"multiples of 16"), (dict(ldw=136), _lib.LLQ_EINVAL, b"16-byte"),
                            (dict(w=8), _lib.LLQ_EINVAL, b"16-byte"), (dict(xs=None), _lib.LLQ_EINVAL, b"scales"),
                            (dict(ldx=136), _lib.LLQ_EINVAL, b"16-byte"), (dict(dt=9), _lib.LLQ_EUNSUPPORTED, b"dtype"),
+                           (dict(K=2 ** 30 + 16, ldx=2 ** 31, ldw=2 ** 31), _lib.LLQ_EINVAL, b"K too large"),
+                           (dict(dt=_lib.LLQ_BF16, M=17, xs=None), _lib.LLQ_ENOSPACE, b"workspace"),
                            (dict(out=None), _lib.LLQ_EINVAL, b"null")):
         rc, msg = lin(**kw)
         assert rc == code and text in msg, (kw, msg)
