@@ -46,7 +46,7 @@ struct Divider {
   }
   __device__ __forceinline__ float operator()(float v) const {
     const float n = __fmul_rn(v, 0.4375f), q = __fmul_rn(n, r);
-    return copysignf(__fmaf_rn(__fmaf_rn(-q, a, n), r, q), v);  // (the correction makes +0 of -0)
+    return __fmaf_rn(-__fmaf_rn(q, a, -n), r, q);  // (so written it keeps the sign of a zero)
   }
 };
 
@@ -134,9 +134,13 @@ struct Raw16 {
       for (int i = 0; i < 16; ++i) m = max(m, w[i] & 0x7fffffffu);
       return m;
     }
+    using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) m = __vmaxu2(m, w[i] & 0x7fff7fffu);  // halves order as magnitudes too
-    const uint32_t t = max(m >> 16, m & 0xffffu);
+    for (int i = 0; i < 8; ++i) {
+      const T2 v = __hmax2_nan(__habs2(*reinterpret_cast<const T2*>(&w[i])), *reinterpret_cast<const T2*>(&m));
+      m = *reinterpret_cast<const uint32_t*>(&v);
+    }
+    const uint32_t t = max(m >> 16, m & 0xffffu);  // (patterns order as magnitudes, NaN above all)
     return std::is_same<T, __half>::value ? __float_as_uint(__half2float(__ushort_as_half(static_cast<uint16_t>(t)))) : t << 16;
   }
 
