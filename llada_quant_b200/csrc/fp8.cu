@@ -58,8 +58,8 @@ __device__ __forceinline__ uint16_t to_e4m3x2(float lo, float hi) {
 }
 
 // The codes of N values of type T of a group: e4m3 of ratio(v).  (A division for each value took 42 us at 8192 x 4096
-// bf16 where this took 28, and a test for borders with the division behind it 50: a quarter of all groups of bf16 values
-// has some on one.)
+// bf16 where this took 28 then, and a test for borders with the division behind it 50: a quarter of all groups of bf16
+// values has some on one.)
 template <typename T, int N>
 __device__ __forceinline__ void quantize_values(const float (&v)[N], float amax, const Divider& div, uint16_t (&q)[N / 2]) {
   uint32_t differ = 0;
@@ -178,14 +178,15 @@ struct Raw16 {
   }
 };
 
-// One scale per 128 values of a row: 8 lanes hold a group, 16 values each.  I: 32-bit indices of groups where they fit
-// (a 64-bit division per group took as long as all the rest).  It has to read 2 (4) bytes a value and write 1; what holds
-// it below the memory's rate is that a warp computes while it has no load under way, so many warps are needed:
-// 8192 x 4096 bf16 takes 21.8 us at 6 CTAs per SM (4.7 TB/s), 23.6 at 4, 26.7 at 3 and 22.7 at 8, where registers spill;
-// asking for the next group ahead took 25.8.  fp32: 32.5 us at 4 CTAs (5.2 TB/s).
+// One scale per 128 values of a row: 8 lanes hold a group, 16 values each.  I: 32-bit indices of groups where they fit.
+// It has to read 2 (4) bytes a value and write 1; what holds it below the memory's rate is that a warp computes while it
+// has no load under way, about 6 instructions a value, so many warps and few instructions are wanted: 8192 x 4096 bf16
+// takes 18.4 us at 6 CTAs per SM (5.5 TB/s), 19.1 at 5 and 19.7 at 7; with a division per group for its row 19.6, and asking for the
+// next group ahead took 25.8 where this took 21.8.  fp32: 28.8 us at 5 CTAs (5.8 TB/s), 30.0 at 4, 31.6 at 6.
 template <typename T>
-constexpr int kRowsBlocks = sizeof(T) == 4 ? 4 : 6;
-// the same for blocks of 128 rows: 4096 x 8192 bf16 20.2 us at 4 CTAs per SM (5.0 TB/s), 23.9 at 5, 26.9 at 6, 21.3 at 3
+constexpr int kRowsBlocks = sizeof(T) == 4 ? 5 : 6;
+// the same for blocks of 128 rows: 4096 x 8192 bf16 18.7 us at 4 CTAs per SM (5.4 TB/s); before the values took fewer
+// instructions 20.2, and then 23.9 at 5, 26.9 at 6 and 21.3 at 3
 template <typename T>
 constexpr int kBlocksBlocks = sizeof(T) == 4 ? 2 : 4;
 
@@ -197,12 +198,13 @@ __global__ void __launch_bounds__(256, kRowsBlocks<T>) fp8_rows_kernel(const T* 
   const int l = threadIdx.x & 7;
   const I stride = static_cast<I>(gridDim.x) * (blockDim.x >> 3);
   const I i0 = static_cast<I>(blockIdx.x) * (blockDim.x >> 3) + (threadIdx.x >> 3);
+  const I rows = stride / G, rest = stride - rows * G;
+  I m = i0 / G, g = i0 - m * G;  // group g of row m
 #pragma unroll 1
   for (I i = i0; i - (threadIdx.x >> 3 & 3) < n; i += stride) {  // a warp's four groups leave the loop together
-    const I m = i < n ? i / G : 0;
-    const int64_t c = i < n ? static_cast<int64_t>(i - m * G) * BLK + 16 * l : K;
+    const int64_t c = i < n ? static_cast<int64_t>(g) * BLK + 16 * l : K;
     Raw16<T> raw;
-    raw.load(x + static_cast<int64_t>(m) * ldx, c, K, vec != 0);
+    raw.load(x + (i < n ? static_cast<int64_t>(m) * ldx : 0), c, K, vec != 0);
     uint32_t b = raw.top();
 #pragma unroll
     for (int o = 4; o > 0; o >>= 1) b = max(b, __shfl_xor_sync(0xffffffffu, b, o));
@@ -211,6 +213,12 @@ __global__ void __launch_bounds__(256, kRowsBlocks<T>) fp8_rows_kernel(const T* 
     raw.codes(amax, Divider(amax), w);
     store16(codes + static_cast<int64_t>(m) * ldc, c, K, w);
     if (l == 0 && i < n) scale[i] = group_scale(amax);
+    m += rows;
+    g += rest;
+    if (g >= G) {
+      g -= G;
+      ++m;
+    }
   }
 }
 
