@@ -499,11 +499,12 @@ int fp8_quantize(const void* x, int x_dtype, int64_t M, int64_t K, int64_t ldx, 
   return fail(LLQ_EUNSUPPORTED, "unknown dtype %d", x_dtype);
 }
 
-// Does the product run on fp8_few_rows_kernel (else on fp8_tc_kernel)?  Up to 16 rows it always won (16 x 2048 x 2048 3.1 us
-// against 7.9, 16 x 8192 x 4096 11.9 against 16.3); with 32, where every CTA reads
-// more of x than of the weight, only small weights are faster there (32 x 4096 x 2048 6.5 us against 10.5, 32 x 4096 x 4096
-// 10.6 against 11.9, 32 x 8192 x 4096 18.5 against 14.0).
-static bool few_rows(int64_t M, int64_t K, int64_t N) { return M <= 16 || (M <= 32 && N * K <= 1 << 24); }
+// Does the product run on fp8_few_rows_kernel (else on fp8_tc_kernel)?  Up to 16 rows it is faster, or as fast with large
+// weights (us: 8 x 2048 x 2048 2.4 against 6.4, 8 x 8192 x 4096 9.0 against 11, 16 x 4096 x 4096 6.9 against 10.3, 16 x 8192 x 4096 12.0
+// against 11.0, 16 x 4096 x 14336 17.2 against 18.2); with 32, where a CTA reads more of x than of the weight, for few
+// and small weight rows (32 x 2048 x 2048 4.4 against 6.4, 32 x 2048 x 4096 7.2 against 8.1, 32 x 4096 x 2048 6.7 against 6.4, 32 x
+// 8192 x 1024 7.9 against 4.7, 32 x 8192 x 4096 18.5 against 11.0).
+static bool few_rows(int64_t M, int64_t K, int64_t N) { return M <= 16 || (M <= 32 && N <= 4096 && N * K <= 1 << 24); }
 
 // Do its CTAs quantize the rows for themselves?  Each does all of them again, N / 16 times together, which beats a launch for
 // few values (1 x 1024 x 1024 2.2 us against 3.1, 8 x 2048 x 2048 4.0 against 4.2, 1 x 3000 x 7168 9.1 against 10.1) and not

@@ -70,6 +70,7 @@ struct F8Args {
   int mtiles, tiles;
   int split;
   int tma_out;       // rows of out are 16-byte aligned
+  int box;           // rows of x that a copy brings
 };
 
 // instruction descriptor of kind::f8f6f4: D f32, A and B e4m3 (0), both K-major
@@ -228,7 +229,7 @@ __global__ void __launch_bounds__(F8Cfg<BN>::THREADS, 1)
         const int m0 = u % a.mtiles * BM, n0 = u / a.mtiles * BN;
         for (int g = g0; g < g1; ++g) {
           if (!mbar_wait(&empty[rs], ph ^ 1, abort_flag, 0x500 + rs)) { ok = false; break; }
-          mbar_expect_tx(&full[rs], C::STAGE_BYTES);
+          mbar_expect_tx(&full[rs], a.box * BK + BN * BK);
           uint8_t* dst = smem + rs * C::STAGE_BYTES;
           tma_load_2d(dst, &tm_x, g * BK, m0, &full[rs]);
           tma_load_2d(dst + C::A_BYTES, &tm_w, g * BK, n0, &full[rs]);
@@ -457,7 +458,7 @@ int launch_tc(const Fp8Operands& p, const F8Args& in, CUtensorMapDataType ot, cu
   using C = F8Cfg<BN>;
   F8Args a = in;
   CUtensorMap tx, tw, to;
-  int rc = make_map(&tx, p.x, CU_TENSOR_MAP_DATA_TYPE_UINT8, p.K, p.M, p.ldx, BK, BM, CU_TENSOR_MAP_SWIZZLE_128B);
+  int rc = make_map(&tx, p.x, CU_TENSOR_MAP_DATA_TYPE_UINT8, p.K, p.M, p.ldx, BK, a.box, CU_TENSOR_MAP_SWIZZLE_128B);
   if (rc) return rc;
   rc = make_map(&tw, p.w, CU_TENSOR_MAP_DATA_TYPE_UINT8, p.K, p.N, p.ldw, BK, BN, CU_TENSOR_MAP_SWIZZLE_128B);
   if (rc) return rc;
@@ -518,18 +519,21 @@ int fp8_gemm_tc(const Fp8Operands& p, cudaStream_t st) {
   const int64_t mt = (p.M + BM - 1) / BM;
   const int sms = num_sms();
   auto tiles = [&](int bn) { return mt * ((p.N + bn - 1) / bn); };
-  // Tile width and K split by the bytes that the busiest SM brings from L2: waves x blocks of K x (128 + BN) rows of 128
-  // bytes; a split costs about as much as 1500 such rows, and its clusters must fit at once (148 SMs hold 132 CTAs in
-  // clusters of four, 120 in clusters of eight).  Measured with each width forced (256 / 128 / 64, us): 256 x 8192 x 2048
-  // 13.1 / 9.8 / 16.3, 1024 x 4096 x 4096 24.2 / 26.3 / 46.1, 64 x 8192 x 2048 12.2 / 11.0 / 10.0; without a split
-  // 256 x 2048 x 8192 takes 22.4 instead of 14.6 and 512 x 1000 x 7168 20.6 instead of 13.5.
+  // Tile width and K split by an estimate in ns, fitted to sweeps with each forced: the start, then per 128 of K the chain of
+  // hand-overs or the bytes that all CTAs together bring from L2 (13.6 TB/s), whichever is longer, and for a split the
+  // cluster's start and the exchange of the parts.  Its clusters must fit at once (148 SMs hold 132 CTAs in clusters of
+  // four, 120 in clusters of eight).  Measured (us): 64 wide 48 x 2048 x 2048 6.5 whole, 7.6 in two, 7.8 in four; 64 x 2048 x 4096
+  // 10.2, 9.5, 8.2; 48 x 1024 x 8192 17.2, 13.0, 9.6; 256 x 8192 x 2048 256 wide 13.1, 128 wide 9.0, 64 wide 16; 1024 x 4096 x
+  // 4096 19.6, 26.3, 46.
   int bn = 64, split = 1;
   int64_t best = INT64_MAX;
   for (int w : {256, 128, 64}) {
-    for (int sp : {1, 2, 4, 8}) {
+    const int64_t start = w == 64 ? 2800 : w == 128 ? 3400 : 4000, chain = w == 64 ? 235 : w == 128 ? 260 : 600;
+    for (int sp = 1, exchange = 0; sp <= 8; sp *= 2, exchange = (exchange == 0 ? (w == 64 ? 2000 : 3000) : exchange) + 750) {
       const int room = sp == 8 ? sms * 120 / 148 : sp == 4 ? sms * 132 / 148 : sms;
       if (sp > 1 && (tiles(w) * sp > room || sp * 2 > p.G || w == 256)) break;
-      const int64_t cost = (tiles(w) + sms - 1) / sms * ((p.G + sp - 1) / sp) * (BM + w) + (sp > 1 ? 1500 : 0);
+      const int64_t at_once = std::min<int64_t>(tiles(w) * sp, sms), waves = (tiles(w) * sp + sms - 1) / sms;
+      const int64_t cost = start + exchange + waves * ((p.G + sp - 1) / sp) * std::max(chain, (BM + w) * BK * at_once / 13600);
       if (cost < best) {
         best = cost;
         bn = w;
@@ -549,6 +553,9 @@ int fp8_gemm_tc(const Fp8Operands& p, cudaStream_t st) {
   a.mtiles = static_cast<int>(mt);
   a.tiles = static_cast<int>(tiles(bn));
   a.split = split;
+  // with fewer rows than a tile has, the copies bring these alone (the other lanes' sums are not stored): filling the rest
+  // with zeros cost 15.0 us against 11.0 at 16 x 8192 x 4096, 12.2 against 10.3 at 24 x 4096 x 4096
+  a.box = static_cast<int>(std::min<int64_t>(BM, (p.M + 7) / 8 * 8));
   return bn == 256 ? launch_out<256>(p, a, st) : bn == 128 ? launch_out<128>(p, a, st) : launch_out<64>(p, a, st);
 }
 
