@@ -318,8 +318,8 @@ struct Codes {};  // tag: x holds e4m3 codes
 // exact and sums are fp32.  The order of K within a group is free as long as both sides agree: lane t of a quad
 // has bytes 16 t and 64 + 16 t of a group's 128, so that a quad reads 64 bytes at once.
 // T other than Codes (NB = 1): every CTA quantizes the rows for itself into shared memory, which saves a launch.
-// The weight's bytes bound it: 8 x 8192 x 4096 takes 9.1 us (3.7 TB/s; 8 warps 8.5), 8 x 4096 x 14336 12.5 (4.7 TB/s; 8 warps
-// 16.2), 8 x 2048 x 2048 2.6 (8 warps 2.7), one token 2048 x 2048 with its quantization 2.8.
+// The weight's bytes bound it, with a start of about 2 us: 8 x 8192 x 4096 takes 8.6 us (3.9 TB/s), 8 x 4096 x 14336 12.5 (4.7
+// TB/s), one token 2048 x 2048 with its quantization 2.7.
 template <int W, int NB>
 constexpr int kFewRed = W * 16 * (NB * 8 + 1) * 4;
 
@@ -453,6 +453,15 @@ int launch_few(const LinArgs& a, cudaStream_t st) {
   return check_launch("fp8_few_rows_kernel");
 }
 
+// Up to 8 rows.  16 warps share a CTA's 16 weight rows, two CTAs per SM; where these do not fit at once, 8 warps and four CTAs (us,
+// 16 warps / 8 warps: 8 x 2048 x 2048 2.6 / 2.7, 8 x 4096 x 14336 12.5 / 16.2, 8 x 5120 x 4096 7.5 / 6.9, 8 x 16384 x 2048 10.6 / 9.2,
+// 1 x 8192 x 2048 with its quantization 7.3 / 5.9).
+template <typename T>
+int launch_eight(const LinArgs& a, cudaStream_t st) {
+  if (a.N > 32 * num_sms()) return launch_few<T, 8, 1, 4>(a, st);
+  return launch_few<T, 16, 1, 2>(a, st);
+}
+
 template <typename T>
 int launch_rows(const void* x, int64_t M, int64_t K, int64_t ldx, int block_rows, uint8_t* codes, int64_t ldc, float* scale,
                 cudaStream_t st) {
@@ -500,7 +509,7 @@ int fp8_quantize(const void* x, int x_dtype, int64_t M, int64_t K, int64_t ldx, 
 }
 
 // Does the product run on fp8_few_rows_kernel (else on fp8_tc_kernel)?  Up to 16 rows it is faster, or as fast with large
-// weights (us: 8 x 2048 x 2048 2.4 against 6.4, 8 x 8192 x 4096 9.0 against 11, 16 x 4096 x 4096 6.9 against 10.3, 16 x 8192 x 4096 12.0
+// weights (us: 8 x 2048 x 2048 2.4 against 6.4, 8 x 8192 x 4096 8.6 against 11, 16 x 4096 x 4096 6.9 against 10.3, 16 x 8192 x 4096 12.0
 // against 11.0, 16 x 4096 x 14336 17.2 against 18.2); with 32, where a CTA reads more of x than of the weight, for few
 // and small weight rows (32 x 2048 x 2048 4.4 against 6.4, 32 x 2048 x 4096 7.2 against 8.1, 32 x 4096 x 2048 6.7 against 6.4, 32 x
 // 8192 x 1024 7.9 against 4.7, 32 x 8192 x 4096 18.5 against 11.0).
@@ -508,7 +517,7 @@ static bool few_rows(int64_t M, int64_t K, int64_t N) { return M <= 16 || (M <= 
 
 // Do its CTAs quantize the rows for themselves?  Each does all of them again, N / 16 times together, which beats a launch for
 // few values (1 x 1024 x 1024 2.2 us against 3.1, 8 x 2048 x 2048 4.0 against 4.2, 1 x 3000 x 7168 9.1 against 10.1) and not
-// for many (1 x 8192 x 4096 10.7 against 9.7, 8 x 8192 x 4096 20.0 against 10.0).
+// for many (1 x 8192 x 4096 9.4 against 9.5, 8 x 8192 x 4096 20.0 against 10.0).
 static bool few_quantizes(int64_t M, int64_t K, int64_t N) {
   return M <= 8 && K <= kOwnK && M * K * ((N + 15) / 16) <= 1 << 21;
 }
@@ -585,12 +594,12 @@ int fp8_linear(const void* x, int x_dtype, const float* x_scale, int64_t M, int 
   if (!own) {
     if (M > 16) return launch_few<Codes, 8, 4, 2>(a, st);
     if (M > 8) return launch_few<Codes, 8, 2, 2>(a, st);
-    return launch_few<Codes, 16, 1, 2>(a, st);
+    return launch_eight<Codes>(a, st);
   }
   switch (x_dtype) {
-    case LLQ_F32: return launch_few<float, 16, 1, 2>(a, st);
-    case LLQ_F16: return launch_few<__half, 16, 1, 2>(a, st);
-    default: return launch_few<__nv_bfloat16, 16, 1, 2>(a, st);
+    case LLQ_F32: return launch_eight<float>(a, st);
+    case LLQ_F16: return launch_eight<__half>(a, st);
+    default: return launch_eight<__nv_bfloat16>(a, st);
   }
 }
 

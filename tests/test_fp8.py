@@ -187,7 +187,8 @@ def test_product_of_values(M, N, K, dtype):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("M,N,K", [(1, 130, 16384), (2, 1000, 16400), (8, 4500, 1040), (16, 2050, 2048), (24, 4352, 4096)])
+@pytest.mark.parametrize("M,N,K", [(1, 130, 16384), (2, 1000, 16400), (8, 4500, 1040), (16, 2050, 2048), (24, 4352, 4096),
+                                   (8, 5001, 1040), (3, 9000, 144), (17, 5000, 512), (48, 300, 4096), (200, 512, 4096)])
 def test_product_on_either_side_of_each_choice(M, N, K):
     """Rows quantized by the product or before it; few rows with a large weight."""
     from llada_quant_b200.fp8 import fp8_linear, quantize_fp8
