@@ -136,6 +136,9 @@ class Fp8Linear(nn.Module):
     def extra_repr(self) -> str:
         return f"{self.in_features} -> {self.out_features}, e4m3 codes, blocks of {BLOCK}"
 
+    def __getstate__(self):
+        return {**self.__dict__, "_ready": None}  # addresses do not outlive the object
+
     def _multiplier(self) -> ops.Fp8Weight:
         """The checked operand of the buffers as they are now (checked again when one was replaced)."""
         b, r = self._buffers, self._ready

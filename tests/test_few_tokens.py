@@ -270,6 +270,33 @@ def test_moe_layer_and_fused_moe_reach_it():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("T,bits,E", [(1, 8, 40), (32, 8, 40), (32, 4, 3)])
+def test_the_longest_rows_and_offsets_beyond_32_bits(T, bits, E):
+    """H = I = 8192; with 40 INT8 experts w1 has 5.4 GB, and the tokens choose the last experts."""
+    from llada_quant_b200.few_tokens import FewTokenMoE
+    H = I = 8192
+    per = 2 if bits == 4 else 1
+    g = torch.Generator("cuda").manual_seed(T + bits)
+    q1 = torch.randint(-128, 128, (E, 2 * I, H // per), generator=g, device="cuda", dtype=torch.int8)
+    q2 = torch.randint(-128, 128, (E, H, I // per), generator=g, device="cuda", dtype=torch.int8)
+    s1 = torch.rand(E, 2 * I, H // 128, generator=g, device="cuda") * 1e-4
+    s2 = torch.rand(E, H, I // 128, generator=g, device="cuda") * 1e-4
+    layer = (q1, s1, q2, s2, bits)
+    x = torch.randn(T, H, generator=g, device="cuda").to(torch.bfloat16)
+    ids = (E - 1 - torch.arange(2, device="cuda", dtype=torch.int32)).repeat(T, 1)
+    ids[T // 2:, 1] = E
+    weights = torch.rand(T, 2, generator=g, device="cuda")
+    gate = (torch.randn(E, H, generator=g, device="cuda") * 0.02).to(torch.bfloat16)
+    bias = torch.full((E,), -torch.inf, device="cuda")
+    bias[E - 2:] = 0
+    moe = FewTokenMoE(packed_of(layer, 128), gate, 2, bias)
+    check(moe.routed(x, weights, ids), x, layer, weights, ids)
+    out, w, ids = moe(x)
+    assert bool((ids >= E - 2).all())
+    check(out, x, layer, w, ids)
+
+
+@pytest.mark.gpu
 def test_copied_router_operands_live_until_the_call():
     """gate_w and bias that have to be copied: the copies' memory is not given to the call's own tensors."""
     from llada_quant_b200.fused_moe import moe_layer

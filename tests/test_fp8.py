@@ -215,6 +215,24 @@ def test_product_with_many_tiles_per_sm(N, dtype):
 
 
 @pytest.mark.gpu
+def test_offsets_beyond_32_bits():
+    """2.2 G values in and out: the last rows equal a call of their own."""
+    from llada_quant_b200.fp8 import Fp8Tensor, fp8_linear, quantize_fp8
+    rows = values(300, 32768, torch.bfloat16, 1)
+    x = rows.repeat(220, 1)  # 66000 x 32768
+    for r in (1, 128):
+        q, part = quantize_fp8(x, r), quantize_fp8(rows[-80:], r)  # (66000 = 515 * 128 + 80)
+        assert torch.equal(q.codes.view(torch.uint8)[-80:], part.codes.view(torch.uint8))
+        assert torch.equal(q.scale[-part.scale.shape[0]:], part.scale)
+        del q
+    del x
+    q = quantize_fp8(values(66000, 128, torch.bfloat16, 2))
+    w = quantize_fp8(values(33024, 128, torch.float32, 3) * 0.05, 128)
+    last = Fp8Tensor(q.codes[-80:], q.scale[-80:], 1)
+    assert torch.equal(fp8_linear(q, w)[-80:], fp8_linear(last, w))
+
+
+@pytest.mark.gpu
 def test_linear_module_against_the_layer_it_replaces():
     from llada_quant_b200.fp8 import Fp8Linear
     g = torch.Generator().manual_seed(5)
@@ -241,6 +259,26 @@ def test_linear_module_against_the_layer_it_replaces():
         other(x)
     assert m.storage_bytes() == 520 * 1024 + 5 * 8 * 4 + 520 * 2
     assert torch.equal(m(x[:, :0]), y[:, :0])
+
+
+@pytest.mark.gpu
+def test_linear_module_copied_pickled_and_changed_in_place():
+    import copy
+    import io
+    from llada_quant_b200.fp8 import Fp8Linear, quantize_fp8
+    m = Fp8Linear.from_codes(quantize_fp8(values(200, 256, torch.float32, 1), 128), values(1, 200, torch.bfloat16, 2)[0])
+    x = values(5, 256, torch.bfloat16, 3)
+    y = m(x)
+    twin, file = copy.deepcopy(m), io.BytesIO()
+    torch.save(m, file)
+    file.seek(0)
+    for other in (twin, torch.load(file, weights_only=False)):
+        assert other.qweight.data_ptr() != m.qweight.data_ptr() and torch.equal(other(x), y)
+    twin.scale.mul_(2)
+    twin.bias.mul_(2)
+    assert torch.equal(twin(x), y * 2) and torch.equal(m(x), y)
+    twin.qweight = m.qweight.clone().zero_()
+    assert torch.equal(twin(x), twin.bias.expand(5, 200))
 
 
 @pytest.mark.gpu
