@@ -23,8 +23,6 @@ __device__ __forceinline__ float group_amax(uint32_t bits) {
   return m < kAmaxFloor ? kAmaxFloor : m;
 }
 
-__device__ __forceinline__ uint32_t mag(float v) { return __float_as_uint(v) & 0x7fffffffu; }
-
 __device__ __forceinline__ float group_scale(float amax) { return __fdiv_rn(amax, 448.f); }
 
 // v * 448 / amax, correctly rounded in fp32; 448 = 0.4375 * 2^10, so that no product overflows
@@ -129,19 +127,20 @@ struct Raw16 {
   // the largest magnitude's bits as fp32
   __device__ __forceinline__ uint32_t top() const {
     uint32_t m = 0;
-    if (sizeof(T) == 4) {
+    if constexpr (sizeof(T) == 4) {
 #pragma unroll
       for (int i = 0; i < 16; ++i) m = max(m, w[i] & 0x7fffffffu);
       return m;
-    }
-    using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+    } else {
+      using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const T2 v = __hmax2_nan(__habs2(*reinterpret_cast<const T2*>(&w[i])), *reinterpret_cast<const T2*>(&m));
-      m = *reinterpret_cast<const uint32_t*>(&v);
+      for (int i = 0; i < 8; ++i) {
+        const T2 v = __hmax2_nan(__habs2(*reinterpret_cast<const T2*>(&w[i])), *reinterpret_cast<const T2*>(&m));
+        m = *reinterpret_cast<const uint32_t*>(&v);
+      }
+      const uint32_t t = max(m >> 16, m & 0xffffu);  // (patterns order as magnitudes, NaN above all)
+      return std::is_same<T, __half>::value ? __float_as_uint(__half2float(__ushort_as_half(static_cast<uint16_t>(t)))) : t << 16;
     }
-    const uint32_t t = max(m >> 16, m & 0xffffu);  // (patterns order as magnitudes, NaN above all)
-    return std::is_same<T, __half>::value ? __float_as_uint(__half2float(__ushort_as_half(static_cast<uint16_t>(t)))) : t << 16;
   }
 
   // the codes under a group's largest magnitude
