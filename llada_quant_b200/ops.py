@@ -716,10 +716,9 @@ def _fp8_quantize_impl(x: torch.Tensor, block_rows: int) -> Tuple[torch.Tensor, 
     x = _fp8_values(x)
     M, K = x.shape
     pitch = -(-K // 16) * 16
-    codes = torch.empty(M, pitch, dtype=torch.float8_e4m3fn, device=x.device)
-    if pitch != K:
-        codes = codes[:, :K]
-    scale = torch.empty(-(-M // block_rows), -(-K // FP8_BLOCK), dtype=torch.float32, device=x.device)
+    device = x.device
+    codes = torch.empty_strided((M, K), (pitch, 1), dtype=torch.float8_e4m3fn, device=device)
+    scale = torch.empty(-(-M // block_rows), -(-K // FP8_BLOCK), dtype=torch.float32, device=device)
     rc = (_lib._lib or load()).llq_fp8_quantize(x.data_ptr(), kind, M, K, x.stride(0) if M > 1 else K, block_rows,
                                                 codes.data_ptr(), pitch, scale.data_ptr(), _raw_stream(x))
     if rc:
