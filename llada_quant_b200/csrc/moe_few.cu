@@ -1069,12 +1069,14 @@ __global__ void __launch_bounds__(THREADS2, 1)
     else __stcg(mine + i, v);
   }
   if (a.split == 1) return;
-  __threadfence();
   __syncthreads();
-  if (threadIdx.x == 0) sm.last = atomicAdd(&a.plan->done[panel], 1) == a.split - 1;
+  if (threadIdx.x == 0) {  // (its fences hold for what the CTA's threads stored before and load behind the barriers)
+    __threadfence();
+    sm.last = atomicAdd(&a.plan->done[panel], 1) == a.split - 1;
+    __threadfence();
+  }
   __syncthreads();
   if (!sm.last) return;
-  __threadfence();
   // the CTA that finishes last adds the CTAs' parts, again in the order of their steps
   const float4* all = reinterpret_cast<const float4*>(a.partial + static_cast<int64_t>(panel) * a.split * (PANEL * a.T));
   const int vecs = PANEL * a.T / 4;
