@@ -290,7 +290,7 @@ __device__ __forceinline__ uint32_t order_key(float z) {
 
 constexpr int MAX_DEPTH1 = 2;
 constexpr int SLOT1 = 4096;      // 16 gate and 16 up rows of 128 bytes (two steps at INT4, one at INT8): one copy
-constexpr int RED_SLICES = WARPS / 2;
+constexpr int RED_SLICES = (WARPS + 1) / 2;
 constexpr int RED_PITCH = MAX_T + 1;
 constexpr int RED_BYTES = RED_SLICES * 64 * RED_PITCH * 4;
 constexpr int ROUTER_BYTES = RED_BYTES + CL1 * MAX_EXP * MAX_T * 4;  // over the rings and tokens, before they are used
@@ -311,7 +311,7 @@ struct Smem1 {
 
 using LogitPart = float[MAX_T][MAX_EXP];
 
-// The router: K is split over the CTAs of the cluster and seven slices of warps in each; half of the warps take 32 of
+// The router: K is split over the CTAs of the cluster and eight slices of warps in each; half of the warps take 32 of
 // 64 experts at a time, the others the next 32.  A slice's sums meet in `red`, a CTA's in parts[rank] of both CTAs.
 template <int NT>  // tiles of 8 tokens
 __device__ void router_logits(const FewArgs& a, float (*red)[64][RED_PITCH], LogitPart* parts, cg::cluster_group& cluster) {
@@ -322,19 +322,20 @@ __device__ void router_logits(const FewArgs& a, float (*red)[64][RED_PITCH], Log
   const int p0 = pairs * rank / CL1, p1 = pairs * (rank + 1) / CL1;
 #pragma unroll 1
   for (int eg = 0; eg < a.E; eg += 64) {
-    if (warp < 2 * RED_SLICES) {
+    {
       float d[2][NT][4] = {};
       const __nv_bfloat16* w[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i)  // experts beyond the last read it and are not kept
         w[i] = a.gate + static_cast<int64_t>(min(eg + half * 32 + i * 8 + g, a.E - 1)) * a.H + 8 * t;
+      constexpr int CH = NT == 1 ? 4 : 2;  // chunks whose loads are under way together
 #pragma unroll 1
-      for (int p = p0 + slice; p < p1; p += RED_SLICES) {
-        uint4 u[2][4], x[2][NT];
+      for (int p = p0 + slice; p < p1; p += RED_SLICES * CH / 2) {
+        uint4 u[CH][4], x[CH][NT];
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          const int at = p * 64 + c * 32;
-          const bool in = at < a.H;
+        for (int c = 0; c < CH; ++c) {
+          const int q = p + c / 2 * RED_SLICES, at = q * 64 + c % 2 * 32;
+          const bool in = q < p1 && at < a.H;
 #pragma unroll
           for (int i = 0; i < 4; ++i)
             u[c][i] = in ? __ldg(reinterpret_cast<const uint4*>(w[i] + at)) : make_uint4(0, 0, 0, 0);
@@ -345,15 +346,13 @@ __device__ void router_logits(const FewArgs& a, float (*red)[64][RED_PITCH], Log
                                        : make_uint4(0, 0, 0, 0);
         }
 #pragma unroll
-        for (int c = 0; c < 2; ++c)
+        for (int c = 0; c < CH; ++c)
 #pragma unroll
           for (int n = 0; n < NT; ++n)
-            {
 #pragma unroll
-              for (int m = 0; m < 2; ++m) {
-                mma_bf16(d[m][n], u[c][2 * m].x, u[c][2 * m + 1].x, u[c][2 * m].y, u[c][2 * m + 1].y, x[c][n].x, x[c][n].y);
-                mma_bf16(d[m][n], u[c][2 * m].z, u[c][2 * m + 1].z, u[c][2 * m].w, u[c][2 * m + 1].w, x[c][n].z, x[c][n].w);
-              }
+            for (int m = 0; m < 2; ++m) {
+              mma_bf16(d[m][n], u[c][2 * m].x, u[c][2 * m + 1].x, u[c][2 * m].y, u[c][2 * m + 1].y, x[c][n].x, x[c][n].y);
+              mma_bf16(d[m][n], u[c][2 * m].z, u[c][2 * m + 1].z, u[c][2 * m].w, u[c][2 * m + 1].w, x[c][n].z, x[c][n].w);
             }
       }
 #pragma unroll
