@@ -875,7 +875,7 @@ struct Smem2 {
 };
 
 // GEMM2 and the combine.  The same layer: 20 us for 71 MB at 32 tokens (issue again: two MMAs for h's two parts), then 5 for
-// the parts; one token 3 and 4.  All of it: 32 tokens 81 us (INT8 105), one token 26 (INT8 31), 8 tokens INT8 with given
+// the parts; one token 3 and 4.  All of it: 32 tokens 81 us (INT8 105), one token 26 (INT8 30), 8 tokens INT8 with given
 // routing 67 (4.0 TB/s).
 template <int BITS, bool V4>
 __global__ void __launch_bounds__(THREADS2, 1)
