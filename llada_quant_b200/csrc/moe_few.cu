@@ -26,8 +26,8 @@
 // lost below is 2^-40 of it.  (fp16 rather than bf16 because its ten mantissa bits take an INT8 code, or
 // the upper nibble of a byte, where it lies: 40 instead of 56 logic instructions per lane and 128-group at
 // INT4, 48 instead of 96 at INT8; the logic pipe is what bounds the arithmetic.)  h travels between the
-// kernels as two bf16 numbers, hi + lo (16 significant bits).  So no MMA adds a visible rounding: the
-// layer rounds once, at its end.
+// kernels as three bf16 numbers that add up to the fp32 value (8 + 8 + 8 significant bits; the third is short only
+// where h lies below 2^-110).  So no MMA adds a visible rounding: the layer rounds once, at its end.
 //
 // The packed bytes and their scales reach shared memory by TMA (swizzled) into rings that are deep
 // enough for HBM's latency; the tokens lie in shared memory in MMA order.  Measured on the way
@@ -68,6 +68,12 @@ struct Segment {
   __device__ __forceinline__ int token(int c) const { return static_cast<int>(tokens >> (8 * c)) & 0xff; }
 };
 
+// Planes of 8 columns that the three parts of h of a segment of n tokens take: side by side in one with at most 2 tokens;
+// with 3 or 4 the first two in one and the third in another, behind it zeros; with more each in one of its own.
+__host__ __device__ __forceinline__ constexpr int planes_of(int n) { return n <= 2 ? 1 : n <= 4 ? 2 : 3; }
+// 16-byte pieces from the first part of a column to its part i (to the zeros where i is 3: n 3 or 4 alone)
+__device__ __forceinline__ int part_piece(int n, int i) { return n <= 2 ? 8 * i : n <= 4 ? (i >> 1) * 128 + (i & 1) * 16 : 128 * i; }
+
 // what kernel 1 tells kernel 2 about the routing
 struct FewPlan {
   Segment seg[MAX_SEG];
@@ -93,10 +99,11 @@ struct FewArgs {
   float* topk_w;
   int32_t* topk_ids;
   FewPlan* plan;
-  // [segment][step of I][plane][piece j of 4][lane], 4 KB a step: the B operand of kernel 2's MMAs.  Columns are the
-  // segment's tokens; plane 0 holds the hi parts, plane 1 the lo parts, but with at most 4 tokens the lo parts are
-  // columns 4 to 7 of plane 0 and half of the bytes and MMAs fall away.
+  // [segment][step of I][plane][piece j of 4][lane], 2 KB a plane: the B operand of kernel 2's MMAs.  Columns are the
+  // segment's tokens, a plane for each of h's three parts; with fewer tokens the parts share planes (part_piece), and
+  // bytes and MMAs fall away.
   uint4* h;
+  int planes;            // of a step in h: as many as a segment of min(T, 8) tokens has
   float* partial;        // [panel][split][128 features][T]
   int split;             // CTAs of a panel in kernel 2
   __nv_bfloat16* out;
@@ -468,35 +475,41 @@ __device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
 }
 
-// h of a finished job: features 16 rb and on of segment seg (a function of its own: it is called from two places)
+// h of a finished job: features 16 rb and on of segment seg.  (Inlined at both of its calls: called, with three parts, it
+// makes the compiler copy the arguments to each thread's stack, 3 us more for one token.)
 template <int BITS>
-__device__ __noinline__ void emit(const FewArgs& a, const Segment& sg, const float* col_w, int seg, int rb,
+__device__ __forceinline__ void emit(const FewArgs& a, const Segment& sg, const float* col_w, int seg, int rb,
                                   const float (&acc)[2][4]) {
   const int lane = threadIdx.x & 31, t = lane & 3, r = Codes<BITS>::row_of(lane >> 2);
-  const int hsteps = (a.I + KG - 1) / KG, ntok = sg.n;
-  const int lo = (ntok <= 4 ? 16 : 128);  // pieces from the hi to the lo parts: four columns, or a plane, further
+  const int hsteps = (a.I + KG - 1) / KG, ntok = sg.n, nparts = planes_of(ntok) == 2 ? 4 : 3;  // the fourth is zero
+  const int o1 = part_piece(ntok, 1) * 8, o2 = part_piece(ntok, 2) * 8;
 #pragma unroll
   for (int q = 0; q < 2; ++q) {
     // feature n of columns 2t and 2t + 1: its place in the 16 bytes of the 8 features from n - r on
     const int n = rb * 16 + q * 8 + r, s = n / KG, pt = (n % KG) / 32, pj = (n % 32) / 8;
-    uint4* step = a.h + (static_cast<int64_t>(seg) * hsteps + s) * 256 + pj * 32 + pt;
+    uint4* step = a.h + (static_cast<int64_t>(seg) * hsteps + s) * (a.planes * 128) + pj * 32 + pt;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const int col = 2 * t + i;
       if (col < ntok) {
         const float ga = acc[q][i], up = acc[q][2 + i];
-        const float h = __fdiv_rn(ga, 1.f + expf(-ga)) * up * col_w[col];
-        const __nv_bfloat16 hi = __float2bfloat16_rn(h);
+        float h = __fdiv_rn(ga, 1.f + expf(-ga)) * up * col_w[col];
         __nv_bfloat16* at = reinterpret_cast<__nv_bfloat16*>(step + col * 4) + pair_place<BITS>(n);
+        const __nv_bfloat16 hi = __float2bfloat16_rn(h);
+        h = __hisinf(hi) ? 0.f : h - __bfloat162float(hi);  // (infinity minus itself is a NaN)
+        const __nv_bfloat16 mid = __float2bfloat16_rn(h);
         at[0] = hi;
-        at[lo * 8] = __float2bfloat16_rn(__hisinf(hi) ? 0.f : h - __bfloat162float(hi));  // (infinity minus itself is a NaN)
+        at[o1] = mid;
+        at[o2] = __float2bfloat16_rn(h - __bfloat162float(mid));
+        if (nparts == 4) at[part_piece(ntok, 3) * 8] = __float2bfloat16_rn(0.f);
       }
     }
   }
   if (rb == a.I / 16 - 1) {  // zeros behind the last feature of the last step
     for (int p = a.I / 8; p < hsteps * 16; ++p) {
-      uint4* piece = a.h + (static_cast<int64_t>(seg) * hsteps + p / 16) * 256 + p % 4 * 32 + p % 16 / 4;
-      if (lane < 2 * ntok) piece[(lane & 1) * lo + (lane >> 1) * 4] = make_uint4(0, 0, 0, 0);
+      uint4* piece = a.h + (static_cast<int64_t>(seg) * hsteps + p / 16) * (a.planes * 128) + p % 4 * 32 + p % 16 / 4;
+      const int part = lane >> 3, col = lane & 7;
+      if (part < nparts && col < ntok) piece[part_piece(ntok, part) + col * 4] = make_uint4(0, 0, 0, 0);
     }
   }
 }
@@ -862,8 +875,7 @@ template <int BITS>
 struct Stage2 {  // 128 bytes of the panel's packed rows (two steps at INT4, one at INT8), and h
   static constexpr int STEPS = Codes<BITS>::STEPS;
   static constexpr int W = PANEL * 128;
-  static constexpr int H = STEPS * 4096;
-  static constexpr int BYTES = W + H;
+  static __host__ __device__ constexpr int bytes(int planes) { return W + STEPS * planes * 2048; }
 };
 
 struct Smem2 {
@@ -874,9 +886,9 @@ struct Smem2 {
   int last;
 };
 
-// GEMM2 and the combine.  The same layer: 20 us for 71 MB at 32 tokens (issue again: two MMAs for h's two parts), then 5 for
-// the parts; one token 3 and 4.  All of it: 32 tokens 81 us (INT8 105), one token 26 (INT8 30), 8 tokens INT8 with given
-// routing 67 (4.0 TB/s).
+// GEMM2 and the combine.  The same layer: 22 us for 71 MB at 32 tokens (issue again: up to three MMAs for h's three parts), then
+// 5 for the outputs' parts; one token 3 and 4.  All of it: 32 tokens 83 us (INT8 105), one token 26 (INT8 30), 8 tokens INT8
+// with given routing 66 (4.1 TB/s).  (With two parts of h, 16 bits of it, 81 (105), 26 (30) and 67.)
 template <int BITS, bool V4>
 __global__ void __launch_bounds__(THREADS2, 1)
     few_gemm2_kernel(const __grid_constant__ CUtensorMap tm_w, const FewArgs a) {
@@ -884,9 +896,9 @@ __global__ void __launch_bounds__(THREADS2, 1)
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
   using S = Stage2<BITS>;
   constexpr int SS = S::STEPS;
-  const int depth = a.depth2;
-  Smem2& sm = *reinterpret_cast<Smem2*>(base + GROUPS * depth * S::BYTES);
-  float* parts = reinterpret_cast<float*>(base + GROUPS * depth * S::BYTES + sizeof(Smem2));  // [GROUPS][PANEL][pitch]
+  const int depth = a.depth2, stage_bytes = S::bytes(a.planes), hstep = a.planes * 2048;
+  Smem2& sm = *reinterpret_cast<Smem2*>(base + GROUPS * depth * stage_bytes);
+  float* parts = reinterpret_cast<float*>(base + GROUPS * depth * stage_bytes + sizeof(Smem2));  // [GROUPS][PANEL][pitch]
   const int pitch = a.T | 1;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int panel = blockIdx.x / a.split, rank = blockIdx.x % a.split, tile = warp % MT, group = warp / MT;
@@ -935,17 +947,17 @@ __global__ void __launch_bounds__(THREADS2, 1)
           if (!ok) break;
           const Segment sg = sm.seg[seg[q]];
           uint64_t* bar = &sm.full[q][st[q]];
-          uint8_t* dst = base + (q * depth + st[q]) * S::BYTES;
+          uint8_t* dst = base + (q * depth + st[q]) * stage_bytes;
           const int n = min(SS, steps - z[q] * SS);
-          const int hb = sg.n <= 4 ? 2048 : 4096;  // of a step
+          const int hb = planes_of(sg.n) * 2048;  // of a step
           const int y = sg.expert * a.H + panel * PANEL;
           if (lane == 0) mbar_expect_tx(bar, S::W + n * hb);
           __syncwarp();
           if (lane == 0) {
             tma_load_2d(dst, &tm_w, z[q] * 128, y, bar);
           } else if (lane <= n) {
-            bulk_load(dst + S::W + (lane - 1) * 4096, a.h + (static_cast<int64_t>(seg[q]) * steps + z[q] * SS + lane - 1) * 256,
-                      hb, bar);
+            bulk_load(dst + S::W + (lane - 1) * hstep,
+                      a.h + (static_cast<int64_t>(seg[q]) * steps + z[q] * SS + lane - 1) * (a.planes * 128), hb, bar);
           }
           ++at[q];
           ++issued[q];
@@ -979,17 +991,17 @@ __global__ void __launch_bounds__(THREADS2, 1)
     for (int at = begin; at < end && ok;) {
       const int si = at / slots, za = at - si * slots, zb = min(slots, za + end - at);
       const Segment sg = sm.seg[si];
-      const bool packed = sg.n <= 4;
+      const int planes = planes_of(sg.n), lo = planes > 2 ? 4096 : 2048;
       RowScales<SS, V4> scales;
       scales.start(a.s2 + (static_cast<int64_t>(sg.expert) * a.H + ns) * a.groups2, za * SS, steps, a.gsteps2);
       float acc[2][4] = {};
       for (int z = za; z < zb; ++z, ++at) {
         ok = mbar_wait(&sm.full[group][st], phase, abort_flag, 0x610 + group);
         if (!ok) break;
-        const uint32_t stage = smem_u32(base + (group * depth + st) * S::BYTES);
+        const uint32_t stage = smem_u32(base + (group * depth + st) * stage_bytes);
         uint32_t rows = stage + lane_row, ha = stage + S::W + lane * 16;
 #pragma unroll 1
-        for (int h = 0; h < SS; ++h, rows ^= 64, ha += 4096) {
+        for (int h = 0; h < SS; ++h, rows ^= 64, ha += hstep) {
           if (z * SS + h < steps) {
             Codes<BITS> w[2][2];
 #pragma unroll
@@ -1001,6 +1013,11 @@ __global__ void __launch_bounds__(THREADS2, 1)
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
               const uint4 hv = lds16(ha + j * 512);
+              uint4 mv, lv;  // asked for together, ahead of the MMAs (32 tokens 83.4 us; each before its own 86.0)
+              if (planes > 1) {
+                mv = lds16(ha + 2048 + j * 512);
+                lv = lds16(ha + lo + j * 512);
+              }
               uint32_t p[2][2][4];
 #pragma unroll
               for (int q = 0; q < 2; ++q) {
@@ -1009,8 +1026,14 @@ __global__ void __launch_bounds__(THREADS2, 1)
                 mma_bf16(d0[q], p[q][0][0], p[q][1][0], p[q][0][1], p[q][1][1], hv.x, hv.y);
                 mma_bf16(d1[q], p[q][0][2], p[q][1][2], p[q][0][3], p[q][1][3], hv.z, hv.w);
               }
-              if (!packed) {
-                const uint4 lv = lds16(ha + 2048 + j * 512);
+              if (planes > 1) {
+#pragma unroll
+                for (int q = 0; q < 2; ++q) {
+                  mma_bf16(d0[q], p[q][0][0], p[q][1][0], p[q][0][1], p[q][1][1], mv.x, mv.y);
+                  mma_bf16(d1[q], p[q][0][2], p[q][1][2], p[q][0][3], p[q][1][3], mv.z, mv.w);
+                }
+              }
+              if (planes > 2) {
 #pragma unroll
                 for (int q = 0; q < 2; ++q) {
                   mma_bf16(d0[q], p[q][0][0], p[q][1][0], p[q][0][1], p[q][1][1], lv.x, lv.y);
@@ -1033,11 +1056,14 @@ __global__ void __launch_bounds__(THREADS2, 1)
           phase ^= 1;
         }
       }
-      if (packed) {  // columns 4 to 7 are the lo parts of 0 to 3
+      if (planes < 3) {  // the other parts of a quad's lane 0 (and 1): in lanes 1 and 2 with at most 2 tokens, else in 2 (and 3)
 #pragma unroll
         for (int q = 0; q < 2; ++q)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) acc[q][i] = __fadd_rn(acc[q][i], __shfl_xor_sync(0xffffffffu, acc[q][i], 2));
+          for (int i = 0; i < 4; ++i) {
+            const float v = acc[q][i], far = __shfl_sync(0xffffffffu, v, lane + 2), near = __shfl_sync(0xffffffffu, v, lane + 1);
+            acc[q][i] = __fadd_rn(v, planes == 1 ? __fadd_rn(near, far) : far);
+          }
       }
       // rows belong to this warp alone, and the tokens of a segment are distinct
 #pragma unroll
@@ -1172,9 +1198,10 @@ int launch_gemm2(FewArgs& a, cudaStream_t st) {
   if (rc) return rc;
   // as deep as the partial outputs leave room for
   const int fixed = 1024 + static_cast<int>(sizeof(Smem2)) + GROUPS * PANEL * (a.T | 1) * 4;
-  a.depth2 = std::min(MAX_DEPTH2, (kSmemMost - fixed) / (GROUPS * Stage2<BITS>::BYTES));
+  const int stage = GROUPS * Stage2<BITS>::bytes(a.planes);
+  a.depth2 = std::min(MAX_DEPTH2, (kSmemMost - fixed) / stage);
   return launch_few_kernel(few_gemm2_kernel<BITS, V4>, panels_of(a.H) * a.split, 1, THREADS2,
-                           fixed + GROUPS * a.depth2 * Stage2<BITS>::BYTES, st, tw, a, "few_gemm2_kernel");
+                           fixed + a.depth2 * stage, st, tw, a, "few_gemm2_kernel");
 }
 
 template <int BITS>
@@ -1202,7 +1229,7 @@ struct FewWorkspace {
 FewWorkspace few_workspace(int64_t T, int k, int E, int H, int I) {
   FewWorkspace w;
   w.h = up256(sizeof(FewPlan));
-  w.partial = w.h + static_cast<size_t>(few_segments(T, k, E)) * ((I + KG - 1) / KG) * 4096;
+  w.partial = w.h + static_cast<size_t>(few_segments(T, k, E)) * ((I + KG - 1) / KG) * planes_of(static_cast<int>(T)) * 2048;
   w.total = w.partial + static_cast<size_t>(panels_of(H)) * MAX_SPLIT * PANEL * T * 4;
   return w;
 }
@@ -1261,6 +1288,7 @@ int moe_few(const llq_few_layer& L, const void* x, int64_t T, float* logits, flo
   a.plan = reinterpret_cast<FewPlan*>(ws);
   const FewWorkspace w = few_workspace(T, L.k, L.E, L.H, L.I);
   a.h = reinterpret_cast<uint4*>(ws + w.h);
+  a.planes = planes_of(a.T);
   a.partial = reinterpret_cast<float*>(ws + w.partial);
   a.split = split_of(L.H);
   a.out = static_cast<__nv_bfloat16*>(out);

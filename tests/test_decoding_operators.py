@@ -1,0 +1,56 @@
+"""The decoding step's operators where a value is held between kernels or between calls."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T", [1, 2, 3, 4, 5, 8, 9, 10, 12, 32])  # segments of 1 to 8 tokens, alone and behind full ones
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("inter", [32, 160, 384])
+def test_h_keeps_the_bits_of_fp32(T, bits, inter):
+    """out = h0 - h1 for two fp32 numbers that agree in their upper 16 bits: the lower 8, exactly.
+
+    Every feature has a = 32 and b = 2^-5, so h = silu(a) b w = w in fp32 (exp(-32) < 2^-24).  Expert 0 adds the h of one
+    feature to each output and expert 1 takes it away.  w0 has 24 bits in [1, 1.5) and w1 is w0 without its lower 8, so
+    that parts of either, and any sum of them, are multiples of 2^-23 below 2: fp32 sums in any order are exact, and the
+    8 bits that are left are a bf16 number.
+    """
+    from llada_quant_b200.few_tokens import FewTokenMoE
+    from llada_quant_b200.moe import PackedExperts
+    H, one = 64, 1 if bits == 8 else 0x01
+    w1 = torch.zeros(2, 2 * inter, H * bits // 8, dtype=torch.int8)
+    w1[:, :, 0] = one
+    s1 = torch.cat([torch.full((2, inter, 1), 32.0), torch.full((2, inter, 1), 2.0 ** -5)], 1)
+    w2 = torch.zeros(2, H, inter, dtype=torch.int8)
+    for r in range(H):
+        w2[0, r, r * 37 % inter], w2[1, r, r * 37 % inter] = 1, -1
+    if bits == 4:
+        w2 = (w2[..., 0::2] & 15) | (w2[..., 1::2] << 4)
+    packed = PackedExperts(w1.cuda(), s1.cuda(), w2.contiguous().cuda(), torch.ones(2, H, 1, device="cuda"), bits, -1)
+    x = torch.zeros(T, H, dtype=torch.bfloat16, device="cuda")
+    x[:, 0] = 1
+    low = torch.randint(1, 256, (T,), generator=torch.Generator().manual_seed(T))
+    high = torch.randint(2 ** 15, 3 * 2 ** 14, (T,), generator=torch.Generator().manual_seed(T + 1)) * 256
+    weights = (torch.stack([high + low, high], 1).double() * 2.0 ** -23).float().cuda()
+    ids = torch.tensor([[0, 1]], dtype=torch.int32, device="cuda").repeat(T, 1)
+    out = FewTokenMoE(packed, None, 2).routed(x, weights, ids)
+    want = (low.double() * 2.0 ** -23).cuda()[:, None].expand(T, H)
+    assert torch.equal(out.double(), want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("T", [1, 2])
+def test_an_infinite_h_of_one_or_two_tokens_stays_infinite(T, bits):
+    """The parts of h side by side in one plane: infinity and zeros, no NaN."""
+    from llada_quant_b200.few_tokens import FewTokenMoE
+    from llada_quant_b200.moe import PackedExperts
+    one = torch.full((2, 64, 32 if bits == 8 else 16), 1 if bits == 8 else 0x11, dtype=torch.int8, device="cuda")
+    packed = PackedExperts(one, torch.ones(2, 64, 1, device="cuda"), one[:, :32].contiguous(), torch.ones(2, 32, 1, device="cuda"),
+                           bits, -1)
+    x = torch.full((T, 32), 1e30, dtype=torch.bfloat16, device="cuda")
+    out = FewTokenMoE(packed, None, 1).routed(x, torch.ones(T, 1, device="cuda"), torch.ones(T, 1, dtype=torch.int32, device="cuda"))
+    assert bool((out == float("inf")).all())
