@@ -29,36 +29,57 @@ class FewTokenMoE:
 
     ``gate_w`` bf16 ``[E, H]`` (may be None for :meth:`routed` alone), ``bias`` fp32 ``[E]`` added to
     the logits (``-inf`` bars an expert), ``renormalize`` divides a token's weights by their sum.
+    An operand whose memory was exchanged (``module.to()``, ``parameter.data = ...``) is seen by the
+    next call, which checks all of them again; until then the layer holds the memory that they had.
     """
 
     def __init__(self, packed: PackedExperts, gate_w: Optional[torch.Tensor], top_k: int,
                  bias: Optional[torch.Tensor] = None, renormalize: bool = False) -> None:
         if not 1 <= top_k <= packed.num_experts:
             raise ValueError(f"top_k must be 1 to {packed.num_experts}, got {top_k}")
+        self.top_k, self._renormalize = top_k, renormalize
+        self._packed, self._gate, self._bias = packed, gate_w, bias
+        given = (packed.qw1, packed.sw1, packed.qw2, packed.sw2, gate_w, bias)
+        self._operands = tuple(t for t in given if t is not None)
+        self._prepare()
+
+    def _prepare(self) -> tuple:
+        """The descriptors of the operands as they are now: (addresses, what keeps them alive, layer, routed layer)."""
+        p, gate_w, bias = self._packed, self._gate, self._bias
         ops._no_grad_through("the few-token layer", gate_w, bias)
-        gate_w = None if gate_w is None else ops._aligned(gate_w)
-        bias = None if bias is None else bias.to(torch.float32).contiguous()
-        self._held = (packed, gate_w, bias)  # the descriptor has their addresses
-        args = (packed.qw1, packed.sw1, packed.qw2, packed.sw2, top_k, packed.bits)
-        self._layer = None if gate_w is None else ops.few_layer(*args, gate_w, bias, renormalize)
-        self._routed = ops.few_layer(*args)
-        self.top_k = top_k
-        self.num_experts, self.hidden = packed.num_experts, packed.hidden
-        self.device = packed.qw1.device
+        at = [t.data_ptr() for t in self._operands]
+        # (an alias owns its storage even where the operand gets another: no address of `at` is given away)
+        held = [t.detach() for t in self._operands]
+        args = (p.qw1, p.sw1, p.qw2, p.sw2, self.top_k, p.bits)
+        layer = None
+        if gate_w is not None:
+            gate_w = ops._aligned(gate_w)
+            bias = None if bias is None else bias.to(torch.float32).contiguous()
+            held += [gate_w, bias]
+            layer = ops.few_layer(*args, gate_w, bias, self._renormalize)
+        self._ready = ready = (at, held, layer, ops.few_layer(*args))
+        self.num_experts, self.hidden, self.device = p.num_experts, p.hidden, p.qw1.device
+        return ready
+
+    def _checked(self) -> tuple:
+        ready = self._ready
+        return ready if [t.data_ptr() for t in self._operands] == ready[0] else self._prepare()
 
     def __call__(self, x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
         """x bf16 ``[T <= 32, H]`` -> (out bf16 ``[T, H]``, weights fp32 ``[T, k]``, ids int32 ``[T, k]``)."""
+        ready = self._checked()
         x, weights, ids = self._outputs(x)
-        return ops.few_call(self._layer, x, weights, ids), weights, ids
+        return ops.few_call(ready[2], x, weights, ids), weights, ids
 
     def with_logits(self, x: torch.Tensor):
         """As a call, with the router's logits (bias added) fp32 ``[T, E]`` as the fourth."""
+        ready = self._checked()
         x, weights, ids = self._outputs(x)
         logits = torch.empty(x.shape[0], self.num_experts, dtype=torch.float32, device=self.device)
-        return ops.few_call(self._layer, x, weights, ids, logits), weights, ids, logits
+        return ops.few_call(ready[2], x, weights, ids, logits), weights, ids, logits
 
     def _outputs(self, x: torch.Tensor):
-        if self._layer is None:
+        if self._gate is None:
             raise ValueError("this layer was made without gate_w: call routed(x, weights, ids)")
         x = ops.few_rows(x, self.hidden, self.device)
         T = x.shape[0]
@@ -68,6 +89,7 @@ class FewTokenMoE:
     def routed(self, x: torch.Tensor, topk_weights: torch.Tensor, topk_ids: torch.Tensor) -> torch.Tensor:
         """The experts alone, with the caller's routing ``[T, k]``.  Ids outside ``[0, E)`` contribute
         nothing; an expert that a token names twice counts with the sum of the two weights."""
+        ready = self._checked()
         x = ops.few_rows(x, self.hidden, self.device)
         w, ids = ops.few_routing(topk_weights, topk_ids, x.shape[0], self.top_k, self.num_experts, self.device)
-        return ops.few_call(self._routed, x, w, ids)
+        return ops.few_call(ready[3], x, w, ids)

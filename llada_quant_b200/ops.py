@@ -580,6 +580,8 @@ def few_layer(qw1: torch.Tensor, sw1: torch.Tensor, qw2: torch.Tensor, sw2: torc
     devs = {t.device for t in (qw1, sw1, qw2, sw2, gate_w, bias) if t is not None}
     if len(devs) > 1:
         raise ValueError(f"one layer's tensors lie on several devices: {sorted(map(str, devs))}")
+    if any(t is not None and t.data_ptr() == 0 for t in (qw1, sw1, qw2, sw2, gate_w, bias)):
+        raise ValueError("one of the layer's tensors has no memory")  # (a null gate_w would say that the caller routes)
     return _lib.FewLayer(_ptr(gate_w), _ptr(bias), qw1.data_ptr(), sw1.data_ptr(), qw2.data_ptr(), sw2.data_ptr(),
                          E, H, inter, k, bits, group, int(renormalize))
 

@@ -54,3 +54,72 @@ def test_an_infinite_h_of_one_or_two_tokens_stays_infinite(T, bits):
     x = torch.full((T, 32), 1e30, dtype=torch.bfloat16, device="cuda")
     out = FewTokenMoE(packed, None, 1).routed(x, torch.ones(T, 1, device="cuda"), torch.ones(T, 1, dtype=torch.int32, device="cuda"))
     assert bool((out == float("inf")).all())
+
+
+# ---------------------------------------------------------------------------
+# operands that change between calls
+# ---------------------------------------------------------------------------
+
+def layer_parts(device):
+    from llada_quant_b200.moe import PackedExperts
+    from tests.test_few_tokens import make_layer
+    layer, x, gate, weights, ids = make_layer(4, 8, 256, 128, 2, 4, 128, device=device)
+    return PackedExperts(*layer[:4], 4, 128), x, gate, weights, ids
+
+
+def test_exchanged_operands_reach_the_next_call_without_a_gpu(monkeypatch):
+    """The addresses that a call passes are those of the operands at the call."""
+    from llada_quant_b200 import ops
+    from llada_quant_b200.few_tokens import FewTokenMoE
+    passed = []
+    monkeypatch.setattr(ops, "_need_cuda", lambda *ts: None)
+    monkeypatch.setattr(ops, "few_call", lambda layer, x, *a: passed.append(layer) or x)
+    packed, x, gate, weights, ids = layer_parts("cpu")
+    router = torch.nn.Linear(256, 8, bias=False, dtype=torch.bfloat16).requires_grad_(False)
+    router.weight.copy_(gate)
+    bias = torch.zeros(8)
+    moe = FewTokenMoE(packed, router.weight, 2, bias)
+    moe(x)
+    old = router.weight.data_ptr()
+    router.float()
+    with pytest.raises(ValueError, match="gate_w must be"):
+        moe(x)
+    router.bfloat16()
+    moe(x)
+    assert passed[0].gate_w == old and passed[1].gate_w == router.weight.data_ptr()
+    for t, name in ((packed.qw1, "qw1"), (packed.sw1, "sw1"), (packed.qw2, "qw2"), (packed.sw2, "sw2"), (bias, "bias")):
+        t.data = t.data.clone()
+        moe.with_logits(x)
+        assert getattr(passed[-1], name) == t.data_ptr(), name
+        moe.routed(x, weights, ids)
+        assert name == "bias" or getattr(passed[-1], name) == t.data_ptr(), name
+    router.weight.data = router.weight.data[:, 128:]
+    with pytest.raises(ValueError, match="gate_w must be"):
+        moe(x)
+    router.weight.data = gate.clone()
+    moe(x)
+    router.weight.data.untyped_storage().resize_(0)
+    with pytest.raises(ValueError, match="no memory"):
+        moe(x)
+
+
+@pytest.mark.gpu
+def test_exchanged_operands_reach_the_next_call():
+    from llada_quant_b200.few_tokens import FewTokenMoE
+    packed, x, gate, weights, ids = layer_parts("cuda")
+    router = torch.nn.Linear(256, 8, bias=False, dtype=torch.bfloat16, device="cuda").requires_grad_(False)
+    router.weight.copy_(gate)
+    moe = FewTokenMoE(packed, router.weight, 2)
+    want = moe(x)
+    router.float()  # the bf16 storage is given back
+    fill = [torch.full((8, 256), float("nan"), dtype=torch.bfloat16, device="cuda") for _ in range(8)]
+    with pytest.raises(ValueError, match="gate_w must be"):
+        moe(x)
+    router.bfloat16()
+    assert all(torch.equal(a, b) for a, b in zip(moe(x), want))
+    router.weight.data = gate.flip(0).contiguous()
+    assert torch.equal(moe(x)[2], 7 - want[2])
+    was = moe.routed(x, weights, ids)
+    packed.sw2.data = packed.sw2 * 2
+    assert torch.equal(moe.routed(x, weights, ids), was * 2)
+    del fill
