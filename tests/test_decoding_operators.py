@@ -2,6 +2,8 @@
 
 from __future__ import annotations
 
+import ctypes
+
 import pytest
 import torch
 
@@ -123,3 +125,52 @@ def test_exchanged_operands_reach_the_next_call():
     packed.sw2.data = packed.sw2 * 2
     assert torch.equal(moe.routed(x, weights, ids), was * 2)
     del fill
+
+
+def odd_router(gate, bias):
+    """gate_w between other columns, and a bias that is exact in bf16: both have to be copied."""
+    wide = torch.zeros(gate.shape[0], gate.shape[1] + 7, dtype=gate.dtype, device=gate.device)
+    wide[:, 3:3 + gate.shape[1]] = gate
+    return wide[:, 3:3 + gate.shape[1]], bias.to(torch.bfloat16)
+
+
+def test_copied_operands_are_copied_for_each_call_without_a_gpu(monkeypatch):
+    from llada_quant_b200 import ops
+    from llada_quant_b200.few_tokens import FewTokenMoE
+    seen = []
+
+    def call(layer, x, *a):
+        seen.append((list((ctypes.c_float * 8).from_address(layer.bias)),
+                     list((ctypes.c_int16 * 2048).from_address(layer.gate_w))))
+        return x
+
+    monkeypatch.setattr(ops, "_need_cuda", lambda *ts: None)
+    monkeypatch.setattr(ops, "few_call", call)
+    packed, x, gate, _, _ = layer_parts("cpu")
+    g, b = odd_router(gate, torch.arange(8) / 8)
+    moe = FewTokenMoE(packed, g, 2, b)
+    for change in (lambda: None, lambda: b.fill_(3), lambda: g.mul_(2)):
+        change()
+        for run in (moe, moe.with_logits):
+            run(x)
+            assert seen[-1] == (b.tolist(), g.contiguous().view(torch.int16).flatten().tolist())
+
+
+@pytest.mark.gpu
+def test_operands_changed_in_place_reach_calls_and_replays():
+    from llada_quant_b200.few_tokens import FewTokenMoE
+    packed, x, gate, _, _ = layer_parts("cuda")
+    plain = torch.arange(8, device="cuda") / 8
+    for g, b in ((gate.clone(), plain.clone()), odd_router(gate, plain)):
+        moe, graph = FewTokenMoE(packed, g, 2, b), torch.cuda.CUDAGraph()
+        moe(x)
+        with torch.cuda.graph(graph):
+            held = moe(x)
+        eager = moe(x)  # before any replay
+        for change in (lambda: None, lambda: b.copy_(plain.flip(0)), lambda: g.copy_(gate.flip(0))):
+            change()
+            want = FewTokenMoE(packed, g.contiguous(), 2, b.float())(x)
+            graph.replay()
+            for got in (moe(x), held):
+                assert all(torch.equal(p, q) for p, q in zip(got, want))
+        assert all(torch.equal(p, q) for p, q in zip(eager, FewTokenMoE(packed, gate, 2, plain)(x)))
