@@ -75,8 +75,10 @@ def _multiply(w: ops.Fp8Weight, x: Union[torch.Tensor, Fp8Tensor]) -> torch.Tens
 
 
 class Fp8Linear(nn.Module):
-    """Linear layer on e4m3 weights: ``qweight`` uint8 ``[out, pitch]`` (the codes' bytes, rows padded to
-    16), ``scale`` fp32 ``[ceil(out / 128), ceil(in / 128)]``, ``bias`` of ``compute_dtype`` or None.
+    """Linear layer on e4m3 weights: ``qweight`` uint8 ``[out, in]`` (the codes' bytes), ``scale`` fp32
+    ``[ceil(out / 128), ceil(in / 128)]``, ``bias`` of ``compute_dtype`` or None.  Calls see what the buffers
+    hold at the call; a bias of another type, or a buffer that is not contiguous and 16-byte aligned, is
+    copied for every call.
 
     The buffers are bytes, not float8, so that ``module.half()`` and the like leave them alone.
     """
@@ -140,13 +142,15 @@ class Fp8Linear(nn.Module):
         return {**self.__dict__, "_ready": None}  # addresses do not outlive the object
 
     def _multiplier(self) -> ops.Fp8Weight:
-        """The checked operand of the buffers as they are now (checked again when one was replaced)."""
+        """The checked operand of the buffers as they are now, kept until one is replaced.  An operand that copied one of
+        them serves this call alone: the next sees what the buffer holds then, in its own stream's order and graph."""
         b, r = self._buffers, self._ready
         q, s, bias = b["qweight"], b["scale"], b["bias"]
         at = (q.data_ptr(), s.data_ptr(), 0 if bias is None else bias.data_ptr())
         if r is None or r[0] is not q or r[1] is not s or r[2] is not bias or r[3] != at:
             w = ops.Fp8Weight(q.view(torch.float8_e4m3fn), s, bias, self.compute_dtype)
-            self._ready = r = (q, s, bias, at, w)
+            self._ready = None if w.copied else (q, s, bias, at, w)
+            return w
         return r[4]
 
     def forward(self, x: Union[torch.Tensor, Fp8Tensor]) -> torch.Tensor:

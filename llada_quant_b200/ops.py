@@ -751,9 +751,11 @@ def fp8_operand(codes: torch.Tensor, what: str) -> torch.Tensor:
 
 
 class Fp8Weight:
-    """A checked e4m3 weight [N, K] with its scales and bias, ready to multiply."""
+    """A checked e4m3 weight [N, K] with its scales and bias, ready to multiply: aliases of the given tensors, or
+    (``copied``) copies of those that the kernels cannot read as they are."""
 
-    __slots__ = ("codes", "scale", "bias", "N", "K", "G", "ldw", "device", "dtype", "_out", "_w", "_s", "_b", "_need")
+    __slots__ = ("codes", "scale", "bias", "copied", "N", "K", "G", "ldw", "device", "dtype", "_out", "_w", "_s", "_b",
+                 "_need")
 
     def __init__(self, codes: torch.Tensor, scale: torch.Tensor, bias: Optional[torch.Tensor],
                  out_dtype: torch.dtype) -> None:
@@ -761,6 +763,7 @@ class Fp8Weight:
         _no_grad_through("the e4m3 product", bias)
         if out_dtype not in _DT:
             raise ValueError(f"the e4m3 product gives fp32, fp16 or bf16, not {out_dtype}")
+        given = (codes, scale, bias)
         codes = fp8_operand(codes, "the weight")
         self.N, self.K = codes.shape
         self.G = fp8_groups(self.K)
@@ -771,7 +774,8 @@ class Fp8Weight:
             if tuple(bias.shape) != (self.N,):
                 raise ValueError(f"bias must be [{self.N}], got {tuple(bias.shape)}")
             bias = bias.detach().to(out_dtype).contiguous()
-        self.codes, self.scale, self.bias = codes, scale.contiguous(), bias
+        self.codes, self.scale, self.bias = codes, scale.detach().contiguous(), bias
+        self.copied = any(t is not None and t.data_ptr() != g.data_ptr() for t, g in zip((codes, self.scale, bias), given))
         self.device, self.dtype, self._out = codes.device, out_dtype, _DT[out_dtype]
         if any(t is not None and t.device != self.device for t in (scale, bias)):
             raise ValueError("the product's operands lie on several devices")

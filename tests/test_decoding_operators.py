@@ -174,3 +174,62 @@ def test_operands_changed_in_place_reach_calls_and_replays():
             for got in (moe(x), held):
                 assert all(torch.equal(p, q) for p, q in zip(got, want))
         assert all(torch.equal(p, q) for p, q in zip(eager, FewTokenMoE(packed, gate, 2, plain)(x)))
+
+
+def linear_of(device, bias_dtype=torch.bfloat16, compute=torch.bfloat16):
+    """An Fp8Linear 256 -> 40 on random bytes, with a bias that is exact in every type."""
+    from llada_quant_b200.fp8 import Fp8Linear
+    m = Fp8Linear(256, 40, bias=True, compute_dtype=compute)
+    g = torch.Generator().manual_seed(1)
+    m.qweight.copy_(torch.randint(0, 0x70, m.qweight.shape, generator=g, dtype=torch.uint8))
+    m.scale.copy_(torch.rand(m.scale.shape, generator=g) / 64)
+    m.bias = (torch.arange(40) / 4).to(bias_dtype)
+    return m.to(device)
+
+
+def odd_buffers(m):
+    """Replaces each buffer of m by one that has to be copied."""
+    bad = torch.empty(m.qweight.numel() + 1, dtype=torch.uint8, device=m.qweight.device)[1:].view(m.qweight.shape)
+    m.qweight = bad.copy_(m.qweight)
+    m.scale = m.scale.t().contiguous().t() if m.scale.shape[0] > 1 else m.scale.repeat_interleave(2, 1)[:, ::2]
+    m.bias = m.bias.float()
+    return m
+
+
+def test_copied_buffers_are_copied_for_each_call_without_a_gpu(monkeypatch):
+    """The operand of a call holds what the buffers hold at the call, whether they are read in place or copied."""
+    from llada_quant_b200 import ops
+    seen = []
+    monkeypatch.setattr(ops, "_need_cuda", lambda *ts: None)
+    monkeypatch.setattr(ops.Fp8Weight, "multiply", lambda w, x, s=None: seen.append(
+        (w.codes.view(torch.uint8).clone(), w.scale.clone(), w.bias.float())) or x.new_zeros(x.shape[0], w.N))
+    x = torch.zeros(3, 256)
+    one_by_one = [lambda m: setattr(m, "bias", m.bias.float()), lambda m: setattr(m, "scale", odd_buffers(linear_of("cpu")).scale)]
+    for make in (lambda m: None, odd_buffers, *one_by_one):
+        m = linear_of("cpu")
+        make(m)
+        for change in (lambda: None, lambda: m.bias.fill_(3), lambda: m.scale.mul_(2), lambda: m.qweight.fill_(8),
+                       lambda: m.load_state_dict(linear_of("cpu").state_dict())):
+            change()
+            m(x)
+            assert all(torch.equal(a, b) for a, b in zip(seen[-1], (m.qweight, m.scale, m.bias.float())))
+
+
+@pytest.mark.gpu
+def test_buffers_changed_in_place_reach_calls_and_replays():
+    from tests.test_fp8 import check_product
+    from llada_quant_b200.fp8 import quantize_fp8
+    x = torch.randn(5, 256, generator=torch.Generator().manual_seed(2)).to(torch.bfloat16).cuda()
+    q = quantize_fp8(x)
+    for make in (lambda m: m, odd_buffers):
+        m, graph = make(linear_of("cuda")), torch.cuda.CUDAGraph()
+        make(linear_of("cuda"))(x)
+        with torch.cuda.graph(graph):
+            held = m(x)  # the module's first call
+        eager = m(x)  # before any replay
+        check_product(eager, q.codes, q.scale, m.weight, m.bias)
+        for change in (lambda: None, lambda: m.bias.fill_(3), lambda: m.scale.mul_(2), lambda: m.qweight.sub_(8).clamp_(0, 0x70)):
+            change()
+            graph.replay()
+            assert torch.equal(held, m(x))
+            check_product(held, q.codes, q.scale, m.weight, m.bias)
