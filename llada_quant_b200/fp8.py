@@ -147,7 +147,7 @@ class Fp8Linear(nn.Module):
         b, r = self._buffers, self._ready
         q, s, bias = b["qweight"], b["scale"], b["bias"]
         at = (q.data_ptr(), s.data_ptr(), 0 if bias is None else bias.data_ptr())
-        if r is None or r[0] is not q or r[1] is not s or r[2] is not bias or r[3] != at:
+        if r is None or r[0] is not q or r[1] is not s or r[2] is not bias or r[3] != at or r[4].dtype is not self.compute_dtype:
             w = ops.Fp8Weight(q.view(torch.float8_e4m3fn), s, bias, self.compute_dtype)
             self._ready = None if w.copied else (q, s, bias, at, w)
             return w

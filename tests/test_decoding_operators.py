@@ -233,3 +233,13 @@ def test_buffers_changed_in_place_reach_calls_and_replays():
             graph.replay()
             assert torch.equal(held, m(x))
             check_product(held, q.codes, q.scale, m.weight, m.bias)
+
+
+def test_a_changed_compute_dtype_reaches_the_next_call_without_a_gpu(monkeypatch):
+    from llada_quant_b200 import ops
+    monkeypatch.setattr(ops, "_need_cuda", lambda *ts: None)
+    monkeypatch.setattr(ops.Fp8Weight, "multiply", lambda w, x, s=None: x.new_zeros(x.shape[0], w.N, dtype=w.dtype))
+    m, x = linear_of("cpu"), torch.zeros(3, 256)
+    for dtype in (torch.bfloat16, torch.float32, torch.float16, torch.bfloat16):
+        m.compute_dtype = dtype
+        assert m(x).dtype == dtype and m(x).dtype == dtype
