@@ -141,6 +141,19 @@ class Fp8Linear(nn.Module):
     def __getstate__(self):
         return {**self.__dict__, "_ready": None}  # addresses do not outlive the object
 
+    def __setattr__(self, name, value) -> None:
+        if name in ("qweight", "scale", "bias"):
+            self.__dict__["_ready"] = None  # (it would keep the old buffer's memory until the next call)
+        super().__setattr__(name, value)
+
+    def _apply(self, fn, recurse=True):
+        self._ready = None
+        return super()._apply(fn, recurse)
+
+    def _load_from_state_dict(self, *args, **kwargs) -> None:
+        self._ready = None
+        super()._load_from_state_dict(*args, **kwargs)
+
     def _multiplier(self) -> ops.Fp8Weight:
         """The checked operand of the buffers as they are now, kept until one is replaced.  An operand that copied one of
         them serves this call alone: the next sees what the buffer holds then, in its own stream's order and graph."""

@@ -3,6 +3,8 @@
 from __future__ import annotations
 
 import ctypes
+import gc
+import weakref
 
 import pytest
 import torch
@@ -243,3 +245,32 @@ def test_a_changed_compute_dtype_reaches_the_next_call_without_a_gpu(monkeypatch
     for dtype in (torch.bfloat16, torch.float32, torch.float16, torch.bfloat16):
         m.compute_dtype = dtype
         assert m(x).dtype == dtype and m(x).dtype == dtype
+
+
+def test_replaced_buffers_are_given_back_without_a_gpu(monkeypatch):
+    """Moved, loaded by assignment or set: nothing keeps what the buffers were until the next call."""
+    from llada_quant_b200 import ops
+    monkeypatch.setattr(ops, "_need_cuda", lambda *ts: None)
+    fresh = linear_of("cpu")
+    for replace in (lambda m: m.to_empty(device="cpu"), lambda m: m.load_state_dict(fresh.state_dict(), assign=True),
+                    lambda m: [setattr(m, n, getattr(fresh, n).clone()) for n in ("qweight", "scale", "bias")]):
+        m = linear_of("cpu")
+        w = m._multiplier()
+        assert w is m._multiplier()
+        old = [weakref.ref(t) for t in (m.qweight, m.scale, m.bias, w.codes, w.scale, w.bias)]
+        del w
+        replace(m)
+        gc.collect()
+        assert all(r() is None for r in old)
+
+
+@pytest.mark.gpu
+def test_a_moved_module_gives_its_memory_back():
+    from llada_quant_b200.fp8 import Fp8Linear
+    m = Fp8Linear(4096, 4096).cuda()
+    x = torch.ones(1, 4096, dtype=torch.bfloat16, device="cuda")
+    y = m(x)
+    before = torch.cuda.memory_allocated()
+    m.cpu()
+    assert before - torch.cuda.memory_allocated() >= 4096 * 4096
+    assert torch.equal(m.cuda()(x), y)
