@@ -656,7 +656,7 @@ moe_few = torch.library.custom_op("llada_quant::moe_few", mutates_args=())(_moe_
 @moe_few.register_fake
 def _(x, gate_w, bias, renormalize, qw1, sw1, qw2, sw2, k, bits):
     T = x.shape[0]
-    return (torch.empty_like(x), x.new_empty(T, k, dtype=torch.float32), x.new_empty(T, k, dtype=torch.int32),
+    return (x.new_empty(x.shape), x.new_empty(T, k, dtype=torch.float32), x.new_empty(T, k, dtype=torch.int32),
             x.new_empty(T, gate_w.shape[0], dtype=torch.float32))
 
 
@@ -675,7 +675,7 @@ moe_few_routed = torch.library.custom_op("llada_quant::moe_few_routed", mutates_
 
 @moe_few_routed.register_fake
 def _(x, qw1, sw1, qw2, sw2, topk_w, topk_ids, bits):
-    return torch.empty_like(x)
+    return x.new_empty(x.shape)
 
 
 # ---------------------------------------------------------------------------

@@ -274,3 +274,70 @@ def test_a_moved_module_gives_its_memory_back():
     m.cpu()
     assert before - torch.cuda.memory_allocated() >= 4096 * 4096
     assert torch.equal(m.cuda()(x), y)
+
+
+# ---------------------------------------------------------------------------
+# registered operators
+# ---------------------------------------------------------------------------
+
+def operator_calls(device):
+    """name -> (operator, arguments), with x transposed, sliced or wide where a caller may have it so."""
+    from llada_quant_b200 import ops  # noqa: F401
+    from llada_quant_b200.fp8 import quantize_fp8
+    packed, x, gate, weights, ids = layer_parts(device)
+    p = (packed.qw1, packed.sw1, packed.qw2, packed.sw2)
+    calls = {}
+    wide = torch.zeros(4, 300, dtype=torch.bfloat16, device=device)
+    for name, v in (("plain", x), ("transposed", x.t().contiguous().t()), ("sliced", wide[:, 7:263])):
+        calls[f"moe_few {name}"] = (torch.ops.llada_quant.moe_few, (v, gate, None, True, *p, 2, 4))
+        calls[f"moe_few_routed {name}"] = (torch.ops.llada_quant.moe_few_routed, (v, *p, weights, ids, 4))
+        for rows in (1, 128):
+            calls[f"fp8_quantize {name} {rows}"] = (torch.ops.llada_quant.fp8_quantize, (v[:, :201], rows))
+        if device == "cuda":
+            w, q = quantize_fp8(gate, 128), quantize_fp8(v)
+            for out in (torch.bfloat16, torch.float32):
+                calls[f"fp8_linear values {name} {out}"] = (torch.ops.llada_quant.fp8_linear,
+                                                            (v, None, w.codes, w.scale, gate[:, 0].to(out), out))
+                calls[f"fp8_linear codes {name} {out}"] = (torch.ops.llada_quant.fp8_linear,
+                                                           (q.codes, q.scale, w.codes, w.scale, None, out))
+    return calls
+
+
+def test_fake_outputs_are_laid_out_like_the_real_ones():
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    calls = operator_calls("cpu")
+    with FakeTensorMode(allow_non_fake_inputs=True):
+        for name, (op, args) in calls.items():
+            out = op(*args)
+            for t in out if isinstance(out, tuple) else (out,):
+                assert t.stride(1) == 1 and t.stride(0) in (t.shape[1], -(-t.shape[1] // 16) * 16), name
+
+
+@pytest.mark.gpu
+def test_registered_operators_hold_to_their_contract():
+    """Fake outputs against real ones; schema and a traced graph where no tensor is float8, which those checks multiply."""
+    for name, (op, args) in operator_calls("cuda").items():
+        more = ("test_schema", "test_aot_dispatch_static") if name.startswith("moe") else ()
+        torch.library.opcheck(op.default, args, test_utils=("test_faketensor", *more))
+
+
+@pytest.mark.gpu
+def test_registered_operators_equal_the_python_entry_points():
+    from llada_quant_b200.few_tokens import FewTokenMoE
+    from llada_quant_b200.fp8 import Fp8Tensor, fp8_linear, quantize_fp8
+    packed, _, gate, _, _ = layer_parts("cuda")
+    moe = FewTokenMoE(packed, gate, 2, renormalize=True)
+    for name, (op, args) in operator_calls("cuda").items():
+        got, x = op(*args), args[0]
+        if name.startswith("moe_few_routed"):
+            want = (moe.routed(x, *args[5:7]),)
+        elif name.startswith("moe_few"):
+            want = moe.with_logits(x)
+        elif name.startswith("fp8_quantize"):
+            q = quantize_fp8(*args)
+            want, got = (q.codes.float(), q.scale), (got[0].float(), got[1])
+        else:
+            x = Fp8Tensor(x, args[1], 1) if args[1] is not None else x
+            want = (fp8_linear(x, Fp8Tensor(args[2], args[3], 128), args[4], args[5]),)
+        got = got if isinstance(got, tuple) else (got,)
+        assert all(torch.equal(a, b) for a, b in zip(got, want)) and len(got) == len(want), name
