@@ -339,7 +339,7 @@ typedef struct llq_few_layer {
  * rounding of each weight, router logits and h kept in fp32 accuracy, one
  * rounding of the result: close to, and more exact than, the calls for many
  * tokens, which round logits, weights and h to bf16.  logits float32 [T, E]
- * or NULL.  Ids outside [0, E) contribute nothing (experts of other ranks); an
+ * (before the bias, as theirs) or NULL.  Ids outside [0, E) contribute nothing (experts of other ranks); an
  * expert that appears twice in a token counts with the sum of its weights.
  * T <= 32, E <= 256, k <= 32, H and I in multiples of 32 up to 8192, a group
  * size in multiples of 128 or one scale per row (others: LLQ_EUNSUPPORTED).

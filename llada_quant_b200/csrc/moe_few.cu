@@ -389,10 +389,12 @@ __device__ void router_logits(const FewArgs& a, float (*red)[64][RED_PITCH], Log
   }
 }
 
+__device__ __forceinline__ float raw_logit(const LogitPart* parts, int e, int tok) {
+  return __fadd_rn(parts[0][tok][e], parts[1][tok][e]);
+}
 __device__ __forceinline__ float logit_of(const FewArgs& a, const LogitPart* parts, int e, int tok) {
-  float z = __fadd_rn(parts[0][tok][e], parts[1][tok][e]);
-  if (a.bias != nullptr) z = __fadd_rn(z, __ldg(a.bias + e));
-  return z;
+  const float z = raw_logit(parts, e, tok);
+  return a.bias != nullptr ? __fadd_rn(z, __ldg(a.bias + e)) : z;
 }
 
 // softmax and top-k of one token by one warp, 32 PER experts at most, into sm.ids, sm.w and sm.mask.  (Here and in all
@@ -560,7 +562,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       }
     }
     if (a.logits != nullptr && cta == grid - 1)
-      for (int i = threadIdx.x; i < a.T * a.E; i += THREADS) a.logits[i] = logit_of(a, parts, i % a.E, i / a.E);
+      for (int i = threadIdx.x; i < a.T * a.E; i += THREADS) a.logits[i] = raw_logit(parts, i % a.E, i / a.E);
     __syncthreads();
     if (cta == 0) {
       for (int i = threadIdx.x; i < a.T * a.k; i += THREADS) {

@@ -93,7 +93,8 @@ class FewTokenMoE:
         layer, held = self._layer()
         x, weights, ids = self._outputs(x)
         logits = torch.empty(x.shape[0], self.num_experts, dtype=torch.float32, device=self.device)
-        return ops.few_call(layer, x, weights, ids, logits), weights, ids, logits
+        out = ops.few_call(layer, x, weights, ids, logits)
+        return out, weights, ids, logits if self._bias is None else logits.add_(self._bias)
 
     def _outputs(self, x: torch.Tensor):
         if self._gate is None:

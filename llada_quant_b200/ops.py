@@ -636,7 +636,7 @@ def _moe_few_impl(x: torch.Tensor, gate_w: torch.Tensor, bias: Optional[torch.Te
                   qw1: torch.Tensor, sw1: torch.Tensor, qw2: torch.Tensor, sw2: torch.Tensor, k: int,
                   bits: int) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
     """Router + routed experts on PACKED weights for at most 32 tokens, two launches ->
-    (out bf16 [T,H], topk_w f32 [T,k], topk_ids i32 [T,k], logits f32 [T,E])."""
+    (out bf16 [T,H], topk_w f32 [T,k], topk_ids i32 [T,k], logits f32 [T,E] before the bias)."""
     _need_cuda(gate_w, bias)
     _no_grad_through("the few-token layer", gate_w, bias)
     gate_w = _aligned(gate_w)  # (held until the call: the layer has their addresses)

@@ -341,3 +341,26 @@ def test_registered_operators_equal_the_python_entry_points():
             want = (fp8_linear(x, Fp8Tensor(args[2], args[3], 128), args[4], args[5]),)
         got = got if isinstance(got, tuple) else (got,)
         assert all(torch.equal(a, b) for a, b in zip(got, want)) and len(got) == len(want), name
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bias_dtype", [torch.float32, torch.bfloat16])
+def test_captured_logits_are_those_before_the_bias(bias_dtype):
+    """As the layer for many tokens records them; with_logits adds the bias."""
+    from llada_quant_b200.few_tokens import FewTokenMoE
+    from llada_quant_b200.fused_moe import moe_layer
+    from llada_quant_b200.router_capture import RouterCapture
+    from tests.test_few_tokens import logits64
+    packed, x, gate, _, _ = layer_parts("cuda")
+    bias = torch.arange(8, device="cuda").to(bias_dtype)
+    bias[3] = -torch.inf
+    z, dz = logits64(x, gate, None)
+    for name, impl, step in (("few", "few", 0.0), ("many", "auto", 2.0 ** -8)):
+        cap = RouterCapture()
+        moe_layer(x, gate, packed, 2, bias, impl=impl, capture=cap, name=name)
+        off = (cap.gates[name].double().cuda() - z).abs()
+        assert bool((off <= dz + step * (z.abs() + dz)).all()), (name, off.max().item())
+    logits = FewTokenMoE(packed, gate, 2, bias).with_logits(x)[3].double()
+    zb, dzb = logits64(x, gate, bias)
+    assert bool((((logits - zb).abs() <= dzb) | (torch.isinf(zb) & (logits == zb))).all())
+    assert bool((logits[:, 3] == -torch.inf).all())
