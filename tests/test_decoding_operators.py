@@ -364,3 +364,49 @@ def test_captured_logits_are_those_before_the_bias(bias_dtype):
     zb, dzb = logits64(x, gate, bias)
     assert bool((((logits - zb).abs() <= dzb) | (torch.isinf(zb) & (logits == zb))).all())
     assert bool((logits[:, 3] == -torch.inf).all())
+
+
+# ---------------------------------------------------------------------------
+# quantizer and product through their module
+# ---------------------------------------------------------------------------
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M,K", [(1, 1), (1, 16), (3, 127), (5, 128), (129, 129)])
+@pytest.mark.parametrize("rows", [1, 128])
+def test_codes_have_their_shape_and_an_aligned_pitch(M, K, rows):
+    from llada_quant_b200.fp8 import quantize_fp8
+    q = quantize_fp8(torch.ones(M, K, device="cuda"), rows)
+    assert q.codes.shape == q.shape == (M, K) and q.scale.shape == (-(-M // rows), -(-K // 128))
+    assert M == 1 or q.codes.stride() == (-(-K // 16) * 16, 1)
+    assert bool((q.codes.float() == 448).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16, torch.float64])
+def test_from_linear_holds_the_quantized_weight_and_multiplies_by_it(dtype):
+    from llada_quant_b200.fp8 import Fp8Linear, quantize_fp8
+    from tests.test_fp8 import check_product, plain_quantize
+    g = torch.Generator().manual_seed(5)
+    lin = torch.nn.Linear(1040, 520, bias=True, dtype=dtype)
+    with torch.no_grad():
+        lin.weight.copy_(torch.randn(520, 1040, generator=g) * 0.02)
+        lin.bias.copy_((torch.randn(520, generator=g) * 0.1).bfloat16())  # exact in the module's type
+    m = Fp8Linear.from_linear(lin.cuda())
+    code, scale = plain_quantize(lin.weight.detach().float(), 128)
+    assert torch.equal(m.qweight.cpu(), code.view(torch.uint8)) and torch.equal(m.scale.cpu(), scale)
+    for M in (1, 6, 40):
+        x = torch.randn(M, 1040, generator=g).to(torch.bfloat16).cuda()
+        q = quantize_fp8(x)
+        check_product(m(x), q.codes, q.scale, m.weight, lin.bias.detach().bfloat16())
+        check_product(m(q), q.codes, q.scale, m.weight, lin.bias.detach().bfloat16())
+
+
+@pytest.mark.gpu
+def test_few_token_layer_without_tokens_records_nothing():
+    from llada_quant_b200.fused_moe import moe_layer
+    from llada_quant_b200.router_capture import RouterCapture
+    from llada_quant_b200.routing_stats import RoutingRecorder
+    packed, x, gate, _, _ = layer_parts("cuda")
+    rec, cap = RoutingRecorder(8, "cuda"), RouterCapture()
+    assert moe_layer(x[:0], gate, packed, 2, impl="few", recorder=rec, capture=cap, name="l").shape == (0, 256)
+    assert rec.stats().counts == [0] * 8 and cap.gates["l"].shape == (0, 8) and cap.topk_ids["l"].shape == (0, 2)
