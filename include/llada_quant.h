@@ -360,7 +360,9 @@ int llq_moe_few(const llq_few_layer* layer, const void* x, int64_t T, float* log
  * per 128 values of a row, block_rows == 128 one per 128 x 128 block; the last
  * block of a row or column may be short.  amax = max(|x| of the block,
  * 448 * 2^-60); scale [ceil(M / block_rows), ceil(K / 128)] = amax / 448; code =
- * nearest e4m3 (ties to even) to x * 448 / amax.  A NaN or an infinity makes
+ * nearest e4m3 (ties to even) to x * 448 / amax.  For float32 x the quotient is
+ * taken in fp32 steps (x * 0.4375 rounded, divided by amax * 2^-10, rounded), so an
+ * x within 2^-23 of the border between two codes may get either.  A NaN or an infinity makes
  * its block's products NaN.  codes: row pitch ldc bytes, base and pitch
  * multiples of 16; bytes past K are not written.
  */

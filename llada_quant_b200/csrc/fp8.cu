@@ -25,7 +25,8 @@ __device__ __forceinline__ float group_amax(uint32_t bits) {
 
 __device__ __forceinline__ float group_scale(float amax) { return __fdiv_rn(amax, 448.f); }
 
-// v * 448 / amax, correctly rounded in fp32; 448 = 0.4375 * 2^10, so that no product overflows
+// v * 448 / amax in fp32; 448 = 0.4375 * 2^10, so that no product overflows.  For bf16 and fp16 values the product is exact
+// and the quotient correctly rounded; for fp32 values both are rounded, so it is within 2^-23 of itself.
 __device__ __forceinline__ float ratio(float v, float amax) {
   return __fdiv_rn(__fmul_rn(v, 0.4375f), __fmul_rn(amax, 0x1p-10f));
 }

@@ -410,3 +410,26 @@ def test_few_token_layer_without_tokens_records_nothing():
     rec, cap = RoutingRecorder(8, "cuda"), RouterCapture()
     assert moe_layer(x[:0], gate, packed, 2, impl="few", recorder=rec, capture=cap, name="l").shape == (0, 256)
     assert rec.stats().counts == [0] * 8 and cap.gates["l"].shape == (0, 8) and cap.topk_ids["l"].shape == (0, 2)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [1, 128])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_codes_are_the_nearest_within_the_quotients_rounding(rows, dtype):
+    """In 64 bits: bf16 and fp16 exactly the nearest, fp32 up to 2^-23 of the value (two fp32 roundings)."""
+    from llada_quant_b200.fp8 import quantize_fp8
+    x = torch.randn(256, 1024, generator=torch.Generator("cuda").manual_seed(4), device="cuda")
+    x[:, ::128] = 4.0
+    # 448 x / 4 next to borders between codes, from both sides
+    edge = torch.tensor([(8 + m + 0.5) * 2.0 ** e / 112 for e in range(-9, 4) for m in range(8)], device="cuda")
+    for i in range(64):
+        x[i, 1:1 + edge.numel()] = edge * (1 + (i - 32) * 2.0 ** -24)
+    x[128, :128] = 0.9962565898895264 / 4
+    x[128, :2] = torch.tensor([0.9962565898895264, 4.1261671867687255e-05], device="cuda")
+    x = x.to(dtype)
+    q = quantize_fp8(x, rows)
+    amax = x.double().view(256 // rows, rows, 8, 128).abs().amax((1, 3))
+    v = x.double() * 448 / amax.repeat_interleave(rows, 0).repeat_interleave(128, 1)
+    step = torch.exp2(torch.floor(torch.log2(v.abs().clamp(min=2.0 ** -6))) - 3)
+    slack = 2.0 ** -23 if dtype == torch.float32 else 0.0
+    assert bool(((q.codes.double() - v).abs() <= step / 2 + (slack + 2.0 ** -50) * v.abs()).all())
