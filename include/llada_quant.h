@@ -341,7 +341,7 @@ typedef struct llq_few_layer {
  * tokens, which round logits, weights and h to bf16.  logits float32 [T, E]
  * (before the bias, as theirs) or NULL.  Ids outside [0, E) contribute nothing (experts of other ranks); an
  * expert that appears twice in a token counts with the sum of its weights.
- * T <= 32, E <= 256, k <= 32, H and I in multiples of 32 up to 8192, a group
+ * T <= 32, E <= 256, k <= 32 and k <= E, H and I in multiples of 32 up to 8192, a group
  * size in multiples of 128 or one scale per row (others: LLQ_EUNSUPPORTED).
  * workspace: llq_moe_few_workspace_size bytes, of this call alone until it is
  * done on the stream.

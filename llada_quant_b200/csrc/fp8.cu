@@ -56,9 +56,9 @@ __device__ __forceinline__ uint16_t to_e4m3x2(float lo, float hi) {
   return r;
 }
 
-// The codes of N values of type T of a group: e4m3 of ratio(v).  (A division for each value took 42 us at 8192 x 4096
-// bf16 where this took 28 then, and a test for borders with the division behind it 50: a quarter of all groups of bf16
-// values has some on one.)
+// The codes of N values of type T of a group: e4m3 of ratio(v).  (With a division for each value 8192 x 4096 bf16
+// takes 27.4 us, with this 18.4; fp32 28.8 both.  A test for borders with the division behind it is slower than either for
+// bf16: a quarter of all groups has some on one.)
 template <typename T, int N>
 __device__ __forceinline__ void quantize_values(const float (&v)[N], float amax, const Divider& div, uint16_t (&q)[N / 2]) {
   uint32_t differ = 0;
@@ -182,11 +182,11 @@ struct Raw16 {
 // It has to read 2 (4) bytes a value and write 1; what holds it below the memory's rate is that a warp computes while it
 // has no load under way, about 6 instructions a value, so many warps and few instructions are wanted: 8192 x 4096 bf16
 // takes 18.4 us at 6 CTAs per SM (5.5 TB/s), 19.1 at 5 and 19.7 at 7; with a division per group for its row 19.6, and asking for the
-// next group ahead took 25.8 where this took 21.8.  fp32: 28.8 us at 5 CTAs (5.8 TB/s), 30.0 at 4, 31.6 at 6.
+// next group ahead costs a fifth, in registers.  fp32: 28.8 us at 5 CTAs (5.8 TB/s), 30.0 at 4, 31.6 at 6.
 template <typename T>
 constexpr int kRowsBlocks = sizeof(T) == 4 ? 5 : 6;
-// the same for blocks of 128 rows: 4096 x 8192 bf16 18.7 us at 4 CTAs per SM (5.4 TB/s); before the values took fewer
-// instructions 20.2, and then 23.9 at 5, 26.9 at 6 and 21.3 at 3
+// the same for blocks of 128 rows: 4096 x 8192 bf16 18.7 us at 4 CTAs per SM (5.4 TB/s), 19.7 at 3, 22.9 at 5, 25.7 at 6;
+// fp32 35.7 at 2 (4.7 TB/s), 35.4 at 1, 41.6 at 3, 49.3 at 4, and 1000 x 2048 4.5 at 2 and 1, 5.2 at 3
 template <typename T>
 constexpr int kBlocksBlocks = sizeof(T) == 4 ? 2 : 4;
 
@@ -318,8 +318,8 @@ struct Codes {};  // tag: x holds e4m3 codes
 // exact and sums are fp32.  The order of K within a group is free as long as both sides agree: lane t of a quad
 // has bytes 16 t and 64 + 16 t of a group's 128, so that a quad reads 64 bytes at once.
 // T other than Codes (NB = 1): every CTA quantizes the rows for itself into shared memory, which saves a launch.
-// The weight's bytes bound it, with a start of about 2 us: 8 x 8192 x 4096 takes 8.6 us (3.9 TB/s), 8 x 4096 x 14336 12.5 (4.7
-// TB/s), one token 2048 x 2048 with its quantization 2.7.
+// The weight's bytes bound it, with a start of about 2 us: 8 x 8192 x 4096 takes 8.5 us (4.0 TB/s), 8 x 4096 x 14336 12.5 (4.7
+// TB/s), both with weights from HBM; one token 2048 x 2048 with its quantization 2.5 with weights in L2, 3.2 from HBM.
 template <int W, int NB>
 constexpr int kFewRed = W * 16 * (NB * 8 + 1) * 4;
 
@@ -508,10 +508,10 @@ int fp8_quantize(const void* x, int x_dtype, int64_t M, int64_t K, int64_t ldx, 
   return fail(LLQ_EUNSUPPORTED, "unknown dtype %d", x_dtype);
 }
 
-// Does the product run on fp8_few_rows_kernel (else on fp8_tc_kernel)?  Up to 16 rows it is faster, or as fast with large
-// weights (us: 8 x 2048 x 2048 2.4 against 6.4, 8 x 8192 x 4096 8.6 against 11, 16 x 4096 x 4096 6.9 against 10.3, 16 x 8192 x 4096 12.0
+// Does the product run on fp8_few_rows_kernel (else on fp8_tc_kernel)?  Up to 8 rows it is faster, from 9 to 16 with all but the
+// largest weights, where the rule costs up to 9 % (us: 8 x 2048 x 2048 2.4 against 6.4, 8 x 8192 x 4096 8.6 against 11, 16 x 4096 x 4096 6.9 against 10.3, 16 x 8192 x 4096 12.0
 // against 11.0, 16 x 4096 x 14336 17.2 against 18.2); with 32, where a CTA reads more of x than of the weight, for few
-// and small weight rows (32 x 2048 x 2048 4.4 against 6.4, 32 x 2048 x 4096 7.2 against 8.1, 32 x 4096 x 2048 6.7 against 6.4, 32 x
+// and small weight rows, at the end of that range 5 % slower (32 x 2048 x 2048 4.4 against 6.4, 32 x 2048 x 4096 7.2 against 8.1, 32 x 4096 x 2048 6.7 against 6.4, 32 x
 // 8192 x 1024 7.9 against 4.7, 32 x 8192 x 4096 18.5 against 11.0).
 static bool few_rows(int64_t M, int64_t K, int64_t N) { return M <= 16 || (M <= 32 && N <= 4096 && N * K <= 1 << 24); }
 

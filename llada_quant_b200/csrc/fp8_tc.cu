@@ -17,9 +17,10 @@
 // What bounds a large product is the chain of these hand-overs: of about 950 cycles that 128 x 256 x 128 takes, the tensor
 // core works 510 and the epilogue's threads 600 (its reads of TMEM and its 128 sums are 256 each), and they overlap
 // only as far as two accumulator buffers let them.  So a thread asks for its next 32 columns before it adds the last,
-// which takes 216 registers at BN = 256.  8192 x 8192 x 2048: 140 us, 1.96 PFLOP/s.  Tried and not better: fma.rn.f32x2
-// for the sums (three instructions a pair, 176 us against 170 then), three column parts of 64 at BN = 192 (147 against 136), a pair of
-// CTAs on 256 x 256 (cta_group::2, 130 against 136, and 21 against 19.9 at 1024 x 4096 x 4096).
+// which takes 216 registers at BN = 256.  8192 x 8192 x 2048: 140 us, 1.96 PFLOP/s, at the full clock (call after call the
+// card's power limit holds it at 1.5 GHz and 165 us).  Other forms: fma.rn.f32x2 for the sums (three instructions a pair) 4 %
+// slower, three column parts of 64 at BN = 192 8 %; a pair of CTAs on 256 x 256 (cta_group::2) 4 % faster there, 6 % slower at
+// 1024 x 4096 x 4096, and not built in.
 // Persistent over tiles when K is not split.  When the tiles do not cover the SMs, a cluster of `split`
 // CTAs shares one tile, each takes a part of K, and the parts meet in distributed shared memory and are
 // added in rank order.
@@ -284,7 +285,7 @@ __global__ void __launch_bounds__(F8Cfg<BN>::THREADS, 1)
     bool ok = true;
     for (int u = blockIdx.x / a.split; u < a.tiles && ok; u += stride) {
       const int64_t m = static_cast<int64_t>(u % a.mtiles) * BM + r0;
-      const float* p0 = a.xs + (m < a.M ? m : 0) * a.G;  // rows behind the last are zero, whatever scales them
+      const float* p0 = a.xs + (m < a.M ? m : 0) * a.G;  // rows behind the last are not stored, whatever scales them
       const float* p1 = a.xs + (m + 32 < a.M ? m + 32 : 0) * a.G;
       auto fetch = [&](const float* p, int g) {
         if (vec && g < g1) return __ldg(reinterpret_cast<const float4*>(p + g));

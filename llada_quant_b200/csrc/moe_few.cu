@@ -25,16 +25,17 @@
 // magnitude lies in [2^14, 2^15): exact for every bf16 value within 2^-31 of the largest, and what is
 // lost below is 2^-40 of it.  (fp16 rather than bf16 because its ten mantissa bits take an INT8 code, or
 // the upper nibble of a byte, where it lies: 40 instead of 56 logic instructions per lane and 128-group at
-// INT4, 48 instead of 96 at INT8; the logic pipe is what bounds the arithmetic.)  h travels between the
+// INT4, 48 instead of 96 at INT8.)  h travels between the
 // kernels as three bf16 numbers that add up to the fp32 value (8 + 8 + 8 significant bits; the third is short only
 // where h lies below 2^-110).  So no MMA adds a visible rounding: the layer rounds once, at its end.
 //
-// The packed bytes and their scales reach shared memory by TMA (swizzled) into rings that are deep
-// enough for HBM's latency; the tokens lie in shared memory in MMA order.  Measured on the way
-// (32 tokens, INT4, both kernels): lanes loading their own bytes with cp.async and their tokens from L1,
-// 132 us, bound by the L1 wavefronts that eight scattered rows per instruction cost; a register ring
-// unrolled over its slots, 527 us, its code larger than the instruction cache; TMA rings whose refill the
-// computing warps issued themselves, 87 us (a copy holds its warp up for hundreds of cycles).
+// The packed bytes reach shared memory by TMA (swizzled) into rings that are deep enough for HBM's latency;
+// their scales go from global memory to registers, up to eight steps ahead (RowScales); the tokens lie in
+// shared memory in MMA order.  Other forms (32 tokens, INT4, both kernels, where this takes 83 us): lanes loading their
+// own bytes with cp.async and their tokens from L1, 132 us, bound by the L1 wavefronts that eight scattered
+// rows per instruction cost; a register ring unrolled over its slots, 527 us, its code larger than the
+// instruction cache; rings whose refill the computing warps issue themselves, 4 us more (a copy holds its
+// warp up for hundreds of cycles).
 #include <algorithm>
 
 #include <cooperative_groups.h>
@@ -517,8 +518,9 @@ __device__ __forceinline__ void emit(const FewArgs& a, const Segment& sg, const 
 }
 
 // Router, top-k, segments and GEMM1.  32 tokens of a 64 x 2048 x 1024, top-8 INT4 layer: 17 us until the first product
-// (router 8, top-k and segments 4, tokens 4), then 31 us for 135 MB (4.3 TB/s), where the warps issue in two of three
-// cycles: 9 instructions turn 8 INT4 codes into fp16 pairs.  One token: 9 us, then 7.
+// (router 8, top-k and segments 4, tokens 4), then 31 us for 135 MB (4.3 TB/s): over the whole kernel the warps issue in 47 %
+// of the cycles (9 instructions turn 8 INT4 codes into fp16 pairs) and otherwise wait, for scales first, then for the
+// chain of a step's MMAs; four warps a scheduler are too few to cover for one another.  One token: 9 us, then 7.
 template <int BITS, bool V4>
 __global__ void __launch_bounds__(THREADS, 1)
     few_gemm1_kernel(const __grid_constant__ CUtensorMap tm_w, const FewArgs a) {
@@ -888,8 +890,8 @@ struct Smem2 {
   int last;
 };
 
-// GEMM2 and the combine.  The same layer: 22 us for 71 MB at 32 tokens (issue again: up to three MMAs for h's three parts), then
-// 5 for the outputs' parts; one token 3 and 4.  All of it: 32 tokens 83 us (INT8 105), one token 26 (INT8 30), 8 tokens INT8
+// GEMM2 and the combine.  The same layer: 22 us for 71 MB at 32 tokens (waits and issue, 47 %, again: up to three MMAs for h's three
+// parts), then 5 for the outputs' parts; one token 3 and 4.  All of it: 32 tokens 83 us (INT8 105), one token 26 (INT8 30), 8 tokens INT8
 // with given routing 66 (4.1 TB/s).  (With two parts of h, 16 bits of it, 81 (105), 26 (30) and 67.)
 template <int BITS, bool V4>
 __global__ void __launch_bounds__(THREADS2, 1)

@@ -27,7 +27,7 @@ from .moe import PackedExperts
 class FewTokenMoE:
     """One packed layer, checked once; calls then cost two launches and little host time.
 
-    ``gate_w`` bf16 ``[E, H]`` (may be None for :meth:`routed` alone), ``bias`` fp32 ``[E]`` added to
+    ``top_k`` is at most E.  ``gate_w`` bf16 ``[E, H]`` (may be None for :meth:`routed` alone), ``bias`` fp32 ``[E]`` added to
     the logits (``-inf`` bars an expert), ``renormalize`` divides a token's weights by their sum.
     Calls see what the operands hold at the call.  A gate_w that is not contiguous and 16-byte aligned,
     and a bias of another type, are copied for every call.

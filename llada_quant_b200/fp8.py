@@ -81,7 +81,9 @@ class Fp8Linear(nn.Module):
     hold at the call; a bias of another type, or a buffer that is not contiguous and 16-byte aligned, is
     copied for every call.
 
-    The buffers are bytes, not float8, so that ``module.half()`` and the like leave them alone.
+    The codes are bytes, not float8, so that ``module.half()`` and the like leave them alone.  ``scale`` they
+    round, and a scale that is not fp32 is refused: cast a model before its layers are quantized, or load the
+    scales again after it.
     """
 
     def __init__(self, in_features: int, out_features: int, bias: bool = False,
