@@ -25,20 +25,23 @@ from .moe import PackedExperts
 
 
 class FewTokenMoE:
-    """One packed layer, checked once; calls then cost two launches and little host time.
+    """One packed layer, checked when it is made; calls then cost two launches and little host time.
 
-    ``top_k`` is at most E.  ``gate_w`` bf16 ``[E, H]`` (may be None for :meth:`routed` alone), ``bias`` fp32 ``[E]`` added to
-    the logits (``-inf`` bars an expert), ``renormalize`` divides a token's weights by their sum.
+    ``top_k`` is at most E.  ``gate_w`` bf16 ``[E, H]`` (may be None for :meth:`routed` alone), ``bias``
+    fp32 ``[E]`` added to the logits (``-inf`` bars an expert), ``renormalize`` divides a token's weights
+    by their sum.
+
     Calls see what the operands hold at the call.  A gate_w that is not contiguous and 16-byte aligned,
-    and a bias of another type, are copied for every call.
-    An operand whose memory was exchanged (``module.to()``, ``parameter.data = ...``) is seen by the
-    next call, which checks all of them again; until then the layer holds the memory that they had.
+    and a bias of another type, are copied for every call.  An operand whose memory was exchanged
+    (``module.to()``, ``parameter.data = ...``) is seen by the next call, which checks all of them again;
+    until then the layer holds the memory that they had.
     """
 
     def __init__(self, packed: PackedExperts, gate_w: Optional[torch.Tensor], top_k: int,
                  bias: Optional[torch.Tensor] = None, renormalize: bool = False) -> None:
         if not 1 <= top_k <= packed.num_experts:
             raise ValueError(f"top_k must be 1 to {packed.num_experts}, got {top_k}")
+        ops._no_grad_through("the few-token layer", gate_w, bias)
         self.top_k, self._renormalize = top_k, renormalize
         self._packed, self._gate, self._bias = packed, gate_w, bias
         given = (packed.qw1, packed.sw1, packed.qw2, packed.sw2, gate_w, bias)
@@ -64,10 +67,9 @@ class FewTokenMoE:
 
     def _router(self) -> tuple:
         """The layer's descriptor, and the copies that it points at where gate_w or bias cannot be read as it is."""
-        p, gate_w, bias = self._packed, self._gate, self._bias
-        ops._no_grad_through("the few-token layer", gate_w, bias)
-        gate_w = ops._aligned(gate_w)
-        bias = None if bias is None else bias.to(torch.float32).contiguous()
+        p = self._packed
+        gate_w = ops._aligned(self._gate.detach())
+        bias = None if self._bias is None else self._bias.detach().to(torch.float32).contiguous()
         layer = ops.few_layer(p.qw1, p.sw1, p.qw2, p.sw2, self.top_k, p.bits, gate_w, bias, self._renormalize)
         pairs = ((gate_w, self._gate), (bias, self._bias))
         return layer, [t for t, given in pairs if t is not None and t.data_ptr() != given.data_ptr()]
@@ -94,7 +96,7 @@ class FewTokenMoE:
         x, weights, ids = self._outputs(x)
         logits = torch.empty(x.shape[0], self.num_experts, dtype=torch.float32, device=self.device)
         out = ops.few_call(layer, x, weights, ids, logits)
-        return out, weights, ids, logits if self._bias is None else logits.add_(self._bias)
+        return out, weights, ids, logits if self._bias is None else logits.add_(self._bias.detach())
 
     def _outputs(self, x: torch.Tensor):
         if self._gate is None:

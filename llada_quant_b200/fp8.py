@@ -48,7 +48,8 @@ def quantize_fp8(x: torch.Tensor, block_rows: int = 1) -> Fp8Tensor:
 
     ``scale = amax / 448`` of the block and ``code`` the e4m3 nearest to ``x * 448 / amax`` (ties to
     even); amax is taken as at least ``448 * 2**-60``.  For fp32 values the quotient is that of fp32
-    steps, within ``2**-23`` of it, so a value that close to the border of two codes may get either.  A block with a NaN or an infinity dequantizes to NaN.
+    steps, within ``2**-23`` of it, so a value that close to the border of two codes may get either.  A block
+    with a NaN or an infinity dequantizes to NaN.
     """
     codes, scale = ops._fp8_quantize_impl(x, block_rows)
     return Fp8Tensor(codes, scale, block_rows)

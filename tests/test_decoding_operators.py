@@ -60,6 +60,26 @@ def test_an_infinite_h_of_one_or_two_tokens_stays_infinite(T, bits):
     assert bool((out == float("inf")).all())
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("T", [1, 2, 3, 4, 5, 12, 32])
+@pytest.mark.parametrize("bits", [4, 8])
+def test_what_the_workspace_held_before_does_not_count(T, bits):
+    """Every byte set: NaN in each place of h and of the partial sums that the call does not write."""
+    from llada_quant_b200 import _lib, ops
+    from llada_quant_b200.few_tokens import FewTokenMoE
+    from tests.test_few_tokens import check, make_layer, packed_of
+    layer, x, _, weights, ids = make_layer(T, 3, 160, 352, 2, bits, -1)
+    want = FewTokenMoE(packed_of(layer, -1), None, 2).routed(x, weights, ids)
+    check(want, x, layer, weights, ids)
+    lib, desc = _lib.load(), ops.few_layer(*layer[:4], 2, bits)
+    nbytes = lib.llq_moe_few_workspace_size(T, 2, 3, 160, 352)
+    ws = torch.full((nbytes + 256,), 0xFF, dtype=torch.uint8, device="cuda")
+    out = torch.full_like(x, float("nan"))
+    _lib.check(lib.llq_moe_few(ctypes.byref(desc), x.data_ptr(), T, None, weights.data_ptr(), ids.data_ptr(), out.data_ptr(),
+                               ws.data_ptr(), nbytes, ops._stream(x)))
+    assert torch.equal(out, want) and bool((ws[nbytes:] == 0xFF).all())
+
+
 # ---------------------------------------------------------------------------
 # operands that change between calls
 # ---------------------------------------------------------------------------
@@ -364,6 +384,9 @@ def test_captured_logits_are_those_before_the_bias(bias_dtype):
     zb, dzb = logits64(x, gate, bias)
     assert bool((((logits - zb).abs() <= dzb) | (torch.isinf(zb) & (logits == zb))).all())
     assert bool((logits[:, 3] == -torch.inf).all())
+    with torch.no_grad():
+        moe = FewTokenMoE(packed, gate, 2, bias.clone().requires_grad_())
+    assert not moe.with_logits(x)[3].requires_grad
 
 
 # ---------------------------------------------------------------------------
