@@ -53,7 +53,7 @@ struct F8Cfg {
   static constexpr int FIRST_EPI = 4;
   static constexpr int THREADS = (FIRST_EPI + EPI_WARPS) * 32;
   static constexpr int OUT_BYTES = EPI_WARPS * 4096;  // per warp twice 32 rows of 64 bytes
-  static constexpr int HEAD_BYTES = 3072;  // barriers (1 KB) and the rows' scales, one vector per accumulator buffer
+  static constexpr int HEAD_BYTES = 3 * 1024;  // barriers (1 KB) and the rows' scales, one vector per accumulator buffer
   static constexpr int STAGES = (232448 - HEAD_BYTES - OUT_BYTES) / STAGE_BYTES;
   static constexpr size_t SMEM_BYTES = HEAD_BYTES + static_cast<size_t>(STAGES) * STAGE_BYTES + OUT_BYTES;
   static_assert(1024 + ACC_BUFS * BM * 4 <= HEAD_BYTES, "head");
